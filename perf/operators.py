@@ -304,7 +304,7 @@ def _run_verify(s):
     n, most, vocab = c["seqs"], c["draft"], c["vocab"]
     off, draft, target, q = s["off"], s["draft"], s["target"], s["q"]
     if own:
-        _ctx().verify_draft(draft.data_ptr(), off.data_ptr(), n, most, target.data_ptr(), _CODE[c["dtype"]], vocab,
+        _ctx().verify_draft(draft.data_ptr(), off.data_ptr(), n, draft.numel(), most, target.data_ptr(), _CODE[c["dtype"]], vocab,
                             q.data_ptr() if q is not None else None, vocab, vocab, s["u_accept"].data_ptr(), s["u_draw"].data_ptr(),
                             s["out"].data_ptr(), s["accepted"].data_ptr(), s["work"].data_ptr(), s["work"].numel())
         return {"tokens": s["out"], "accepted": s["accepted"]}
