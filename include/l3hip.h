@@ -148,6 +148,93 @@ int l3_timing_totals(l3_ctx* ctx, double* ms, int cap, uint64_t* calls);
  * and more that no cut divides) */
 int l3_last_counters(l3_ctx* ctx, uint64_t* out, int cap);
 
+/* ---- operators on token ids: what stands on either side of a model ------------------------------------------------------
+ * NO COUNTERPART IN THE REFERENCE, which ends at the ids.  They take the ids and offsets the encode calls leave in HBM and
+ * give ids that l3_decode_batch takes (-1, like every id outside the vocabulary, decodes to nothing):
+ *   training   encode -> l3_embed -> model -> l3_embed_grad
+ *   serving    encode -> l3_cache_slots -> l3_embed -> model -> l3_verify_draft -> l3_cache_trim -> decode
+ * All pointers named d_* are DEVICE memory of the context's GPU.  The calls queue kernels on `stream` and return without
+ * waiting; there is no ticket, so `stream` is always the caller's: NULL is HIP's null stream (and not, as in the encode
+ * calls, a stream of the context).  They allocate nothing, keep nothing in the context, call nothing a stream capture forbids,
+ * leave the current device as it was, and may run at the same time on several streams and threads, each with a workspace of
+ * its own.  Workspaces need not be cleared, are aligned to 16 bytes and may be used again by the next call on the same
+ * stream; two captured graphs that may run at the same time need two.  Outputs must not overlap inputs unless said so.
+ * What the host can see is refused with L3_E_INVALID_ARG before anything is queued; what only the device can see is answered as
+ * each call says.  Strides are in elements, at least the row's length, and need no alignment beyond the element's own. */
+#define L3_F32 0
+#define L3_F16 1
+#define L3_BF16 2
+
+/* out[t] = scale * table[ids[t]] for t < n_ids, rounded once to out_type (products in 32 bits).  An id outside [0, n_rows),
+ * such as the pad -1, gives a row of zeros.  d_n_ids (may be NULL): only the first min(n_ids, *d_n_ids) ids count, rows behind
+ * them are left as they were -- d_out_off + n_docs of an encode call is such a number. */
+int l3_embed(l3_ctx* ctx, const int32_t* d_ids, uint64_t n_ids, const uint64_t* d_n_ids, const void* d_table, int table_type,
+             uint64_t n_rows, uint64_t dim, uint64_t table_stride, float scale, void* d_out, int out_type, uint64_t out_stride,
+             void* stream);
+
+/* The gradient of l3_embed with respect to its table: G[v] = scale * sum of grad[t] over the t with ids[t] = v, by sorted ids,
+ * summed in 32 bits in a fixed order (the same inputs give the same bits).
+ * accumulate = 1: table[v] = table[v] + G[v] for the rows that occur, rounded once; other rows are not touched.
+ * accumulate = 0: table = G, rows that do not occur become zero.
+ * Ids outside [0, n_rows) and ids behind *d_n_ids take no part.  d_work: l3_embed_grad_workspace(n_ids, dim) bytes (0: the
+ * sizes are out of range). */
+uint64_t l3_embed_grad_workspace(uint64_t n_ids, uint64_t dim);
+int l3_embed_grad(l3_ctx* ctx, const int32_t* d_ids, uint64_t n_ids, const uint64_t* d_n_ids, const void* d_grad, int grad_type,
+                  uint64_t grad_stride, uint64_t n_rows, uint64_t dim, float scale, void* d_table, int table_type,
+                  uint64_t table_stride, int accumulate, void* d_work, uint64_t work_bytes, void* stream);
+
+/* A paged cache of n_pages pages of page_size tokens, for n_seqs requests.  Request i holds the pages table[i][0 .. held[i])
+ * (rows table_stride apart, max_pages entries) and has len[i] tokens on them; entries behind held[i] mean nothing.  The pool is
+ * a stack: free[0 .. *n_free), room for n_pages.
+ *
+ * l3_cache_slots: new_off[i+1] - new_off[i] tokens are new to request i (n_seqs + 1 offsets: d_out_off of an encode call, or
+ * 0, 1, 2, .. for a step of one token each).  Pages that are missing are taken off the end of the pool, in order of the
+ * requests, and entered in the table.  The j-th new token of request i, at t = new_off[i] + j, gets pos[t] = len[i] + j and
+ * slots[t] = table[i][pos / page_size] * page_size + pos % page_size.  len_out, held_out and n_free_out are the state behind
+ * the step.  Slots and positions at or behind new_off[n_seqs] (there are cap of them) are left as they were.
+ * l3_cache_trim: request i keeps its first min(keep[i], len[i]) tokens and the pages these need; the others go to the end of
+ * the pool, in order of the requests.  keep[i] < 0: the request is left as it is.
+ *
+ * The *_out arrays may be the arrays they replace (all the same for n_free).  *d_status: 0, or what kept requests from being
+ * served -- such a request keeps its state, and its tokens get the slot and position -1:
+ *   L3_CACHE_POOL  the pool ran short: no page is left for this request or, where pages are needed, any behind it (trim: the
+ *                  pool would hold more than n_pages)
+ *   L3_CACHE_ROW   more tokens than max_pages pages, or 2^31 - 1, hold
+ *   L3_CACHE_BAD   new_off descends or ends behind cap; len, held or *n_free is negative, or more than there can be
+ *   L3_CACHE_PAGE  (slots) a page outside [0, n_pages): the slots of the tokens on it are -1, nothing else changes
+ * d_work: l3_cache_workspace(n_seqs) bytes.  n_seqs <= 2^20. */
+#define L3_CACHE_POOL 1u
+#define L3_CACHE_ROW 2u
+#define L3_CACHE_BAD 4u
+#define L3_CACHE_PAGE 8u
+uint64_t l3_cache_workspace(uint64_t n_seqs);
+int l3_cache_slots(l3_ctx* ctx, const uint64_t* d_new_off, uint64_t n_seqs, const int32_t* d_len, const int32_t* d_held,
+                   uint32_t page_size, uint32_t n_pages, int32_t* d_table, uint64_t table_stride, uint64_t max_pages,
+                   const int32_t* d_free, const int32_t* d_n_free, int32_t* d_len_out, int32_t* d_held_out, int32_t* d_n_free_out,
+                   int64_t* d_slots, int32_t* d_pos, uint64_t cap, uint32_t* d_status, void* d_work, uint64_t work_bytes, void* stream);
+int l3_cache_trim(l3_ctx* ctx, const int32_t* d_keep, uint64_t n_seqs, const int32_t* d_len, const int32_t* d_held, uint32_t page_size,
+                  uint32_t n_pages, const int32_t* d_table, uint64_t table_stride, uint64_t max_pages, int32_t* d_free,
+                  const int32_t* d_n_free, int32_t* d_len_out, int32_t* d_held_out, int32_t* d_n_free_out, uint32_t* d_status,
+                  void* d_work, uint64_t work_bytes, void* stream);
+
+/* Verification of drafted tokens.  Request i drafted draft[draft_off[i] .. draft_off[i+1]), k of them (k <= max_draft; n_draft is
+ * the length of draft and u_accept).  target has a row of `vocab` probabilities for each drafted token and one more for each
+ * request: the rows draft_off[i] + i + (0 .. k) are request i's.  draft_probs has the rows draft_off[i] + (0 .. k - 1); NULL:
+ * the tokens were drafted with certainty.  u_accept (one per drafted token) and u_draw (one per request) are in [0, 1).
+ *   token j is accepted while u_accept[j] * q_j(d_j) < p_j(d_j), up to the first that is not;
+ *   then one token is drawn: the smallest v with w(0) + .. + w(v) > u_draw * (w(0) + .. + w(vocab - 1)), where w is
+ *   max(p - q, 0) of the rejected token's rows (without draft_probs: p without the rejected token), or p_k if all were accepted.
+ * out[i] (max_draft + 1 entries): the accepted tokens, the drawn one, then -1; accepted[i]: how many were accepted.
+ * Comparisons, differences and sums are in 64 bits.  A weight that is negative, infinite or NaN counts as 0; where max(p - q, 0)
+ * is 0 throughout, p takes its place; where that is 0 throughout too, the drawn token is -1.  A drafted token outside
+ * [0, vocab) is rejected.  A request whose offsets descend, pass n_draft or hold more than max_draft tokens gets accepted = -1
+ * and a row of -1.  d_work: l3_verify_workspace(n_seqs, vocab) bytes. */
+uint64_t l3_verify_workspace(uint64_t n_seqs, uint64_t vocab);
+int l3_verify_draft(l3_ctx* ctx, const int32_t* d_draft, const uint64_t* d_draft_off, uint64_t n_seqs, uint64_t n_draft,
+                    uint32_t max_draft, const void* d_target, int type, uint64_t target_stride, const void* d_draft_probs,
+                    uint64_t draft_stride, uint64_t vocab, const float* d_u_accept, const float* d_u_draw, int32_t* d_out,
+                    int32_t* d_accepted, void* d_work, uint64_t work_bytes, void* stream);
+
 /* ---- several GPUs behind one handle --------------------------------------------------------------------------------
  * NO COUNTERPART IN THE REFERENCE (its only concurrent workload is goroutines calling Encode on one Tokenizer,
  * benchmark_test.go:151-174).  One context per entry of devices[] (a device may be named more than once); a batch is cut

@@ -1,0 +1,775 @@
+"""The operators on token ids on the GPU, through the C ABI, against plain statements in 64 bits (tests/token_ops_ref.py).
+
+Tolerances, from arithmetic.  With u = 2^-24 (half a step of 32 bits) and h = half a step of the stored type (2^-24 / 2^-11 /
+2^-8), s the spacing of the type's subnormal numbers:
+  lookup     one product in 32 bits, one rounding:          |x| (u + h) (1 + 2u) + s / 2 + 2^-149
+  gradient   m terms, any order, then scale and the old value: m + 2 roundings of partial results none of which is larger than
+             A = |old| + scale * sum |g|:                   (m + 2) u A (1 + (m + 2) u) + h |x| + s / 2 + 2^-149
+Whole numbers are equal."""
+import numpy as np
+import pytest
+
+from tests import corpus, token_ops_ref as ref
+from tests.test_token_ops_host import random_cache
+from tokenizer_amd import capi
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = capi.L3_F32, capi.L3_F16, capi.L3_BF16
+HALF = {F32: 2.0 ** -24, F16: 2.0 ** -11, BF16: 2.0 ** -8}
+STEP0 = {F32: 2.0 ** -149, F16: 2.0 ** -24, BF16: 2.0 ** -133}
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = capi.Context(device=0)
+    yield c
+    c.close()
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+    return torch
+
+
+def _t(torch, code):
+    return {F32: torch.float32, F16: torch.float16, BF16: torch.bfloat16}[code]
+
+
+def _matrix(torch, values, code, stride, shift=0, fill=0.0):
+    """float64 (n, d) -> (what the GPU holds as float64, the buffer, pointer of the first element); `shift` elements off an aligned address"""
+    n, d = values.shape
+    buf = torch.full((shift + n * stride + 8,), fill, dtype=_t(torch, code), device="cuda")
+    view = buf[shift:shift + n * stride].view(n, stride)[:, :d]
+    view.copy_(torch.from_numpy(values).cuda())
+    return view.double().cpu().numpy(), buf, buf.data_ptr() + shift * buf.element_size(), view
+
+
+def _ids(rng, n, rows):
+    ids = rng.integers(0, rows, n)
+    odd = rng.random(n) < 0.15
+    ids[odd] = rng.choice([-1, rows, -2 ** 31, 2 ** 31 - 1], int(odd.sum()))
+    return ids.astype(np.int32)
+
+
+# ---- lookup -------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("n", [1, 2, 63, 64, 65, 517])
+@pytest.mark.parametrize("dim", [1, 7, 8, 9, 64, 511, 513, 1001, 2048])
+def test_embed_sizes(ctx, torch, n, dim):
+    rng = np.random.default_rng(n * 10007 + dim)
+    types = [F32, F16, BF16]
+    T, O = types[(n + dim) % 3], types[(n * 3 + dim // 2) % 3]
+    _embed_case(ctx, torch, rng, n, dim, T, O, rows=37, stride=dim, out_stride=dim, shift=0, scale=1.0)
+
+
+@pytest.mark.parametrize("T", [F32, F16, BF16])
+@pytest.mark.parametrize("O", [F32, F16, BF16])
+def test_embed_types_strides_alignment(ctx, torch, T, O):
+    rng = np.random.default_rng(T * 3 + O)
+    for shift, stride, out_stride, dim in ((0, 72, 80, 64), (1, 65, 67, 64), (3, 100, 99, 33), (5, 1, 1, 1), (2, 4100, 4101, 4099)):
+        _embed_case(ctx, torch, rng, 130, dim, T, O, 50, stride, out_stride, shift, scale=45.25)
+
+
+def _embed_case(ctx, torch, rng, n, dim, T, O, rows, stride, out_stride, shift, scale):
+    held, _keep, ptr, _ = _matrix(torch, rng.standard_normal((rows, dim)), T, stride, shift, fill=float("nan"))
+    ids = _ids(rng, n, rows)
+    d_ids = torch.from_numpy(ids).cuda()
+    out = torch.full((shift + (n + 1) * out_stride + 8,), -7.0, dtype=_t(torch, O), device="cuda")
+    ctx.embed(d_ids.data_ptr(), n, ptr, T, rows, dim, stride, out.data_ptr() + shift * out.element_size(), O, out_stride, scale)
+    got = out.double().cpu().numpy()
+    assert (got[:shift] == -7).all() and (got[shift + (n - 1) * out_stride + dim:] == -7).all()
+    got = got[shift:shift + n * out_stride].reshape(n, out_stride)
+    assert (got[:, dim:] == -7).all()                       # what lies between the rows stays
+    want = ref.embed(ids, held, scale)
+    tol = np.abs(want) * (U + HALF[O]) * (1 + 2 * U) + STEP0[O] / 2 + 2.0 ** -149
+    assert (np.abs(got[:, :dim] - want) <= tol).all()
+
+
+def test_embed_values_at_the_ends_of_the_types(ctx, torch):
+    """Subnormal numbers, the largest ones, infinities and NaN pass through as the type's own conversion has them."""
+    v = torch.tensor([0.0, -0.0, 1e-45, 1e-40, 2.0 ** -126, 6e-8, 3e-8, 65504.0, 65520.0, 3.4e38, float("inf"), float("-inf"), float("nan"),
+                      1.00390625, 1.01171875, -1.00390625], dtype=torch.float32)
+    for T in (F32, F16, BF16):
+        table = v.to(_t(torch, T)).cuda().reshape(1, -1)
+        for O in (F32, F16, BF16):
+            for scale in (1.0, 0.5, 0.0, 3.0):
+                out = torch.full((2, v.numel()), -7.0, dtype=_t(torch, O), device="cuda")
+                ids = torch.tensor([0, -1], dtype=torch.int32, device="cuda")
+                ctx.embed(ids.data_ptr(), 2, table.data_ptr(), T, 1, v.numel(), v.numel(), out.data_ptr(), O, v.numel(), scale)
+                want = (table.cpu().float() * scale).to(_t(torch, O))      # both steps are correctly rounded
+                assert torch.equal(out[0].cpu().nan_to_num(nan=12345.0), want[0].nan_to_num(nan=12345.0))
+                assert torch.equal(torch.isnan(out[0].cpu()), torch.isnan(want[0]))
+                assert (out[1] == 0).all()
+
+
+@pytest.mark.parametrize("count", [0, 1, 99, 100, 101, 2 ** 40])
+def test_embed_counts_on_the_device(ctx, torch, count):
+    ids = torch.arange(100, dtype=torch.int32, device="cuda") % 7
+    table = torch.randn(7, 40, device="cuda")
+    out = torch.full((101, 40), -7.0, device="cuda")
+    n_dev = torch.tensor([count], dtype=torch.int64, device="cuda")
+    ctx.embed(ids.data_ptr(), 100, table.data_ptr(), F32, 7, 40, 40, out.data_ptr(), F32, 40, 1.0, n_dev.data_ptr())
+    k = min(count, 100)
+    assert torch.equal(out[:k], table[ids.long()][:k]) and (out[k:] == -7).all()
+
+
+def test_embed_offsets_beyond_32_bits(ctx, torch):
+    """Element offsets pass 2^32 in the table and in the output (rows far apart)."""
+    rows, dim, stride = 3, 16, (1 << 30) + 8
+    table = torch.zeros(2 * stride + dim + (1 << 30) * 2, dtype=torch.float16, device="cuda")     # 8 GiB
+    assert 2 * stride * 2 > 2 ** 32
+    for r in range(rows):
+        table[r * stride:r * stride + dim] = r + 1
+    ids = torch.tensor([2, 0, 1], dtype=torch.int32, device="cuda")
+    out = torch.full((2 * stride + dim + 8,), -7.0, dtype=torch.float16, device="cuda")
+    ctx.embed(ids.data_ptr(), 3, table.data_ptr(), F16, rows, dim, stride, out.data_ptr(), F16, stride, 1.0)
+    for t, want in enumerate((3, 1, 2)):
+        assert (out[t * stride:t * stride + dim] == want).all()
+    assert (out[dim:dim + 64] == -7).all() and (out[stride - 64:stride] == -7).all()
+
+
+# ---- gradient -----------------------------------------------------------------------------------------------------
+def _grad_case(ctx, torch, rng, ids, dim, G, T, rows, accumulate, scale=1.0, grad_stride=None, table_stride=None, shift=0, n_dev=None, whole=False):
+    n = len(ids)
+    grad_stride, table_stride = grad_stride or dim, table_stride or dim
+    values = rng.integers(-8, 9, (n, dim)).astype(np.float64) if whole else rng.standard_normal((n, dim))
+    g, _k1, gp, _ = _matrix(torch, values, G, grad_stride, shift, fill=float("nan"))
+    old = rng.integers(-8, 9, (rows, dim)).astype(np.float64) if whole else rng.standard_normal((rows, dim))
+    was, buf, tp, view = _matrix(torch, old, T, table_stride, shift, fill=-7.0)
+    d_ids = torch.from_numpy(np.asarray(ids, dtype=np.int32)).cuda()
+    need = capi.embed_grad_workspace(n, dim)
+    work = torch.full((need + 64,), 0xAB, dtype=torch.uint8, device="cuda")
+    count = torch.tensor([n if n_dev is None else n_dev], dtype=torch.int64, device="cuda")
+    ctx.embed_grad(d_ids.data_ptr(), n, gp, G, grad_stride, rows, dim, tp, T, table_stride, work.data_ptr(), need, scale, accumulate,
+                   None if n_dev is None else count.data_ptr())
+    got = view.double().cpu().numpy()
+    used = np.asarray(ids)[:n if n_dev is None else min(n, n_dev)]
+    want, size, terms = ref.embed_grad(used, g[:len(used)], rows, scale, was if accumulate else None)
+    u = (terms[:, None] + 2) * U
+    tol = u * size * (1 + u) + HALF[T] * np.abs(want) + STEP0[T] / 2 + 2.0 ** -149
+    tol[terms == 0] = 0.0
+    if whole:
+        tol[:] = HALF[T] * np.abs(want)                     # whole numbers below 2^24 add up without rounding
+    assert (np.abs(got - want) <= tol).all()
+    full = buf.double().cpu().numpy()
+    assert (full[:shift] == -7).all() and (full[shift + rows * table_stride:] == -7).all()
+    if table_stride > dim:
+        assert (full[shift:shift + rows * table_stride].reshape(rows, table_stride)[:, dim:] == -7).all()
+    assert (work[need:] == 0xAB).all()
+    return view.clone()
+
+
+@pytest.mark.parametrize("n", [1, 2, 7, 8, 9, 64, 300, 1025, 4095, 4096, 4097, 9000])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_grad_lengths(ctx, torch, n, accumulate):
+    rng = np.random.default_rng(n)
+    _grad_case(ctx, torch, rng, _ids(rng, n, 200), 24, BF16, F32, 200, accumulate)
+
+
+@pytest.mark.parametrize("dim", [1, 3, 8, 65, 129, 1001, 2048, 2056, 4104])
+def test_grad_widths(ctx, torch, dim):
+    rng = np.random.default_rng(dim)
+    for accumulate in (False, True):
+        _grad_case(ctx, torch, rng, _ids(rng, 333, 60), dim, F16, F32, 60, accumulate, scale=0.5)
+
+
+@pytest.mark.parametrize("G", [F32, F16, BF16])
+@pytest.mark.parametrize("T", [F32, F16, BF16])
+def test_grad_types_strides_alignment(ctx, torch, G, T):
+    rng = np.random.default_rng(G * 3 + T)
+    for accumulate in (False, True):
+        for shift, gs, ts, dim in ((0, 72, 80, 64), (1, 65, 67, 64), (3, 1003, 1001, 999)):
+            _grad_case(ctx, torch, rng, _ids(rng, 700, 90), dim, G, T, 90, accumulate, 45.25, gs, ts, shift)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 255, 511, 512, 513, 128256, 262143, 262144, 262145])
+def test_grad_numbers_of_digits(ctx, torch, rows):
+    """Keys of one to three digits; the first and last rows among them."""
+    rng = np.random.default_rng(rows)
+    ids = _ids(rng, 5000, rows)
+    ids[:4] = [0, rows - 1, 0, rows - 1]
+    _grad_case(ctx, torch, rng, ids, 8, F32, F32, rows, False)
+    _grad_case(ctx, torch, rng, ids, 8, F32, F32, rows, True)
+
+
+@pytest.mark.parametrize("n", [64, 1000, 8192, 40000])
+def test_grad_long_runs(ctx, torch, n):
+    """One id throughout, two ids, runs that end on every place of a walker's chunk; whole numbers, so nothing is rounded."""
+    rng = np.random.default_rng(n)
+    _grad_case(ctx, torch, rng, np.full(n, 3), 40, BF16, F32, 5, True, whole=True)
+    _grad_case(ctx, torch, rng, np.arange(n) % 2 + 1, 40, BF16, F32, 5, False, whole=True)
+    ids = np.repeat(np.arange(400), np.arange(400) % 131 + 1)[:n]
+    rng.shuffle(ids)
+    _grad_case(ctx, torch, rng, ids, 40, BF16, F32, 400, False, whole=True)
+    _grad_case(ctx, torch, rng, np.full(n, -1), 40, BF16, F32, 5, False, whole=True)      # nobody is named: all rows zero
+    _grad_case(ctx, torch, rng, np.full(n, -1), 40, BF16, F32, 5, True, whole=True)
+
+
+@pytest.mark.parametrize("count", [0, 1, 500, 999, 1000, 2 ** 40])
+def test_grad_counts_on_the_device(ctx, torch, count):
+    rng = np.random.default_rng(5)
+    for accumulate in (False, True):
+        _grad_case(ctx, torch, rng, _ids(rng, 1000, 50), 16, F32, F32, 50, accumulate, n_dev=count)
+
+
+def test_grad_without_ids(ctx, torch):
+    table = torch.full((50, 33), 5.0, dtype=torch.bfloat16, device="cuda")
+    ctx.embed_grad(None, 0, None, F32, 33, 50, 33, table.data_ptr(), BF16, 33, None, 0, 1.0, True)
+    assert (table == 5).all()
+    ctx.embed_grad(None, 0, None, F32, 33, 50, 33, table.data_ptr(), BF16, 33, None, 0, 1.0, False)
+    assert (table == 0).all()
+
+
+def test_grad_is_the_lookups_gradient(ctx, torch):
+    """<G, dW> against differences of <embed(W), dY>, and the same bits from the same ids."""
+    rng = np.random.default_rng(11)
+    n, rows, dim, scale = 600, 80, 48, 0.5
+    ids = _ids(rng, n, rows)
+    d_ids = torch.from_numpy(ids).cuda()
+    dy = torch.from_numpy(rng.integers(-8, 9, (n, dim))).float().cuda()
+    table = torch.from_numpy(rng.integers(-8, 9, (rows, dim))).float().cuda()
+    step = torch.from_numpy(rng.integers(-2, 3, (rows, dim))).float().cuda()
+    need = capi.embed_grad_workspace(n, dim)
+    work = torch.empty(need, dtype=torch.uint8, device="cuda")
+    grad = torch.empty_like(table)
+    ctx.embed_grad(d_ids.data_ptr(), n, dy.data_ptr(), F32, dim, rows, dim, grad.data_ptr(), F32, dim, work.data_ptr(), need, scale)
+
+    def loss(w):
+        out = torch.empty(n, dim, device="cuda")
+        ctx.embed(d_ids.data_ptr(), n, w.data_ptr(), F32, rows, dim, dim, out.data_ptr(), F32, dim, scale)
+        return float((out.double() * dy.double()).sum())
+
+    # the lookup is linear and every number here a small multiple of 1/2: the difference is exact
+    assert loss(table + step) - loss(table - step) == 2 * float((grad.double() * step.double()).sum())
+
+
+def test_grad_same_bits(ctx, torch):
+    rng = np.random.default_rng(12)
+    n, rows, dim = 20000, 300, 264
+    d_ids = torch.from_numpy(_ids(rng, n, rows)).cuda()
+    dy = torch.randn(n, dim, device="cuda").bfloat16()
+    need = capi.embed_grad_workspace(n, dim)
+    got = []
+    for _ in range(3):
+        work = torch.randint(0, 256, (need,), dtype=torch.uint8, device="cuda")
+        grad = torch.empty(rows, dim, device="cuda")
+        ctx.embed_grad(d_ids.data_ptr(), n, dy.data_ptr(), BF16, dim, rows, dim, grad.data_ptr(), F32, dim, work.data_ptr(), need)
+        got.append(grad)
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+
+
+# ---- paged cache --------------------------------------------------------------------------------------------------
+class DeviceCache:
+    """A cache's state on the GPU, its calls in place or to other arrays."""
+
+    def __init__(self, torch, state, in_place=True, stride_more=3):
+        length, held, table, free, n_free, self.page, self.n_pages, self.max_pages = state
+        self.torch, self.n = torch, len(length)
+        i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+        self.stride = self.max_pages + stride_more
+        self.table = torch.full((max(self.n, 1), self.stride), -9, dtype=torch.int32, device="cuda")
+        if self.n:
+            self.table[:, :self.max_pages] = i32(table)
+        self.len, self.held = i32(length), i32(held)
+        self.free, self.n_free = i32(free), i32([n_free])
+        self.len2, self.held2, self.n_free2 = (self.len, self.held, self.n_free) if in_place else (i32(length) - 99, i32(held) - 99, i32([-99]))
+        self.status = torch.full((1,), 77, dtype=torch.int32, device="cuda")
+        self.need = capi.cache_workspace(self.n)
+        self.work = torch.randint(0, 256, (self.need + 64,), dtype=torch.uint8, device="cuda")
+        self.work[self.need:] = 0xAB
+
+    def slots(self, ctx, d_off, slots, pos, cap, stream=None):
+        ctx.cache_slots(d_off.data_ptr(), self.n, self.len.data_ptr(), self.held.data_ptr(), self.page, self.n_pages, self.table.data_ptr(),
+                        self.stride, self.max_pages, self.free.data_ptr(), self.n_free.data_ptr(), self.len2.data_ptr(), self.held2.data_ptr(),
+                        self.n_free2.data_ptr(), slots.data_ptr(), pos.data_ptr(), cap, self.status.data_ptr(), self.work.data_ptr(), self.need,
+                        stream)
+
+    def trim(self, ctx, d_keep, stream=None):
+        ctx.cache_trim(d_keep.data_ptr(), self.n, self.len.data_ptr(), self.held.data_ptr(), self.page, self.n_pages, self.table.data_ptr(),
+                       self.stride, self.max_pages, self.free.data_ptr(), self.n_free.data_ptr(), self.len2.data_ptr(), self.held2.data_ptr(),
+                       self.n_free2.data_ptr(), self.status.data_ptr(), self.work.data_ptr(), self.need, stream)
+
+    def state(self):
+        assert (self.work[self.need:] == 0xAB).all() and (self.table[:, self.max_pages:] == -9).all()
+        return (self.len2.tolist(), self.held2.tolist(), self.table[:self.n, :self.max_pages].tolist(), self.free.tolist(),
+                int(self.n_free2[0]))
+
+    def now(self):
+        """The state that the last call left is the next call's."""
+        self.len, self.held, self.n_free = self.len2, self.held2, self.n_free2
+
+
+def _cache_round(ctx, torch, rng, n, page, max_pages, n_pages, new, in_place, tight=False, odd=False, more_cap=5):
+    import random
+    length, held, table, free, n_free = random_cache(random.Random(int(rng.integers(1 << 30))), n, page, max_pages, n_pages)
+    if tight:
+        n_free = min(n_free, int(sum(new)) // page // 2)
+    if odd and n > 2:
+        length[1], held[1] = -1, 0
+        length[n // 2], held[n // 2] = held[n // 2] * page + 1, held[n // 2]
+        free[max(0, n_free - 2)] = n_pages
+    off = [0] + np.cumsum(new).tolist()
+    cap = off[-1] + more_cap
+    state = (length, held, table, free, n_free, page, n_pages, max_pages)
+    model, dev = ref.Cache(*state), DeviceCache(torch, state, in_place)
+    slots, pos = [-7] * (cap + 1), [-7] * (cap + 1)
+    status = model.slots(off, cap, slots, pos)
+    d_slots = torch.full((cap + 1,), -7, dtype=torch.int64, device="cuda")
+    d_pos = torch.full((cap + 1,), -7, dtype=torch.int32, device="cuda")
+    d_off = torch.tensor(off, dtype=torch.int64, device="cuda")
+    dev.slots(ctx, d_off, d_slots, d_pos, cap)
+    assert dev.state() == (model.length, model.held, model.table, model.free, model.n_free)
+    assert d_slots.tolist() == slots and d_pos.tolist() == pos and int(dev.status[0]) == status
+    dev.now()
+    if not in_place:
+        dev.len2, dev.held2, dev.n_free2 = (x.clone() - 50 for x in (dev.len, dev.held, dev.n_free))
+    keep = [int(rng.choice([-1, 0, max(0, L), max(0, L - 3), L + 9, max(0, L // 2)])) for L in model.length]
+    status = model.trim(keep)
+    dev.trim(ctx, torch.tensor(keep, dtype=torch.int32, device="cuda"))
+    assert dev.state() == (model.length, model.held, model.table, model.free, model.n_free) and int(dev.status[0]) == status
+
+
+@pytest.mark.parametrize("n", [1, 2, 63, 64, 255, 256, 257, 1023, 1024, 1025, 2500])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_cache_requests(ctx, torch, n, in_place):
+    rng = np.random.default_rng(n)
+    page = [16, 1, 7, 64][n % 4]
+    new = rng.choice([0, 1, 1, 5, 40], n)
+    _cache_round(ctx, torch, rng, n, page, 12, n * 10 + 20, new, in_place)
+    _cache_round(ctx, torch, rng, n, page, 12, n * 10 + 20, new, in_place, tight=True, odd=True, more_cap=0)
+
+
+@pytest.mark.parametrize("tokens", [0, 1, 255, 256, 257, 1024, 5000, 20000])
+def test_cache_one_long_request(ctx, torch, tokens):
+    rng = np.random.default_rng(tokens)
+    _cache_round(ctx, torch, rng, 1, 16, 1300, 2700, [tokens], True)
+    _cache_round(ctx, torch, rng, 3, 16, 1300, 7000, [0, tokens, 0], False)
+
+
+def test_cache_single_tokens_step_after_step(ctx, torch):
+    """130 steps of one token each for requests of which some end on the way; pages go round the pool."""
+    import random
+    rng = random.Random(3)
+    n, page, max_pages, n_pages = 70, 8, 24, 600
+    state = (*random_cache(rng, n, page, 8, n_pages, full=0.1), page, n_pages, 8)
+    state = (state[0], state[1], [r + [-5] * 16 for r in state[2]], state[3], state[4], page, n_pages, max_pages)
+    model, dev = ref.Cache(*state), DeviceCache(torch, state)
+    d_slots = torch.empty(n, dtype=torch.int64, device="cuda")
+    d_pos = torch.empty(n, dtype=torch.int32, device="cuda")
+    for step in range(130):
+        new = [0 if rng.random() < 0.1 else 1 for _ in range(n)]
+        off = [0] + np.cumsum(new).tolist()
+        slots, pos = [-7] * n, [-7] * n
+        d_slots.fill_(-7)
+        d_pos.fill_(-7)
+        status = model.slots(off, n, slots, pos)
+        dev.slots(ctx, torch.tensor(off, dtype=torch.int64, device="cuda"), d_slots, d_pos, n)
+        assert d_slots.tolist() == slots and d_pos.tolist() == pos and int(dev.status[0]) == status
+        there = [s for s in slots if s >= 0]
+        assert len(set(there)) == len(there)
+        keep = [0 if rng.random() < 0.04 else -1 for _ in range(n)]
+        status = model.trim(keep)
+        dev.trim(ctx, torch.tensor(keep, dtype=torch.int32, device="cuda"))
+        assert int(dev.status[0]) == status
+        assert dev.state() == (model.length, model.held, model.table, model.free, model.n_free)
+
+
+def test_cache_offsets_that_cannot_be(ctx, torch):
+    """Offsets that descend or end behind cap: those requests keep their state, nothing is written outside the arrays."""
+    state = ([5, 0, 3, 0], [1, 0, 1, 0], [[4, -5], [-5, -5], [6, -5], [-5, -5]], list(range(10, 30)) + [-5] * 12, 20, 8, 32, 2)
+    for off, cap in (([0, 3, 2, 5, 9], 9), ([0, 2, 4, 6, 100], 8), ([7, 8, 9, 10, 11], 11), ([2 ** 63, 2 ** 63 + 1, 2, 3, 4], 4)):
+        dev, model = DeviceCache(torch, state), ref.Cache(*state)
+        d_off = torch.from_numpy(np.array(off, np.uint64).view(np.int64)).cuda()
+        d_slots = torch.full((cap + 64,), -7, dtype=torch.int64, device="cuda")
+        d_pos = torch.full((cap + 64,), -7, dtype=torch.int32, device="cuda")
+        dev.slots(ctx, d_off, d_slots, d_pos, cap)
+        status = model.slots(off, cap, [-7] * cap, [-7] * cap)
+        assert dev.state() == (model.length, model.held, model.table, model.free, model.n_free) and int(dev.status[0]) == status
+        assert (d_slots[cap:] == -7).all() and (d_pos[cap:] == -7).all()
+
+
+@pytest.mark.parametrize("n_free", [-1, -2 ** 31, 33, 2 ** 31 - 1])
+def test_cache_counts_that_cannot_be(ctx, torch, n_free):
+    state = ([5, 16], [1, 2], [[4, -5, -5], [6, 7, -5]], list(range(32)), n_free, 8, 32, 3)
+    dev, model = DeviceCache(torch, state), ref.Cache(*state)
+    off = [0, 1, 2]
+    slots, pos = [-7] * 2, [-7] * 2
+    d_slots = torch.full((2,), -7, dtype=torch.int64, device="cuda")
+    d_pos = torch.full((2,), -7, dtype=torch.int32, device="cuda")
+    status = model.slots(off, 2, slots, pos)
+    dev.slots(ctx, torch.tensor(off, dtype=torch.int64, device="cuda"), d_slots, d_pos, 2)
+    assert int(dev.status[0]) == status == ref.BAD | ref.POOL
+    assert d_slots.tolist() == slots and d_pos.tolist() == pos and int(dev.n_free2[0]) == n_free
+    status = model.trim([0, 0])
+    dev.trim(ctx, torch.zeros(2, dtype=torch.int32, device="cuda"))
+    assert int(dev.status[0]) == status and dev.state() == (model.length, model.held, model.table, model.free, model.n_free)
+
+
+def test_cache_without_requests(ctx, torch):
+    dev = DeviceCache(torch, ([], [], [], [1, 2, 3, 4], 3, 8, 4, 2))
+    z = torch.full((4,), -7, dtype=torch.int64, device="cuda")
+    dev.slots(ctx, torch.zeros(1, dtype=torch.int64, device="cuda"), z, z.int(), 4)
+    assert int(dev.status[0]) == 0 and int(dev.n_free[0]) == 3 and (z == -7).all()
+    dev.status.fill_(9)
+    dev.trim(ctx, torch.zeros(1, dtype=torch.int32, device="cuda"))
+    assert int(dev.status[0]) == 0 and int(dev.n_free[0]) == 3
+
+
+# ---- verification -------------------------------------------------------------------------------------------------
+def _probs(rng, rows, vocab, sharp=3.0):
+    x = rng.standard_normal((rows, vocab)) * sharp
+    x = np.exp(x - x.max(1, keepdims=True)) if rows else x
+    return x / x.sum(1, keepdims=True) if rows else x
+
+
+def _verify(ctx, torch, draft, off, n_draft, max_draft, target, q, code, vocab, ua, ud, stride, q_stride, shift=0):
+    """Runs it and compares with the reference on the values the GPU holds."""
+    n = len(off) - 1
+    t, _k0, tp, _ = _matrix(torch, target, code, stride, shift, fill=float("nan"))
+    qv, qp = None, None
+    if q is not None:
+        qv, _k1, qp, _ = _matrix(torch, q, code, q_stride, shift, fill=float("nan"))
+    dev = lambda a, ty: torch.from_numpy(np.ascontiguousarray(a, dtype=ty)).cuda()  # noqa: E731
+    d_draft, d_off = dev(np.append(draft, 0), np.int32), dev(np.asarray(off, dtype=np.uint64).view(np.int64), np.int64)
+    d_ua, d_ud = dev(np.append(ua, 0), np.float32), dev(ud, np.float32)
+    out = torch.full((n + 1, max_draft + 1), -7, dtype=torch.int32, device="cuda")
+    acc = torch.full((n + 1,), -7, dtype=torch.int32, device="cuda")
+    need = capi.verify_workspace(n, vocab)
+    work = torch.full((need + 64,), 0xAB, dtype=torch.uint8, device="cuda")
+    ctx.verify_draft(d_draft.data_ptr(), d_off.data_ptr(), n, n_draft, max_draft, tp, code, stride, qp, q_stride, vocab, d_ua.data_ptr(),
+                     d_ud.data_ptr(), out.data_ptr(), acc.data_ptr(), work.data_ptr(), need)
+    want, accepted = ref.verify(np.asarray(draft)[:n_draft], off, max_draft, t, qv, vocab, np.asarray(ua, np.float32), np.asarray(ud, np.float32))
+    assert acc[:n].tolist() == accepted.tolist()
+    assert out[:n].tolist() == want.tolist()
+    assert (out[n] == -7).all() and int(acc[n]) == -7 and (work[need:] == 0xAB).all()
+    return want, accepted
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 7, 8, 9, 500, 2047, 2048, 2049, 5001, 128256])
+@pytest.mark.parametrize("code", [F32, F16, BF16])
+@pytest.mark.parametrize("with_q", [False, True])
+def test_verify_vocabularies(ctx, torch, vocab, code, with_q):
+    rng = np.random.default_rng(vocab * 6 + code * 2 + with_q)
+    n, most = 9, 5
+    k = rng.integers(0, most + 1, n)
+    k[0], k[1] = most, 0
+    off = [0] + np.cumsum(k).tolist()
+    total = off[-1]
+    target = _probs(rng, total + n, vocab)
+    row = np.arange(total) + np.repeat(np.arange(n), k)
+    near = target[row] * np.exp(rng.standard_normal((total, vocab)) * 0.5)
+    q = near / near.sum(1, keepdims=True)
+    draft = np.array([rng.choice(vocab, p=r) for r in q] if with_q else q.argmax(1), dtype=np.int32)
+    _verify(ctx, torch, draft, off, total, most, target, q if with_q else None, code, vocab, rng.random(total), rng.random(n),
+            vocab + 3, vocab + 1, shift=1)
+
+
+@pytest.mark.parametrize("k", [1, 2, 63, 64, 65, 130])
+def test_verify_many_drafts(ctx, torch, k):
+    """Every place at which the first rejection can be, beyond a wave's width; draws at both ends of [0, 1)."""
+    rng = np.random.default_rng(k)
+    vocab, n = 40, k + 1
+    off = [i * k for i in range(n + 1)]
+    target = _probs(rng, n * (k + 1), vocab)
+    q = _probs(rng, n * k, vocab)
+    draft = rng.integers(0, vocab, n * k).astype(np.int32)
+    ua = np.zeros((n, k), np.float32)
+    for i in range(k):
+        ua[i, i] = np.float32(1 - 2 ** -24)
+        q[i * k + i, draft[i * k + i]] = 2.0          # with u next to 1 this one is rejected
+    ud = np.where(np.arange(n) % 2, 0.0, 1 - 2.0 ** -24).astype(np.float32)
+    _, accepted = _verify(ctx, torch, draft, off, n * k, k, target, q, F32, vocab, ua.reshape(-1), ud, vocab, vocab)
+    assert accepted.tolist() == list(range(k)) + [k]
+
+
+def test_verify_borders(ctx, torch):
+    """Probabilities and draws whose sums are exact: a draw on a border belongs to the next entry, u q = p is a rejection."""
+    vocab = 8
+    flat = np.full((17, vocab), 1 / 8)
+    off = [0] * 17
+    ud = np.arange(16) / 16
+    want, _ = _verify(ctx, torch, np.zeros(0, np.int32), off, 0, 0, flat[:16], None, F32, vocab, [], ud, vocab, vocab)
+    assert want[:, 0].tolist() == [i // 2 for i in range(16)]
+    p, q = np.full((2, vocab), 1 / 8), np.full((1, vocab), 1 / 8)
+    q[0, 3], q[0, 4] = 1 / 4, 0
+    want, acc = _verify(ctx, torch, np.array([3], np.int32), [0, 1], 1, 1, p, q, F32, vocab, [0.5], [0.0], vocab, vocab)
+    assert acc.tolist() == [0] and want.tolist() == [[4, -1]]            # 0.5 * 0.25 = 0.125 is not below it; only 4 is left
+    want, acc = _verify(ctx, torch, np.array([3], np.int32), [0, 1], 1, 1, p, q, F32, vocab, [0.49], [0.0], vocab, vocab)
+    assert acc.tolist() == [1] and want.tolist() == [[3, 0]]
+
+
+def test_verify_weights_that_are_none(ctx, torch):
+    """Nothing left after the draft: the target itself; no weight at all: -1.  NaN, infinities and negative numbers weigh nothing."""
+    vocab, nan, inf = 3000, float("nan"), float("inf")
+    p = np.zeros((16, vocab))
+    q = np.zeros((8, vocab))
+    p[0, [5, 2900]] = 0.5                        # request 0: q covers p, token 7 (p = 0) rejected -> drawn from p
+    q[0, [5, 7, 2900]] = 0.5, 1.0, 0.5
+    p[2, :] = 0                                  # request 1: no weight anywhere
+    q[1, 9] = 1.0
+    p[4, [1, 2, 3, 2500]] = nan, inf, -1.0, 0.25  # request 2: only 2500 weighs
+    q[2, [1, 2500]] = 1.0, nan                   # ... and q = NaN there: nothing is left, drawn from p
+    p[6, [0, 1]] = 0.5, 0.5                      # request 3: a drafted token that is none
+    q[3, 1] = 0.5
+    off = [0, 1, 2, 3, 4]
+    want, acc = _verify(ctx, torch, np.array([7, 9, 1, -1], np.int32), off, 4, 1, p[:8], q[:4], F32, vocab, [0.5] * 4, [0.6] * 4, vocab, vocab)
+    assert acc.tolist() == [0, 0, 0, 0] and want[:, 0].tolist() == [2900, -1, 2500, 0]
+    # certain drafts: the rejected token is left out, whatever it weighs; one outside the vocabulary leaves all
+    p2 = np.zeros((6, 4))
+    p2[0, [0, 2]] = 0.5
+    p2[2, 1] = 0.25
+    p2[4, 3] = 1.0
+    want, acc = _verify(ctx, torch, np.array([2, 1, 4], np.int32), [0, 1, 2, 3], 3, 1, p2, None, F32, 4, [0.9, 0.5, 0.0], [0.9, 0.9, 0.0], 4, 4)
+    assert acc.tolist() == [0, 0, 0] and want[:, 0].tolist() == [0, 1, 3]
+
+
+def test_verify_offsets_that_cannot_be(ctx, torch):
+    vocab = 16
+    p, q = np.full((12, vocab), 1 / 16), np.full((8, vocab), 1 / 16)
+    off = [0, 2, 1, 4, 8, 9, 2 ** 62]            # descends, holds more than max_draft, passes n_draft
+    want, acc = _verify(ctx, torch, np.arange(8, dtype=np.int32), off, 8, 3, p, q, F32, vocab, [0.5] * 8, [0.5] * 6, vocab, vocab)
+    assert acc.tolist() == [2, -1, 3, -1, -1, -1]
+    assert (want[[1, 3, 4, 5]] == -1).all()
+
+
+def test_verify_draws_what_the_target_says(ctx, torch):
+    """20,000 requests of one drafted token: what comes out is distributed as the target, for each token within five standard
+    deviations of a share of 20,000 (a sound draw misses that once in a million tokens)."""
+    rng = np.random.default_rng(77)
+    vocab, n = 12, 20000
+    p1, q1, p2 = _probs(rng, 1, vocab, 1.0)[0], _probs(rng, 1, vocab, 1.0)[0], _probs(rng, 1, vocab, 1.0)[0]
+    target = np.empty((2 * n, vocab))
+    target[0::2], target[1::2] = p1, p2
+    q = np.tile(q1, (n, 1))
+    draft = rng.choice(vocab, n, p=q1).astype(np.int32)
+    want, acc = _verify(ctx, torch, draft, list(range(n + 1)), n, 1, target, q, F32, vocab, rng.random(n), rng.random(n), vocab, vocab)
+    share = np.bincount(want[:, 0], minlength=vocab) / n
+    assert (np.abs(share - p1) <= 5 * np.sqrt(p1 * (1 - p1) / n)).all()
+    second = want[acc == 1, 1]
+    share = np.bincount(second, minlength=vocab) / len(second)
+    assert (np.abs(share - p2) <= 5 * np.sqrt(p2 * (1 - p2) / len(second))).all()
+
+
+# ---- streams, graphs, threads -------------------------------------------------------------------------------------
+def test_calls_follow_their_stream(ctx, torch):
+    """Inputs that are still being made on the stream, and the null stream for torch's default stream."""
+    ids = torch.zeros(4096, dtype=torch.int32, device="cuda")
+    table = torch.randn(100, 256, device="cuda")
+    out = torch.zeros(4096, 256, device="cuda")
+    big = torch.randn(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    for stream in (torch.cuda.Stream(), None):
+        with torch.cuda.stream(stream) if stream else torch.cuda.stream(torch.cuda.default_stream()):
+            x = big
+            for _ in range(8):
+                x = x @ big * 1e-2
+            ids.copy_((torch.arange(4096, device="cuda") % 100).int() + (x[0, 0] * 0).int())
+            ctx.embed(ids.data_ptr(), 4096, table.data_ptr(), F32, 100, 256, 256, out.data_ptr(), F32, 256, 1.0, None,
+                      torch.cuda.current_stream().cuda_stream)
+            got = out.clone()
+        torch.cuda.synchronize()
+        assert torch.equal(got, table[(torch.arange(4096) % 100).cuda()])
+        ids.zero_()
+        out.zero_()
+        torch.cuda.synchronize()
+
+
+def test_captured_and_replayed(ctx, torch):
+    """All operators in two captured graphs, each replayed several times with new inputs and eager work between, against eager calls."""
+    rng = np.random.default_rng(4)
+    n, rows, dim, seqs, vocab, most = 600, 500, 136, 20, 3001, 3
+
+    def buffers():
+        import random
+        b = dict(ids=torch.zeros(n, dtype=torch.int32, device="cuda"), table=torch.randn(rows, dim, device="cuda").bfloat16(),
+                 out=torch.zeros(n, dim, device="cuda"), dy=torch.randn(n, dim, device="cuda"), grad=torch.zeros(rows, dim, device="cuda"),
+                 whole=torch.zeros(rows, dim, device="cuda"), work=torch.empty(capi.embed_grad_workspace(n, dim), dtype=torch.uint8, device="cuda"),
+                 off=torch.zeros(seqs + 1, dtype=torch.int64, device="cuda"), slots=torch.zeros(n, dtype=torch.int64, device="cuda"),
+                 pos=torch.zeros(n, dtype=torch.int32, device="cuda"), keep=torch.zeros(seqs, dtype=torch.int32, device="cuda"))
+        b["cache"] = DeviceCache(torch, (*random_cache(random.Random(1), seqs, 8, 40, 2000, full=0.03), 8, 2000, 40))
+        k = np.arange(seqs) % (most + 1)
+        total = int(k.sum())
+        b["voff"] = torch.from_numpy(np.append(0, np.cumsum(k))).cuda()
+        b["draft"] = torch.zeros(total, dtype=torch.int32, device="cuda")
+        b["target"] = torch.softmax(torch.randn(total + seqs, vocab, device="cuda"), -1)
+        b["q"] = torch.softmax(torch.randn(total, vocab, device="cuda"), -1)
+        b["ua"], b["ud"] = torch.zeros(total, device="cuda"), torch.zeros(seqs, device="cuda")
+        b["vout"], b["acc"] = torch.zeros(seqs, most + 1, dtype=torch.int32, device="cuda"), torch.zeros(seqs, dtype=torch.int32, device="cuda")
+        b["vwork"] = torch.empty(capi.verify_workspace(seqs, vocab), dtype=torch.uint8, device="cuda")
+        return b
+
+    def run(b):
+        s = torch.cuda.current_stream().cuda_stream
+        ctx.embed(b["ids"].data_ptr(), n, b["table"].data_ptr(), BF16, rows, dim, dim, b["out"].data_ptr(), F32, dim, 2.0, b["off"].data_ptr() + 8 * seqs, s)
+        for t, acc in ((b["grad"], True), (b["whole"], False)):
+            ctx.embed_grad(b["ids"].data_ptr(), n, b["dy"].data_ptr(), F32, dim, rows, dim, t.data_ptr(), F32, dim, b["work"].data_ptr(),
+                           b["work"].numel(), 1.0, acc, b["off"].data_ptr() + 8 * seqs, s)
+        b["cache"].slots(ctx, b["off"], b["slots"], b["pos"], n, s)
+        b["cache"].trim(ctx, b["keep"], s)
+        ctx.verify_draft(b["draft"].data_ptr(), b["voff"].data_ptr(), seqs, b["draft"].numel(), most, b["target"].data_ptr(), F32, vocab,
+                         b["q"].data_ptr(), vocab, vocab, b["ua"].data_ptr(), b["ud"].data_ptr(), b["vout"].data_ptr(), b["acc"].data_ptr(),
+                         b["vwork"].data_ptr(), b["vwork"].numel(), s)
+
+    def inputs(bs, rng):
+        new = rng.integers(0, 25, seqs)
+        off = np.minimum(np.append(0, np.cumsum(new)), n)
+        ids = _ids(rng, n, rows)
+        keep = rng.choice([-1, 0, 30, 1000], seqs).astype(np.int32)
+        total = bs[0]["draft"].numel()
+        draft, ua, ud = rng.integers(0, vocab, total).astype(np.int32), rng.random(total).astype(np.float32), rng.random(seqs).astype(np.float32)
+        for b in bs:
+            for k, v in (("off", off), ("ids", ids), ("keep", keep), ("draft", draft), ("ua", ua), ("ud", ud)):
+                b[k].copy_(torch.from_numpy(v))
+
+    pairs = []
+    for _ in range(2):
+        torch.manual_seed(5)
+        a = buffers()
+        torch.manual_seed(5)
+        b = buffers()
+        inputs((a, b), rng)
+        g = torch.cuda.CUDAGraph()
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.graph(g, stream=s):
+            run(a)
+        pairs.append((g, a, b))
+    for turn in range(4):
+        for g, a, b in pairs:
+            inputs((a, b), rng)
+            g.replay()
+            run(b)
+            torch.cuda.synchronize()
+            for k in ("out", "grad", "whole", "slots", "pos", "vout", "acc"):
+                assert torch.equal(a[k], b[k]), (turn, k)
+            assert a["cache"].state() == b["cache"].state() and int(a["cache"].status[0]) == int(b["cache"].status[0])
+
+
+def test_two_threads(ctx, torch):
+    """Calls on one context from two threads, each on a stream and workspace of its own."""
+    import threading
+    rng = np.random.default_rng(6)
+    n, rows, dim = 3000, 400, 72
+    jobs, errors = [], []
+    for _ in range(2):
+        ids = torch.from_numpy(_ids(rng, n, rows)).cuda()
+        dy = torch.from_numpy(rng.integers(-8, 9, (n, dim))).float().cuda()
+        there = ((ids >= 0) & (ids < rows)).float()[:, None]
+        want = torch.zeros(rows, dim, device="cuda").index_add_(0, ids.clamp(0, rows - 1).long(), dy * there)
+        jobs.append((ids, dy, want, torch.empty(rows, dim, device="cuda"), torch.empty(capi.embed_grad_workspace(n, dim), dtype=torch.uint8, device="cuda")))
+    torch.cuda.synchronize()
+
+    def go(ids, dy, want, got, work):
+        try:
+            s = torch.cuda.Stream()
+            for _ in range(50):
+                ctx.embed_grad(ids.data_ptr(), n, dy.data_ptr(), F32, dim, rows, dim, got.data_ptr(), F32, dim, work.data_ptr(), work.numel(), 1.0,
+                               False, None, s.cuda_stream)
+                s.synchronize()
+                assert torch.equal(got, want)
+        except Exception as e:   # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=go, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+
+
+def test_refusals_leave_the_context_usable(ctx, torch):
+    table = torch.randn(4, 8, device="cuda")
+    out = torch.full((2, 8), -7.0, device="cuda")
+    ids = torch.tensor([1, 3], dtype=torch.int32, device="cuda")
+    with pytest.raises(capi.L3Error) as e:
+        ctx.embed(ids.data_ptr(), 2, table.data_ptr(), 9, 4, 8, 8, out.data_ptr(), F32, 8)
+    assert e.value.code == capi.L3_E_INVALID_ARG and "type" in str(e.value)
+    with pytest.raises(capi.L3Error) as e:
+        ctx.embed_grad(ids.data_ptr(), 2, out.data_ptr(), F32, 8, 4, 8, table.data_ptr(), F32, 8, table.data_ptr(), 16)
+    assert "l3_embed_grad_workspace" in str(e.value)
+    assert (out == -7).all()
+    ctx.embed(ids.data_ptr(), 2, table.data_ptr(), F32, 4, 8, 8, out.data_ptr(), F32, 8)
+    assert torch.equal(out, table[ids.long()])
+
+
+# ---- together -----------------------------------------------------------------------------------------------------
+def test_from_text_to_text(ctx, torch, oracle):
+    """Prompts are encoded, take pages, are looked up; drafts are verified, what was not accepted is trimmed, the answers decoded; and
+    the lookup's gradient comes back.  The ids never leave the GPU before decode."""
+    import random
+    rng = random.Random(8)
+    docs = [b"Hello, world!", b"", "don't 12345 café\n\n".encode()] + [corpus.random_doc(rng, max_pieces=12) for _ in range(29)]
+    text, off = capi.pack_docs(docs)
+    n, vocab, dim, most, page = len(docs), ctx.vocab_size(), 64, 4, 16
+    cap = int(text.size) * 3 + 2 * n
+    d_text = torch.from_numpy(text.copy()).cuda()
+    d_doc = torch.from_numpy(off.astype(np.int64)).cuda()
+    ids = torch.full((cap,), -1, dtype=torch.int32, device="cuda")
+    d_off = torch.zeros(n + 1, dtype=torch.int64, device="cuda")
+    torch.cuda.synchronize()
+    rc, total = ctx.encode_batch_device(d_text.data_ptr(), int(text.size), d_doc.data_ptr(), n, capi.L3_BOS, ids.data_ptr(), cap, d_off.data_ptr())
+    assert rc == capi.L3_OK
+    want_ids, want_off = oracle.encode_batch(text, off, True, False, threads=2)
+    lens = np.diff(want_off.astype(np.int64))
+
+    max_pages = int(-(-(lens.max() + most + 1) // page))
+    state = ([0] * n, [0] * n, [[-5] * max_pages] * n, list(range(n * max_pages)), n * max_pages, page, n * max_pages, max_pages)
+    cache = DeviceCache(torch, state)
+    slots = torch.full((cap,), -7, dtype=torch.int64, device="cuda")
+    pos = torch.full((cap,), -7, dtype=torch.int32, device="cuda")
+    cache.slots(ctx, d_off, slots, pos, cap)
+    model = ref.Cache(*state)
+    m_slots, m_pos = [-7] * cap, [-7] * cap
+    assert model.slots(want_off.astype(int).tolist(), cap, m_slots, m_pos) == 0 == int(cache.status[0])
+    assert slots.tolist() == m_slots and pos.tolist() == m_pos
+
+    table = torch.randn(vocab, dim, device="cuda").bfloat16()
+    hidden = torch.full((cap, dim), -7.0, dtype=torch.bfloat16, device="cuda")
+    ctx.embed(ids.data_ptr(), cap, table.data_ptr(), BF16, vocab, dim, dim, hidden.data_ptr(), BF16, dim, 1.0, d_off.data_ptr() + 8 * n)
+    assert torch.equal(hidden[:total], table[torch.from_numpy(want_ids.astype(np.int64)).cuda()]) and (hidden[total:] == -7).all()
+
+    # a model that is certain: it continues every prompt with its own first four tokens; the draft has every third one wrong
+    k = np.minimum(lens, most)
+    voff = np.append(0, np.cumsum(k))
+    first = [want_ids[int(want_off[i]):int(want_off[i]) + k[i]] for i in range(n)]
+    draft = np.concatenate(first).astype(np.int32)
+    target = torch.zeros(int(voff[-1]) + n, vocab, device="cuda")
+    for i in range(n):
+        for j in range(k[i] + 1):
+            target[voff[i] + i + j, int(first[i][j]) if j < k[i] else 128001] = 1.0
+    wrong = np.arange(len(draft)) % 3 == 2
+    d_draft = torch.from_numpy(np.where(wrong, (draft + 1) % 1000, draft).astype(np.int32)).cuda()
+    d_voff = torch.from_numpy(voff).cuda()
+    ua, ud = torch.rand(len(draft), device="cuda"), torch.rand(n, device="cuda")
+    out = torch.empty(n, most + 1, dtype=torch.int32, device="cuda")
+    acc = torch.empty(n, dtype=torch.int32, device="cuda")
+    vwork = torch.empty(capi.verify_workspace(n, vocab), dtype=torch.uint8, device="cuda")
+    # the step's tokens (the last one of the prompt is in the cache already): the k drafted ones
+    s2, p2 = torch.full((len(draft),), -7, dtype=torch.int64, device="cuda"), torch.full((len(draft),), -7, dtype=torch.int32, device="cuda")
+    cache.slots(ctx, d_voff, s2, p2, len(draft))
+    assert int(cache.status[0]) == 0 and int(s2.min()) >= 0
+    ctx.verify_draft(d_draft.data_ptr(), d_voff.data_ptr(), n, len(draft), most, target.data_ptr(), F32, vocab, None, 0, vocab, ua.data_ptr(),
+                     ud.data_ptr(), out.data_ptr(), acc.data_ptr(), vwork.data_ptr(), vwork.numel())
+    keep = (torch.from_numpy(lens).cuda() + acc).int()
+    cache.trim(ctx, keep)
+    assert int(cache.status[0]) == 0 and cache.len.tolist() == keep.tolist()
+    accepted, answers = acc.tolist(), out.cpu().numpy()
+    for i in range(n):
+        good = next((j for j in range(k[i]) if wrong[voff[i] + j] and int(d_draft[voff[i] + j]) != int(draft[voff[i] + j])), k[i])
+        assert accepted[i] == good
+        line = [int(x) for x in first[i][:good + 1]] + ([128001] if good == k[i] else [])
+        assert answers[i].tolist() == line + [-1] * (most + 1 - len(line))
+    got, goff = ctx.decode_batch(answers.reshape(-1), np.arange(n + 1, dtype=np.uint64) * (most + 1))
+    for i in range(n):
+        assert got[int(goff[i]):int(goff[i + 1])].tobytes() == oracle.decode([t for t in answers[i].tolist() if t >= 0])
+
+    grad = torch.empty(vocab, dim, device="cuda")
+    dy = torch.ones(cap, dim, dtype=torch.bfloat16, device="cuda")
+    work = torch.empty(capi.embed_grad_workspace(cap, dim), dtype=torch.uint8, device="cuda")
+    ctx.embed_grad(ids.data_ptr(), cap, dy.data_ptr(), BF16, dim, vocab, dim, grad.data_ptr(), F32, dim, work.data_ptr(), work.numel(), 1.0, False,
+                   d_off.data_ptr() + 8 * n)
+    count = np.bincount(want_ids, minlength=vocab)
+    assert torch.equal(grad.cpu(), torch.from_numpy(np.repeat(count[:, None], dim, 1)).float())

@@ -26,6 +26,13 @@ L3_BOS = 1
 L3_EOS = 2
 L3_NO_SPECIAL = 4
 L3_ONE_PRETOKEN = 8
+L3_F32 = 0
+L3_F16 = 1
+L3_BF16 = 2
+L3_CACHE_POOL = 1
+L3_CACHE_ROW = 2
+L3_CACHE_BAD = 4
+L3_CACHE_PAGE = 8
 
 # every symbol include/l3hip.h declares: (name, restype, argtypes)
 _P = C.c_void_p
@@ -56,6 +63,19 @@ SYMBOLS = [
     ("l3_special_token_id", C.c_int, [_P, C.c_char_p, C.c_size_t, C.POINTER(C.c_int32)]),
     ("l3_vocab_size", C.c_int, [_P]),
     ("l3_token_bytes", C.c_int, [_P, C.c_int32, _P, C.c_size_t]),
+    ("l3_embed", C.c_int, [_P, _P, C.c_uint64, _P, _P, C.c_int, C.c_uint64, C.c_uint64, C.c_uint64, C.c_float, _P, C.c_int, C.c_uint64,
+                           _P]),
+    ("l3_embed_grad_workspace", C.c_uint64, [C.c_uint64, C.c_uint64]),
+    ("l3_embed_grad", C.c_int, [_P, _P, C.c_uint64, _P, _P, C.c_int, C.c_uint64, C.c_uint64, C.c_uint64, C.c_float, _P, C.c_int, C.c_uint64,
+                                C.c_int, _P, C.c_uint64, _P]),
+    ("l3_cache_workspace", C.c_uint64, [C.c_uint64]),
+    ("l3_cache_slots", C.c_int, [_P, _P, C.c_uint64, _P, _P, C.c_uint32, C.c_uint32, _P, C.c_uint64, C.c_uint64, _P, _P, _P, _P, _P, _P, _P,
+                                 C.c_uint64, _P, _P, C.c_uint64, _P]),
+    ("l3_cache_trim", C.c_int, [_P, _P, C.c_uint64, _P, _P, C.c_uint32, C.c_uint32, _P, C.c_uint64, C.c_uint64, _P, _P, _P, _P, _P, _P, _P,
+                                C.c_uint64, _P]),
+    ("l3_verify_workspace", C.c_uint64, [C.c_uint64, C.c_uint64]),
+    ("l3_verify_draft", C.c_int, [_P, _P, _P, C.c_uint64, C.c_uint64, C.c_uint32, _P, C.c_int, C.c_uint64, _P, C.c_uint64, C.c_uint64, _P, _P,
+                                  _P, _P, _P, C.c_uint64, _P]),
     ("l3_set_profiling", C.c_int, [_P, C.c_int]),
     ("l3_last_timings", C.c_int, [_P, _P, C.c_int]),
     ("l3_timing_totals", C.c_int, [_P, _P, C.c_int, C.POINTER(C.c_uint64)]),
@@ -232,6 +252,49 @@ class Context:
         rc = self.lib.l3_encode_wait(self.h, ticket, C.byref(n))
         return rc, int(n.value)
 
+    # ---- operators on token ids (raw device pointers as ints; they queue work on `stream` and return) ------------------
+    # stream: a hipStream_t as an int (torch: torch.cuda.current_stream().cuda_stream); None: the null stream, which is torch's
+    # default stream.  A refused or failed call raises L3Error.
+    def embed(self, d_ids, n_ids, d_table, table_type, n_rows, dim, table_stride, d_out, out_type, out_stride, scale=1.0, d_n_ids=None,
+              stream=None):
+        """out[t] = scale * table[ids[t]] (l3_embed)."""
+        rc = self.lib.l3_embed(self.h, d_ids, n_ids, d_n_ids, d_table, table_type, n_rows, dim, table_stride, scale, d_out, out_type,
+                               out_stride, stream)
+        if rc != L3_OK:
+            raise self._err(rc)
+
+    def embed_grad(self, d_ids, n_ids, d_grad, grad_type, grad_stride, n_rows, dim, d_table, table_type, table_stride, d_work, work_bytes,
+                   scale=1.0, accumulate=False, d_n_ids=None, stream=None):
+        """table[v] (+)= scale * sum of grad[t] over ids[t] = v (l3_embed_grad); d_work: embed_grad_workspace(n_ids, dim) bytes."""
+        rc = self.lib.l3_embed_grad(self.h, d_ids, n_ids, d_n_ids, d_grad, grad_type, grad_stride, n_rows, dim, scale, d_table, table_type,
+                                    table_stride, 1 if accumulate else 0, d_work, work_bytes, stream)
+        if rc != L3_OK:
+            raise self._err(rc)
+
+    def cache_slots(self, d_new_off, n_seqs, d_len, d_held, page_size, n_pages, d_table, table_stride, max_pages, d_free, d_n_free,
+                    d_len_out, d_held_out, d_n_free_out, d_slots, d_pos, cap, d_status, d_work, work_bytes, stream=None):
+        """Pages, slots and positions of a step's new tokens (l3_cache_slots); d_work: cache_workspace(n_seqs) bytes."""
+        rc = self.lib.l3_cache_slots(self.h, d_new_off, n_seqs, d_len, d_held, page_size, n_pages, d_table, table_stride, max_pages, d_free,
+                                     d_n_free, d_len_out, d_held_out, d_n_free_out, d_slots, d_pos, cap, d_status, d_work, work_bytes, stream)
+        if rc != L3_OK:
+            raise self._err(rc)
+
+    def cache_trim(self, d_keep, n_seqs, d_len, d_held, page_size, n_pages, d_table, table_stride, max_pages, d_free, d_n_free, d_len_out,
+                   d_held_out, d_n_free_out, d_status, d_work, work_bytes, stream=None):
+        """Requests cut to keep[i] tokens, their other pages back in the pool (l3_cache_trim)."""
+        rc = self.lib.l3_cache_trim(self.h, d_keep, n_seqs, d_len, d_held, page_size, n_pages, d_table, table_stride, max_pages, d_free,
+                                    d_n_free, d_len_out, d_held_out, d_n_free_out, d_status, d_work, work_bytes, stream)
+        if rc != L3_OK:
+            raise self._err(rc)
+
+    def verify_draft(self, d_draft, d_draft_off, n_seqs, n_draft, max_draft, d_target, prob_type, target_stride, d_draft_probs, draft_stride,
+                     vocab, d_u_accept, d_u_draw, d_out, d_accepted, d_work, work_bytes, stream=None):
+        """Drafted tokens accepted or replaced (l3_verify_draft); d_work: verify_workspace(n_seqs, vocab) bytes."""
+        rc = self.lib.l3_verify_draft(self.h, d_draft, d_draft_off, n_seqs, n_draft, max_draft, d_target, prob_type, target_stride,
+                                      d_draft_probs, draft_stride, vocab, d_u_accept, d_u_draw, d_out, d_accepted, d_work, work_bytes, stream)
+        if rc != L3_OK:
+            raise self._err(rc)
+
     # ---- small queries ------------------------------------------------------------------------------
     def host_alloc(self, nbytes, dtype=np.uint8):
         """Page-locked host buffer from the library as a numpy array (free it with host_free(array))."""
@@ -297,6 +360,26 @@ def partition_by_bytes(doc_off, world):
     if rc != L3_OK:
         raise L3Error(rc, "l3_partition_by_bytes")
     return cuts.astype(np.int64).tolist()
+
+
+def _workspace(name, *sizes):
+    """Bytes of an operator's workspace (no GPU needed)."""
+    n = getattr(load_library(), name)(*sizes)
+    if n == 0:
+        raise L3Error(L3_E_INVALID_ARG, "%s: sizes out of range" % name)
+    return n
+
+
+def embed_grad_workspace(n_ids, dim):
+    return _workspace("l3_embed_grad_workspace", n_ids, dim)
+
+
+def cache_workspace(n_seqs):
+    return _workspace("l3_cache_workspace", n_seqs)
+
+
+def verify_workspace(n_seqs, vocab):
+    return _workspace("l3_verify_workspace", n_seqs, vocab)
 
 
 class MultiContext:

@@ -16,6 +16,7 @@
 #include "../../include/l3hip.h"
 #include "l3_kernels.h"
 #include "l3_tables.h"
+#include "l3_token_kernels.h"
 
 using namespace l3;
 
@@ -1326,6 +1327,108 @@ int l3_multi_encode_batch(l3_multi* m, const uint8_t* text, const uint64_t* doc_
     *n_tok = sum;
     if (sum > out_cap) { m->err = "output buffer too small"; return L3_E_OUTPUT_CAP; }
     return L3_OK;
+}
+
+}  // extern "C"
+
+// ---- operators on token ids ------------------------------------------------------------------------------------
+// They keep nothing in the context: its device and its error text are all they use of it.  So they do not wait for its lock
+// either (an encode call of another thread holds it while its batch runs), except to leave an error text.
+namespace {
+
+static_assert(L3_F32 == kF32 && L3_F16 == kF16 && L3_BF16 == kBF16, "public element types are the kernels'");
+static_assert(L3_CACHE_POOL == kCachePool && L3_CACHE_ROW == kCacheRow && L3_CACHE_BAD == kCacheBad && L3_CACHE_PAGE == kCachePage,
+              "public status bits are the kernels'");
+
+// The context's device for the length of a call: the caller's current device is the caller's, these calls do not end with the
+// work and must not leave another one current.
+struct OnDevice {
+    int before = -1, device;
+    hipError_t e;
+    explicit OnDevice(int d) : device(d) {
+        e = hipGetDevice(&before);
+        if (e == hipSuccess && before != device) e = hipSetDevice(device);
+    }
+    ~OnDevice() { if (before >= 0 && before != device) (void)hipSetDevice(before); }
+};
+
+int leave_error(l3_ctx* c, int rc, const char* what, const char* more) noexcept {
+    try {
+        std::lock_guard<std::mutex> lk(c->mu);
+        c->err = std::string(what) + more;
+    } catch (...) {
+    }
+    return rc;
+}
+
+template <class Args>
+int run_op(l3_ctx* c, const Args& A, const char* wrong, hipError_t (*go)(const Args&, hipStream_t), void* stream) noexcept {
+    if (wrong) return leave_error(c, L3_E_INVALID_ARG, wrong, "");
+    OnDevice here(c->device);
+    hipError_t e = here.e;
+    if (e == hipSuccess) e = go(A, (hipStream_t)stream);
+    return e == hipSuccess ? L3_OK : leave_error(c, L3_E_HIP, "launch: ", hipGetErrorString(e));
+}
+
+}  // namespace
+
+extern "C" {
+
+int l3_embed(l3_ctx* c, const int32_t* d_ids, uint64_t n_ids, const uint64_t* d_n_ids, const void* d_table, int table_type,
+             uint64_t n_rows, uint64_t dim, uint64_t table_stride, float scale, void* d_out, int out_type, uint64_t out_stride,
+             void* stream) {
+    if (!c) return L3_E_INVALID_ARG;
+    EmbedArgs A{d_ids, n_ids, d_n_ids, d_table, table_type, n_rows, dim, table_stride, d_out, out_type, out_stride, scale};
+    return run_op(c, A, check_embed(A), launch_embed, stream);
+}
+
+uint64_t l3_embed_grad_workspace(uint64_t n_ids, uint64_t dim) {
+    return n_ids > kMaxCount || dim > kMaxDim ? 0 : grad_work(n_ids, dim).total;
+}
+
+int l3_embed_grad(l3_ctx* c, const int32_t* d_ids, uint64_t n_ids, const uint64_t* d_n_ids, const void* d_grad, int grad_type,
+                  uint64_t grad_stride, uint64_t n_rows, uint64_t dim, float scale, void* d_table, int table_type,
+                  uint64_t table_stride, int accumulate, void* d_work, uint64_t work_bytes, void* stream) {
+    if (!c) return L3_E_INVALID_ARG;
+    EmbedGradArgs A{d_ids, n_ids, d_n_ids, d_grad, grad_type, grad_stride, n_rows, dim, d_table, table_type, table_stride, scale,
+                    accumulate, d_work, work_bytes};
+    return run_op(c, A, check_embed_grad(A), launch_embed_grad, stream);
+}
+
+uint64_t l3_cache_workspace(uint64_t n_seqs) { return n_seqs > kMaxSeqs ? 0 : cache_work(n_seqs).total; }
+
+int l3_cache_slots(l3_ctx* c, const uint64_t* d_new_off, uint64_t n_seqs, const int32_t* d_len, const int32_t* d_held,
+                   uint32_t page_size, uint32_t n_pages, int32_t* d_table, uint64_t table_stride, uint64_t max_pages,
+                   const int32_t* d_free, const int32_t* d_n_free, int32_t* d_len_out, int32_t* d_held_out, int32_t* d_n_free_out,
+                   int64_t* d_slots, int32_t* d_pos, uint64_t cap, uint32_t* d_status, void* d_work, uint64_t work_bytes, void* stream) {
+    if (!c) return L3_E_INVALID_ARG;
+    CacheArgs A{d_new_off, nullptr, n_seqs, d_len, d_held, page_size, n_pages, d_table, table_stride, max_pages, const_cast<int32_t*>(d_free),
+                d_n_free, d_len_out, d_held_out, d_n_free_out, d_slots, d_pos, cap, d_status, d_work, work_bytes};
+    return run_op(c, A, check_cache(A, false), launch_cache_slots, stream);
+}
+
+int l3_cache_trim(l3_ctx* c, const int32_t* d_keep, uint64_t n_seqs, const int32_t* d_len, const int32_t* d_held, uint32_t page_size,
+                  uint32_t n_pages, const int32_t* d_table, uint64_t table_stride, uint64_t max_pages, int32_t* d_free,
+                  const int32_t* d_n_free, int32_t* d_len_out, int32_t* d_held_out, int32_t* d_n_free_out, uint32_t* d_status,
+                  void* d_work, uint64_t work_bytes, void* stream) {
+    if (!c) return L3_E_INVALID_ARG;
+    CacheArgs A{nullptr, d_keep, n_seqs, d_len, d_held, page_size, n_pages, const_cast<int32_t*>(d_table), table_stride, max_pages, d_free,
+                d_n_free, d_len_out, d_held_out, d_n_free_out, nullptr, nullptr, 0, d_status, d_work, work_bytes};
+    return run_op(c, A, check_cache(A, true), launch_cache_trim, stream);
+}
+
+uint64_t l3_verify_workspace(uint64_t n_seqs, uint64_t vocab) {
+    return n_seqs > kMaxSeqs || vocab > kMaxCount ? 0 : verify_work(n_seqs, vocab);
+}
+
+int l3_verify_draft(l3_ctx* c, const int32_t* d_draft, const uint64_t* d_draft_off, uint64_t n_seqs, uint64_t n_draft,
+                    uint32_t max_draft, const void* d_target, int type, uint64_t target_stride, const void* d_draft_probs,
+                    uint64_t draft_stride, uint64_t vocab, const float* d_u_accept, const float* d_u_draw, int32_t* d_out,
+                    int32_t* d_accepted, void* d_work, uint64_t work_bytes, void* stream) {
+    if (!c) return L3_E_INVALID_ARG;
+    VerifyArgs A{d_draft, d_draft_off, n_seqs, n_draft, max_draft, d_target, type, target_stride, d_draft_probs, draft_stride, vocab,
+                 d_u_accept, d_u_draw, d_out, d_accepted, d_work, work_bytes};
+    return run_op(c, A, check_verify(A), launch_verify, stream);
 }
 
 }  // extern "C"

@@ -1,0 +1,203 @@
+// l3_verify.hip -- verification of drafted tokens against the target's probabilities, from given random numbers.
+//
+// Request i has k drafted tokens d_0 .. d_{k-1}, drawn from the rows q_j, and the target's rows p_0 .. p_k.  Token j is accepted
+// while u_j q_j(d_j) < p_j(d_j); the first that is not (or, if all are, position k) is drawn anew: the smallest v with
+//     w(0) + .. + w(v) > r (w(0) + .. + w(vocab - 1)),   w = max(p_a - q_a, 0) if token a was rejected, p_k if all were accepted,
+// so that what comes out is distributed as the target's own tokens.  Without q the drafted token counts as certain (q = 1 there).
+// Products, differences and sums are in 64 bits: the answer is a whole number, and a border must not move with the order.
+#include "l3_token_kernels.h"
+
+#include "l3_dev.h"
+
+namespace l3 {
+
+namespace {
+
+constexpr int kVerifyThreads = 256;
+
+// What became of a request's drafted tokens.  state: kBadRequest / kDrawTarget (all accepted) / kDrawRest (token `a` rejected).
+enum : int { kBadRequest = 0, kDrawTarget = 1, kDrawRest = 2 };
+struct Verdict { int state; uint32_t a; uint64_t p_row, q_row; int32_t token; };
+
+// Called by a whole wave.
+template <class T>
+__device__ Verdict verdict_of(const VerifyArgs& A, uint64_t i) {
+    Verdict R;
+    R.state = kBadRequest; R.a = 0; R.p_row = R.q_row = 0; R.token = -1;
+    const uint64_t lo = A.off[i], hi = A.off[i + 1];
+    if (lo > hi || hi > A.n_draft || hi - lo > A.max_draft) return R;
+    const uint32_t k = (uint32_t)(hi - lo);
+    uint32_t a = k;
+    for (uint32_t j0 = 0; j0 < k; j0 += 64) {
+        const uint32_t j = j0 + lane_id();
+        bool ok = true;
+        if (j < k) {
+            const int32_t d = A.draft[lo + j];
+            ok = false;
+            if (d >= 0 && (uint64_t)d < A.vocab) {
+                const double p = (double)(float)((const T*)A.target)[(lo + i + j) * A.target_stride + (uint64_t)d];
+                const double q = A.q ? (double)(float)((const T*)A.q)[(lo + j) * A.q_stride + (uint64_t)d] : 1.0;
+                ok = (double)A.u_accept[lo + j] * q < p;
+            }
+        }
+        const u64 no = __ballot(!ok);
+        if (no) { a = j0 + (uint32_t)__builtin_ctzll(no); break; }
+    }
+    R.a = a;
+    R.p_row = lo + i + a;
+    R.q_row = lo + a;
+    R.state = a == k ? kDrawTarget : kDrawRest;
+    if (a < k) R.token = A.draft[lo + a];
+    return R;
+}
+
+// A weight that is no positive finite number counts as none.
+__device__ __forceinline__ double weight(double x) { return x > 0.0 && x < __builtin_huge_val() ? x : 0.0; }
+
+// Eight neighbouring entries: rest = what is left of the target after the draft, full = the target's own.
+template <class T>
+__device__ __forceinline__ void weights8(const VerifyArgs& A, const Verdict& R, uint64_t col, double* rest, double* full) {
+    const T* p = (const T*)A.target + R.p_row * A.target_stride;
+    const T* q = R.state == kDrawRest && A.q ? (const T*)A.q + R.q_row * A.q_stride : nullptr;
+    float pv[8], qv[8];
+    if (col + 8 <= A.vocab) {
+        load8(p + col, pv);
+        if (q) load8(q + col, qv);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const bool in = col + j < A.vocab;
+            pv[j] = in ? (float)p[col + j] : 0.f;
+            if (q) qv[j] = in ? (float)q[col + j] : 0.f;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        full[j] = weight((double)pv[j]);
+        rest[j] = q ? weight((double)pv[j] - (double)qv[j]) : (uint64_t)(int64_t)R.token == col + j ? 0.0 : full[j];
+    }
+}
+
+__device__ __forceinline__ double wave_sum_f64(double v) {
+    for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d, 64);
+    return v;
+}
+
+// Sums of kVerifyChunk entries: sums[i][chunk] = {rest, full}.  A workgroup per request and chunk.
+template <class T>
+__global__ __launch_bounds__(kVerifyThreads) void verify_sum_kernel(VerifyArgs A, uint64_t chunks, double* sums) {
+    __shared__ double tmp[2][kVerifyThreads / 64];
+    for (uint64_t g = blockIdx.x; g < A.n * chunks; g += gridDim.x) {
+        const uint64_t i = g / chunks, c = g % chunks;
+        const Verdict R = verdict_of<T>(A, i);
+        double sr = 0, sf = 0;
+        const uint64_t col = c * kVerifyChunk + (uint64_t)threadIdx.x * 8;
+        if (R.state != kBadRequest && col < A.vocab) {
+            double rest[8], full[8];
+            weights8<T>(A, R, col, rest, full);
+#pragma unroll
+            for (int j = 0; j < 8; j++) { sr += rest[j]; sf += full[j]; }
+        }
+        sr = wave_sum_f64(sr);
+        sf = wave_sum_f64(sf);
+        if (lane_id() == 0) { tmp[0][wave_id()] = sr; tmp[1][wave_id()] = sf; }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            sr = sf = 0;
+            for (int w = 0; w < kVerifyThreads / 64; w++) { sr += tmp[0][w]; sf += tmp[1][w]; }
+            sums[2 * g] = sr;
+            sums[2 * g + 1] = sf;
+        }
+        __syncthreads();
+    }
+}
+
+// A workgroup per request: the chunk the border falls into, then the entry.
+template <class T>
+__global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs A, uint64_t chunks, const double* sums) {
+    __shared__ double tmp[kVerifyThreads / 64];
+    __shared__ double s_before, s_target;
+    __shared__ long long s_chunk;
+    __shared__ int s_use_rest;
+    __shared__ int s_token, s_last;
+    for (uint64_t i = blockIdx.x; i < A.n; i += gridDim.x) {
+        const Verdict R = verdict_of<T>(A, i);
+        int32_t* out = A.out + i * (A.max_draft + 1ull);
+        if (threadIdx.x == 0) {
+            const double* S = sums + 2 * i * chunks;
+            double rest = 0, full = 0;
+            for (uint64_t c = 0; c < chunks; c++) { rest += S[2 * c]; full += S[2 * c + 1]; }
+            const int use_rest = R.state == kDrawRest && rest > 0;
+            const double all = use_rest ? rest : full, target = (double)A.u_draw[i] * all;
+            long long at = -1, last = -1;
+            double run = 0, before = 0;
+            for (uint64_t c = 0; c < chunks; c++) {
+                const double w = S[2 * c + (use_rest ? 0 : 1)];
+                if (w > 0) {
+                    if (at < 0) { last = (long long)c; before = run; }   // (behind the last chunk with weight: the last entry with weight)
+                    run += w;
+                    if (at < 0 && run > target) at = (long long)c;
+                }
+            }
+            s_chunk = at >= 0 ? at : last;
+            s_before = before;
+            s_target = target;
+            s_use_rest = use_rest;
+            s_token = 0x7FFFFFFF;
+            s_last = -1;
+        }
+        __syncthreads();
+        const long long c = R.state == kBadRequest ? -1 : s_chunk;
+        if (c >= 0) {
+            const uint64_t col = (uint64_t)c * kVerifyChunk + (uint64_t)threadIdx.x * 8;
+            double rest[8], full[8], mine = 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) rest[j] = full[j] = 0;
+            if (col < A.vocab) weights8<T>(A, R, col, rest, full);
+#pragma unroll
+            for (int j = 0; j < 8; j++) { if (!s_use_rest) rest[j] = full[j]; mine += rest[j]; }
+            double inc = mine;
+            for (int d = 1; d < 64; d <<= 1) { const double o = __shfl_up(inc, d, 64); if (lane_id() >= d) inc += o; }
+            if (lane_id() == 63) tmp[wave_id()] = inc;
+            __syncthreads();
+            double run = s_before;
+            for (int w = 0; w < wave_id(); w++) run += tmp[w];
+            run += inc - mine;
+            const double target = s_target;
+            int found = 0x7FFFFFFF, last = -1;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                run += rest[j];
+                if (rest[j] > 0) {
+                    last = (int)(col + j);
+                    if (run > target && found == 0x7FFFFFFF) found = last;
+                }
+            }
+            if (found != 0x7FFFFFFF) atomicMin(&s_token, found);
+            if (last >= 0) atomicMax(&s_last, last);
+        }
+        __syncthreads();
+        // a border that rounding has put behind the chunk's last entry falls on the last entry with weight
+        const int32_t token = c < 0 ? -1 : s_token != 0x7FFFFFFF ? s_token : s_last;
+        const uint64_t lo = A.off[i];
+        for (uint32_t j = threadIdx.x; j <= A.max_draft; j += kVerifyThreads)
+            out[j] = R.state == kBadRequest ? -1 : j < R.a ? A.draft[lo + j] : j == R.a ? token : -1;
+        if (threadIdx.x == 0) A.accepted[i] = R.state == kBadRequest ? -1 : (int32_t)R.a;
+        __syncthreads();
+    }
+}
+
+}  // namespace
+
+hipError_t launch_verify(const VerifyArgs& A, hipStream_t stream) {
+    if (A.n == 0) return hipSuccess;
+    const uint64_t chunks = verify_chunks(A.vocab);
+    return with_dtype(A.dtype, [&](auto t) {
+        typedef decltype(t) T;
+        hipError_t e = launch(verify_sum_kernel<T>, capped(A.n * chunks), kVerifyThreads, stream, A, chunks, (double*)A.work);
+        if (e != hipSuccess) return e;
+        return launch(verify_draw_kernel<T>, capped(A.n), kVerifyThreads, stream, A, chunks, (const double*)A.work);
+    });
+}
+
+}  // namespace l3
