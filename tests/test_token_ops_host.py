@@ -89,7 +89,7 @@ REFUSED = [
     ("embed", dict(ids=None), "null"), ("embed", dict(table=None), "null"), ("embed", dict(out=None), "null"), ("embed", dict(ids=AT + 2), "aligned"),
     ("embed", dict(n_dev=AT + 4), "aligned"), ("embed", dict(table=AT + 1), "aligned"), ("embed", dict(dtype=0, table=AT + 2), "aligned"),
     ("embed", dict(out_dtype=0, out=AT + 2), "aligned"),
-    ("grad", dict(dtype=7), "type"), ("grad", dict(table_dtype=3), "type"), ("grad", dict(n=2 ** 31), "split"), ("grad", dict(rows=0), "n_rows"),
+    ("grad", dict(dtype=7), "type"), ("grad", dict(table_dtype=3), "type"), ("grad", dict(n=2 ** 24 + 1), "split"), ("grad", dict(rows=0), "n_rows"), ("grad", dict(rows=2 ** 29 + 1), "n_rows"),
     ("grad", dict(dim=0), "dim"), ("grad", dict(grad_stride=10), "stride"), ("grad", dict(table_stride=10), "stride"), ("grad", dict(accumulate=2), "accumulate"),
     ("grad", dict(table=None), "null"), ("grad", dict(ids=None), "null"), ("grad", dict(grad=None), "null"), ("grad", dict(work=None), "null"),
     ("grad", dict(table=AT + 2), "aligned"), ("grad", dict(grad=AT + 1), "aligned"), ("grad", dict(work=AT + 8), "16 bytes"),
@@ -134,7 +134,7 @@ def test_null_context_is_refused():
 def test_workspace_sizes(lib):
     """The library's answers are the checks' own sizes; 0 stands for sizes that no call takes."""
     L = capi.load_library()
-    for n, dim in ((0, 1), (1, 1), (64, 4096), (65536, 4096), (2 ** 31 - 1, 8)):
+    for n, dim in ((0, 1), (1, 1), (64, 4096), (65536, 4096), (2 ** 24, 8)):
         assert L.l3_embed_grad_workspace(n, dim) == lib.l3t_grad_work(n, dim) > 0
         need = lib.l3t_grad_work(n, dim)
         assert _check(lib, "grad", n=n, dim=dim, grad_stride=dim, table_stride=dim, work_bytes=need) is None
@@ -144,7 +144,7 @@ def test_workspace_sizes(lib):
         assert L.l3_cache_workspace(n) == lib.l3t_cache_work(n) > 0
     for n, v in ((0, 5), (1, 1), (3, 128256)):
         assert L.l3_verify_workspace(n, v) == lib.l3t_verify_work(n, v) > 0
-    assert L.l3_embed_grad_workspace(2 ** 31, 8) == 0 == L.l3_cache_workspace(2 ** 20 + 1) == L.l3_verify_workspace(1, 2 ** 31)
+    assert L.l3_embed_grad_workspace(2 ** 24 + 1, 8) == 0 == L.l3_cache_workspace(2 ** 20 + 1) == L.l3_verify_workspace(1, 2 ** 31)
     with pytest.raises(capi.L3Error):
         capi.cache_workspace(2 ** 20 + 1)
 

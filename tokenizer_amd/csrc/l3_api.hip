@@ -1383,7 +1383,7 @@ int l3_embed(l3_ctx* c, const int32_t* d_ids, uint64_t n_ids, const uint64_t* d_
 }
 
 uint64_t l3_embed_grad_workspace(uint64_t n_ids, uint64_t dim) {
-    return n_ids > kMaxCount || dim > kMaxDim ? 0 : grad_work(n_ids, dim).total;
+    return n_ids > kMaxGradIds || dim > kMaxDim ? 0 : grad_work(n_ids, dim).total;
 }
 
 int l3_embed_grad(l3_ctx* c, const int32_t* d_ids, uint64_t n_ids, const uint64_t* d_n_ids, const void* d_grad, int grad_type,
@@ -1418,7 +1418,7 @@ int l3_cache_trim(l3_ctx* c, const int32_t* d_keep, uint64_t n_seqs, const int32
 }
 
 uint64_t l3_verify_workspace(uint64_t n_seqs, uint64_t vocab) {
-    return n_seqs > kMaxSeqs || vocab > kMaxCount ? 0 : verify_work(n_seqs, vocab);
+    return n_seqs > kMaxSeqs || vocab > kMaxCount ? 0 : verify_work(n_seqs, vocab).total;
 }
 
 int l3_verify_draft(l3_ctx* c, const int32_t* d_draft, const uint64_t* d_draft_off, uint64_t n_seqs, uint64_t n_draft,

@@ -4,10 +4,11 @@
 // Token t of the step, the j-th new one of request i, is at position p = len[i] + j and goes to the slot
 // table[i][p / page] * page + p % page.  Pages that are missing come off the end of the free list, in order of the requests.
 //
-// Two launches, because a request's pages depend on those of all requests before it:
+// A request's pages depend on those of all requests before it, and its state may be replaced in place, so there are two launches:
 //   plan   a thread per request: how many pages it asks for, and their sum over the requests before it in its workgroup; the
-//          sums of the workgroups.  What a request was is copied to the workspace, so that its new state may replace the old.
+//          sums of the workgroups.  What a request was is copied to the workspace.
 //   apply  adds up the workgroups' sums, decides who is served, writes table, slots, positions and the new state.
+// A step that one workgroup has through in the time of a launch does both in one (cache_slots_one_kernel, cache_trim_one_kernel).
 #include "l3_token_kernels.h"
 
 #include "l3_dev.h"
@@ -56,99 +57,300 @@ __global__ __launch_bounds__(kPlanThreads) void cache_plan_kernel(CacheArgs A, P
     }
 }
 
-// pages that the requests in the workgroups before block `b` ask for; b <= n_blocks <= 1,024
-__device__ __forceinline__ u64 pages_before(const u64* blocks, uint64_t b) {
+constexpr int kApplyThreads = 256, kApplyWaves = kApplyThreads / 64;
+
+template <class V>
+__device__ __forceinline__ V apply_sum64(V v, u64* tmp) { return block_sum64<kApplyThreads / 64>(v, tmp); }
+
+// pages that the requests in the plan's workgroups before `b` ask for (give back); by a whole workgroup
+__device__ __forceinline__ u64 pages_before(const u64* blocks, uint64_t b, u64* tmp) {
     u64 s = 0;
-    for (uint64_t k = 0; k < b; k++) s += blocks[k];
-    return s;
+    for (uint64_t k = threadIdx.x; k < b; k += kApplyThreads) s += blocks[k];
+    return apply_sum64(s, tmp);
 }
 
-constexpr int kApplyThreads = 256;
+// The pages of all requests that are served: who asks for pages is served as long as the sum up to and with it is at most
+// `most`, so it is the largest such sum.  One workgroup.
+__device__ u64 pages_served(const PlanRec* recs, const u64* blocks, uint64_t n, u64 most, u64* tmp) {
+    const uint64_t n_blocks = (n + kPlanThreads - 1) / kPlanThreads;   // at most 1,024
+    constexpr int kPer = (int)(kMaxSeqs / kPlanThreads / kApplyThreads);
+    u64 mine[kPer], sum = 0;
+#pragma unroll
+    for (int k = 0; k < kPer; k++) {
+        const uint64_t b = (uint64_t)threadIdx.x * kPer + k;
+        mine[k] = b < n_blocks ? blocks[b] : 0;
+        sum += mine[k];
+    }
+    const u64 inc = wave_iscan64(sum);
+    __syncthreads();
+    if (lane_id() == 63) tmp[wave_id()] = inc;
+    __syncthreads();
+    u64 run = inc - sum, total = 0;
+    for (int w = 0; w < kApplyThreads / 64; w++) { if (w < wave_id()) run += tmp[w]; total += tmp[w]; }
+    __syncthreads();
+    if (total <= most) return total;
+    // the workgroup of the plan in which the sum passes `most`: all before it are served, its own requests one by one
+    u64 here = ~0ull, before = 0;
+#pragma unroll
+    for (int k = 0; k < kPer; k++) {
+        if (here == ~0ull && run + mine[k] > most) { here = (u64)threadIdx.x * kPer + k; before = run; }
+        run += mine[k];
+    }
+    const u64 at = block_min64<kApplyThreads / 64>(here, tmp);
+    const u64 base = apply_sum64(here == at ? before : 0ull, tmp);
+    u64 best = base;
+    for (uint64_t i = at * kPlanThreads + threadIdx.x; i < n && i < (at + 1) * kPlanThreads; i += kApplyThreads) {
+        const u64 e = base + recs[i].before + (u64)recs[i].delta;
+        if (e <= most && e > best) best = e;
+    }
+    __syncthreads();
+    return ~block_min64<kApplyThreads / 64>(~best, tmp);
+}
+
+// The last i < n with off[i] <= t, 64 places at a time, by a whole wave (for offsets that are not in order: some i < n).
+__device__ __forceinline__ uint64_t request_of(const uint64_t* off, uint64_t n, uint64_t t) {
+    uint64_t lo = 0, len = n;
+    while (len > 1) {
+        const uint64_t step = (len + 63) / 64, at = lo + (uint64_t)lane_id() * step;
+        const bool ok = (uint64_t)lane_id() * step < len && off[at] <= t;
+        const u64 m = __ballot(ok);
+        const uint64_t k = m ? 63 - __builtin_clzll(m) : 0;
+        lo += k * step;
+        len = len - k * step < step ? len - k * step : step;
+    }
+    return lo;
+}
+
+// What a token needs of its request.
+struct Owner {
+    uint64_t first, end;     // its new tokens
+    u64 next;                // free list: its first new page is at next - 1
+    int32_t len, held;       // held < 0: not served
+};
+__device__ __forceinline__ Owner owner_of(const CacheArgs& A, const PlanRec& r, uint64_t first, uint64_t end, u64 before, u64 left) {
+    Owner w;
+    w.first = first; w.end = end; w.next = left - before; w.len = r.len;
+    w.held = slots_served(r, before, left) ? r.held : -1;
+    return w;
+}
+// Slot and position of token t of request i.
+__device__ __forceinline__ uint32_t place_token(const CacheArgs& A, const Owner& w, uint64_t i, uint64_t t, int64_t* slot, int32_t* pos) {
+    *slot = -1;
+    *pos = -1;
+    if (w.held < 0 || t < w.first || t >= w.end) return 0;
+    const uint32_t q = (uint32_t)w.len + (uint32_t)(t - w.first), p = q / A.page, in = q - p * A.page;
+    // (pages that are new may not be in the table yet)
+    const int32_t id = p < (uint32_t)w.held ? A.table[i * A.table_stride + p] : A.free_pages[w.next - 1 - (p - (uint32_t)w.held)];
+    *pos = (int32_t)q;
+    *slot = slot_of(id, in, A.page, A.n_pages);
+    return *slot < 0 ? (uint32_t)kCachePage : 0u;
+}
+
+// Tokens in blocks of 1,024, four neighbours a thread; the requests of a block are found once and kept in LDS (more than
+// kOwners of them only where many requests have no new token: then every token looks for its own).
+constexpr int kTokensPer = 4, kTokenBlock = kApplyThreads * kTokensPer, kOwners = 1024;
 
 __global__ __launch_bounds__(kApplyThreads) void cache_slots_kernel(CacheArgs A, const PlanRec* recs, const u64* blocks,
                                                                     const CacheHead* head, uint64_t request_blocks) {
+    __shared__ u64 tmp[kApplyThreads / 64];
+    __shared__ Owner owners[kOwners];
     const uint64_t left = head->left;
     uint32_t bits = 0;
-    if (blockIdx.x < request_blocks) {   // a thread per request: its new state
-        const uint64_t i = (uint64_t)blockIdx.x * kApplyThreads + threadIdx.x;
-        if (i < A.n) {
-            const PlanRec r = recs[i];
-            const u64 before = pages_before(blocks, i / kPlanThreads) + r.before;
-            const bool served = slots_served(r, before, left);
+    if (blockIdx.x == 0) {
+        const u64 taken = pages_served(recs, blocks, A.n, left, tmp);
+        if (threadIdx.x == 0) { const int32_t n = *A.n_free; *A.n_free_out = head->bad ? n : n - (int32_t)taken; }
+        return;
+    }
+    if (blockIdx.x <= request_blocks) {  // a wave per request: its new state, and its new pages into the table
+        const uint64_t i0 = (uint64_t)(blockIdx.x - 1) * kApplyWaves, i = i0 + wave_id();   // (kApplyWaves divides kPlanThreads)
+        const u64 base = pages_before(blocks, i0 / kPlanThreads, tmp);
+        if (i >= A.n) return;
+        const PlanRec r = recs[i];
+        const u64 before = base + r.before;
+        const bool served = slots_served(r, before, left);
+        if (lane_id() == 0) {
             A.len_out[i] = served ? r.new_len : r.len;
             A.held_out[i] = served ? r.held + r.delta : r.held;
             bits = served ? 0u : r.flags ? r.flags : (uint32_t)kCachePool;
         }
-    } else {                             // a thread per token
-        const uint64_t total = A.n ? A.off[A.n] : 0;
-        const uint64_t t = (uint64_t)(blockIdx.x - request_blocks) * kApplyThreads + threadIdx.x;
-        if (t < A.cap && t < total) {
-            uint64_t a = 0, b = A.n;     // the last request that starts at or before t
-            while (b - a > 1) { const uint64_t m = (a + b) / 2; if (A.off[m] <= t) a = m; else b = m; }
-            int64_t slot = -1;
-            int32_t pos = -1;
-            const uint64_t first = A.off[a];
-            const PlanRec r = recs[a];
-            const u64 before = pages_before(blocks, a / kPlanThreads) + r.before;
-            if (first <= t && t < A.off[a + 1] && slots_served(r, before, left)) {
-                pos = r.len + (int32_t)(t - first);
-                const uint32_t p = (uint32_t)pos / A.page, in = (uint32_t)pos % A.page;
-                int32_t id;
-                if (p < (uint32_t)r.held) {
-                    id = A.table[a * A.table_stride + p];
-                } else {
-                    id = A.free_pages[left - 1 - before - (p - (uint32_t)r.held)];
-                    if (in == 0) A.table[a * A.table_stride + p] = id;   // a new page's first slot is always a new token's
-                }
-                slot = slot_of(id, in, A.page, A.n_pages);
-                if (slot < 0) bits = kCachePage;
+        if (served) {
+            int32_t* to = A.table + i * A.table_stride + r.held;
+            const int32_t* from = A.free_pages + (left - before) - 1;
+            for (int32_t j = lane_id(); j < r.delta; j += 64) to[j] = *(from - j);
+        }
+    } else {
+        const uint64_t t0 = (uint64_t)(blockIdx.x - 1 - request_blocks) * kTokenBlock;
+        uint64_t total = A.off[A.n];
+        if (total > A.cap) total = A.cap;
+        if (t0 >= total) return;
+        const uint64_t last = (t0 + kTokenBlock < total ? t0 + kTokenBlock : total) - 1;
+        const uint64_t a0 = request_of(A.off, A.n, t0), a1 = request_of(A.off, A.n, last);
+        const uint64_t b0 = a0 / kPlanThreads;
+        const u64 before0 = pages_before(blocks, b0, tmp);
+        auto load_owner = [&](uint64_t i) {
+            u64 before = before0;
+            for (uint64_t b = b0; b < i / kPlanThreads; b++) before += blocks[b];
+            const PlanRec r = recs[i];
+            return owner_of(A, r, A.off[i], A.off[i + 1], before + r.before, left);
+        };
+        const uint64_t many = a1 >= a0 ? a1 - a0 + 1 : kOwners + 1;
+        const uint64_t t = t0 + (uint64_t)threadIdx.x * kTokensPer;
+        int64_t slot[kTokensPer];
+        int32_t pos[kTokensPer];
+        if (many <= kOwners) {
+            for (uint64_t k = threadIdx.x; k < many; k += kApplyThreads) owners[k] = load_owner(a0 + k);
+            __syncthreads();
+            uint32_t k = 0, e = (uint32_t)many;
+            while (e - k > 1) { const uint32_t m = (k + e) / 2; if (owners[m].first <= t) k = m; else e = m; }
+#pragma unroll
+            for (int j = 0; j < kTokensPer; j++) {
+                while (k + 1 < (uint32_t)many && owners[k + 1].first <= t + j) k++;
+                if (t + j <= last) bits |= place_token(A, owners[k], a0 + k, t + j, &slot[j], &pos[j]);
             }
-            A.slots[t] = slot;
-            A.pos[t] = pos;
+        } else {
+            for (int j = 0; j < kTokensPer; j++) {
+                uint64_t a = 0, b = A.n;
+                while (b - a > 1) { const uint64_t m = (a + b) / 2; if (A.off[m] <= t + j) a = m; else b = m; }
+                if (t + j <= last) {
+                    if (a / kPlanThreads < b0) { slot[j] = -1; pos[j] = -1; continue; }   // (offsets out of order only)
+                    bits |= place_token(A, load_owner(a), a, t + j, &slot[j], &pos[j]);
+                }
+            }
+        }
+        if (t + kTokensPer <= last + 1) {
+            __builtin_memcpy(A.slots + t, slot, sizeof slot);
+            __builtin_memcpy(A.pos + t, pos, sizeof pos);
+        } else {
+            for (int j = 0; j < kTokensPer; j++) if (t + j <= last) { A.slots[t + j] = slot[j]; A.pos[t + j] = pos[j]; }
         }
     }
     if (bits) atomicOr(A.status, bits);
 }
 
-// The new count of the pool: pages of all requests that are served.
-template <bool TRIM>
-__global__ __launch_bounds__(kPlanThreads) void cache_count_kernel(CacheArgs A, const PlanRec* recs, const u64* blocks, const CacheHead* head) {
+// The request that page g of a call belongs to: the last one with before <= g.  (Requests in front of it that take no page share
+// its `before`, those behind it have at least g + 1.  g is smaller than the pages of those that are served, and up to there
+// `before` ascends.)
+__device__ __forceinline__ uint32_t request_of_page(const uint32_t* before, uint32_t n, uint32_t g) {
+    uint32_t k = 0, e = n;
+    while (e - k > 1) { const uint32_t m = (k + e) / 2; if (before[m] <= g) k = m; else e = m; }
+    return k;
+}
+
+// The whole step in one workgroup: at most kPlanThreads requests and kOneTokens tokens.
+constexpr uint64_t kOneTokens = 4096;
+
+__global__ __launch_bounds__(kPlanThreads) void cache_slots_one_kernel(CacheArgs A) {
     __shared__ u64 tmp[kPlanThreads / 64];
-    u64 mine = 0;
-    const uint64_t left = head->left;
-    u64 base = 0;
-    for (uint64_t b = 0; b * kPlanThreads < A.n; b++) {
-        const uint64_t i = b * kPlanThreads + threadIdx.x;
-        if (i < A.n) {
-            const PlanRec r = recs[i];
-            if (TRIM ? trim_served(r, base + r.before, left, A.n_pages) : slots_served(r, base + r.before, left)) mine += (u64)r.delta;
-        }
-        base += blocks[b];
+    __shared__ Owner owners[kPlanThreads];
+    __shared__ uint32_t s_before[kPlanThreads], s_status, s_taken;
+    const uint64_t i = threadIdx.x;
+    const int32_t n_free = *A.n_free;
+    const bool bad = n_free < 0 || (uint32_t)n_free > A.n_pages;
+    const u64 left = bad ? 0 : (u64)n_free;
+    if (threadIdx.x == 0) { s_status = bad ? (uint32_t)kCacheBad : 0u; s_taken = 0; }
+    PlanRec r{};
+    uint64_t first = 0, end = 0, total = 0;
+    if (A.n) total = A.off[A.n];
+    if (i < A.n) {
+        first = A.off[i];
+        end = A.off[i + 1];
+        r = plan_slots(A.len[i], A.held[i], first, end, A.cap, A.page, A.max_pages);
     }
-    u64 total;
-    (void)block_escan64(mine, tmp, &total);
+    u64 all;
+    const u64 before = block_escan64((u64)r.delta, tmp, &all);   // (barriers inside: nobody's state is read behind it)
+    if (i < A.n) {
+        const bool served = slots_served(r, before, left);
+        owners[i] = owner_of(A, r, first, end, before, left);
+        s_before[i] = (uint32_t)before;   // (a request asks for at most kOneTokens pages)
+        A.len_out[i] = served ? r.new_len : r.len;
+        A.held_out[i] = served ? r.held + r.delta : r.held;
+        if (!served) atomicOr(&s_status, r.flags ? r.flags : (uint32_t)kCachePool);
+        else if (r.delta) atomicMax(&s_taken, (uint32_t)(before + (u64)r.delta));
+    }
+    __syncthreads();
+    const uint32_t taken = s_taken;
+    for (uint32_t g = threadIdx.x; g < taken; g += kPlanThreads) {   // new pages into the table
+        const uint32_t k = request_of_page(s_before, (uint32_t)A.n, g);
+        A.table[k * A.table_stride + (uint32_t)owners[k].held + (g - s_before[k])] = A.free_pages[left - 1 - g];
+    }
+    if (total > A.cap) total = A.cap;
+    for (uint64_t t = threadIdx.x; t < total; t += kPlanThreads) {
+        uint32_t k = 0, e = (uint32_t)A.n;
+        while (e - k > 1) { const uint32_t m = (k + e) / 2; if (owners[m].first <= t) k = m; else e = m; }
+        int64_t slot;
+        int32_t pos;
+        const uint32_t bits = place_token(A, owners[k], k, t, &slot, &pos);
+        A.slots[t] = slot;
+        A.pos[t] = pos;
+        if (bits) atomicOr(&s_status, bits);
+    }
+    __syncthreads();
     if (threadIdx.x == 0) {
-        const int32_t n = *A.n_free;
-        *A.n_free_out = head->bad ? n : TRIM ? n + (int32_t)total : n - (int32_t)total;
+        *A.n_free_out = bad ? n_free : n_free - (int32_t)taken;
+        *A.status = s_status;
     }
 }
 
 // A wave per request: its new state, and the pages it gives back to the end of the free list.
 __global__ __launch_bounds__(kApplyThreads) void cache_trim_kernel(CacheArgs A, const PlanRec* recs, const u64* blocks, const CacheHead* head) {
+    __shared__ u64 tmp[kApplyThreads / 64];
     const uint64_t left = head->left;
-    for (uint64_t i = (uint64_t)blockIdx.x * (kApplyThreads / 64) + wave_id(); i < A.n; i += (uint64_t)gridDim.x * (kApplyThreads / 64)) {
-        const PlanRec r = recs[i];
-        const u64 before = pages_before(blocks, i / kPlanThreads) + r.before;
+    if (blockIdx.x == 0) {
+        const u64 given = pages_served(recs, blocks, A.n, A.n_pages - left, tmp);
+        if (threadIdx.x == 0) { const int32_t n = *A.n_free; *A.n_free_out = head->bad ? n : n + (int32_t)given; }
+        return;
+    }
+    const uint64_t i0 = (uint64_t)(blockIdx.x - 1) * kApplyWaves, i = i0 + wave_id();   // (kApplyWaves divides kPlanThreads)
+    const u64 base = pages_before(blocks, i0 / kPlanThreads, tmp);
+    if (i >= A.n) return;
+    const PlanRec r = recs[i];
+    const u64 before = base + r.before;
+    const bool served = trim_served(r, before, left, A.n_pages);
+    if (lane_id() == 0) {
+        A.len_out[i] = served ? r.new_len : r.len;
+        A.held_out[i] = served ? r.held - r.delta : r.held;
+        if (!served) atomicOr(A.status, r.flags ? r.flags : (uint32_t)kCachePool);
+    }
+    if (!served) return;
+    const int32_t* from = A.table + i * A.table_stride + (r.held - r.delta);
+    int32_t* to = A.free_pages + left + before;
+    for (int32_t j = lane_id(); j < r.delta; j += 64) to[j] = from[j];
+}
+
+// The whole call in one workgroup: at most kPlanThreads requests that hold kOnePages pages at the very most.
+constexpr uint64_t kOnePages = 16384;
+
+__global__ __launch_bounds__(kPlanThreads) void cache_trim_one_kernel(CacheArgs A) {
+    __shared__ u64 tmp[kPlanThreads / 64];
+    __shared__ uint32_t s_before[kPlanThreads], s_status, s_given;
+    __shared__ int32_t s_first[kPlanThreads];
+    const uint64_t i = threadIdx.x;
+    const int32_t n_free = *A.n_free;
+    const bool bad = n_free < 0 || (uint32_t)n_free > A.n_pages;
+    const u64 left = bad ? A.n_pages : (u64)n_free;
+    if (threadIdx.x == 0) { s_status = bad ? (uint32_t)kCacheBad : 0u; s_given = 0; }
+    PlanRec r{};
+    if (i < A.n) r = plan_trim(A.len[i], A.held[i], A.keep[i], A.page, A.max_pages);
+    u64 all;
+    const u64 before = block_escan64((u64)r.delta, tmp, &all);   // (at most kOnePages pages)
+    s_before[i] = (uint32_t)before;
+    s_first[i] = r.held - r.delta;
+    if (i < A.n) {
         const bool served = trim_served(r, before, left, A.n_pages);
-        if (lane_id() == 0) {
-            A.len_out[i] = served ? r.new_len : r.len;
-            A.held_out[i] = served ? r.held - r.delta : r.held;
-            if (!served) atomicOr(A.status, r.flags ? r.flags : (uint32_t)kCachePool);
-        }
-        if (!served) continue;
-        const int32_t* from = A.table + i * A.table_stride + (r.held - r.delta);
-        int32_t* to = A.free_pages + left + before;
-        for (int32_t j = lane_id(); j < r.delta; j += 64) to[j] = from[j];
+        A.len_out[i] = served ? r.new_len : r.len;
+        A.held_out[i] = served ? r.held - r.delta : r.held;
+        if (!served) atomicOr(&s_status, r.flags ? r.flags : (uint32_t)kCachePool);
+        else if (r.delta) atomicMax(&s_given, (uint32_t)(before + (u64)r.delta));
+    }
+    __syncthreads();
+    const uint32_t given = s_given;
+    for (uint32_t g = threadIdx.x; g < given; g += kPlanThreads) {
+        const uint32_t k = request_of_page(s_before, (uint32_t)A.n, g);
+        A.free_pages[left + g] = A.table[k * A.table_stride + (uint32_t)s_first[k] + (g - s_before[k])];
+    }
+    if (threadIdx.x == 0) {
+        *A.n_free_out = bad ? n_free : n_free + (int32_t)given;
+        *A.status = s_status;
     }
 }
 
@@ -162,24 +364,21 @@ Parts parts_of(const CacheArgs& A) {
 }  // namespace
 
 hipError_t launch_cache_slots(const CacheArgs& A, hipStream_t stream) {
+    if (A.n <= (uint64_t)kPlanThreads && A.cap <= kOneTokens) return launch(cache_slots_one_kernel, 1, kPlanThreads, stream, A);
     const Parts P = parts_of(A);
     hipError_t e = launch(cache_plan_kernel<false>, P.plan_blocks, kPlanThreads, stream, A, P.recs, P.blocks, P.head);
     if (e != hipSuccess) return e;
-    const uint64_t request_blocks = (A.n + kApplyThreads - 1) / kApplyThreads, token_blocks = (A.cap + kApplyThreads - 1) / kApplyThreads;
-    if (request_blocks + token_blocks)
-        e = launch(cache_slots_kernel, request_blocks + token_blocks, kApplyThreads, stream, A, (const PlanRec*)P.recs, (const u64*)P.blocks, (const CacheHead*)P.head,
-                   request_blocks);
-    if (e != hipSuccess) return e;
-    return launch(cache_count_kernel<false>, 1, kPlanThreads, stream, A, (const PlanRec*)P.recs, (const u64*)P.blocks, (const CacheHead*)P.head);
+    const uint64_t request_blocks = (A.n + kApplyWaves - 1) / kApplyWaves, token_blocks = A.n ? (A.cap + kTokenBlock - 1) / kTokenBlock : 0;
+    return launch(cache_slots_kernel, 1 + request_blocks + token_blocks, kApplyThreads, stream, A, (const PlanRec*)P.recs, (const u64*)P.blocks, (const CacheHead*)P.head,
+                  request_blocks);
 }
 
 hipError_t launch_cache_trim(const CacheArgs& A, hipStream_t stream) {
+    if (A.n <= (uint64_t)kPlanThreads && A.n * A.max_pages <= kOnePages) return launch(cache_trim_one_kernel, 1, kPlanThreads, stream, A);
     const Parts P = parts_of(A);
     hipError_t e = launch(cache_plan_kernel<true>, P.plan_blocks, kPlanThreads, stream, A, P.recs, P.blocks, P.head);
     if (e != hipSuccess) return e;
-    if (A.n) e = launch(cache_trim_kernel, (A.n + kApplyThreads / 64 - 1) / (kApplyThreads / 64), kApplyThreads, stream, A, (const PlanRec*)P.recs, (const u64*)P.blocks, (const CacheHead*)P.head);
-    if (e != hipSuccess) return e;
-    return launch(cache_count_kernel<true>, 1, kPlanThreads, stream, A, (const PlanRec*)P.recs, (const u64*)P.blocks, (const CacheHead*)P.head);
+    return launch(cache_trim_kernel, 1 + (A.n + kApplyWaves - 1) / kApplyWaves, kApplyThreads, stream, A, (const PlanRec*)P.recs, (const u64*)P.blocks, (const CacheHead*)P.head);
 }
 
 }  // namespace l3

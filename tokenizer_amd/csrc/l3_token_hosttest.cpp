@@ -13,7 +13,7 @@ const char* l3t_check_cache(const CacheArgs* A, int trim) { return check_cache(*
 const char* l3t_check_verify(const VerifyArgs* A) { return check_verify(*A); }
 uint64_t l3t_grad_work(uint64_t n, uint64_t dim) { return grad_work(n, dim).total; }
 uint64_t l3t_cache_work(uint64_t n) { return cache_work(n).total; }
-uint64_t l3t_verify_work(uint64_t n, uint64_t vocab) { return verify_work(n, vocab); }
+uint64_t l3t_verify_work(uint64_t n, uint64_t vocab) { return verify_work(n, vocab).total; }
 
 void l3t_cache_slots(const CacheArgs* P) {
     const CacheArgs& A = *P;

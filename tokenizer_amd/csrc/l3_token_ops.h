@@ -14,6 +14,8 @@ L3_HD int dtype_size(int t) { return t == kF32 ? 4 : 2; }
 
 constexpr uint64_t kMaxCount = 0x7FFFFFFFull;    // ids, rows, tokens, pages: 31 bits
 constexpr uint64_t kMaxDim = 1ull << 24;
+constexpr uint64_t kMaxGradIds = 1ull << 24;     // ids sorted in one call: every tile adds up the counts of all tiles before it
+constexpr uint64_t kMaxGradRows = 1ull << 29;    // rows of a gradient: one workgroup for 64 of them
 constexpr uint64_t kMaxSeqs = 1ull << 20;
 constexpr uint64_t kMaxStride = kMaxCount;       // elements: (2^31 - 1) rows of (2^31 - 1) elements of 4 bytes stay inside 64 bits
 
@@ -62,13 +64,15 @@ struct VerifyArgs {
 constexpr uint64_t align256(uint64_t b) { return (b + 255) & ~255ull; }
 
 // Ids are sorted in tiles of kSortTile by digits of at most kSortBits bits.
-constexpr int kSortTile = 4096, kSortBits = 9, kSortBins = 1 << kSortBits;
+constexpr int kSortTile = 2048, kSortBits = 9, kSortBins = 1 << kSortBits;
+// Up to kDirectIds ids are not sorted: every position looks for the others of its id by itself.
+constexpr uint64_t kDirectIds = 2048;
 // Sorted positions one walker adds up.
-inline uint32_t grad_chunk(uint64_t n, uint64_t dim) { (void)dim; return n >= 32768 ? 64 : n >= 4096 ? 16 : 8; }
+inline uint32_t grad_chunk(uint64_t n) { return n >= 32768 ? 64 : n >= 8192 ? 16 : 8; }
 struct GradWork { uint64_t keys0, pos0, keys1, pos1, hist, part, total; uint32_t chunk; uint64_t chunks, dim8; };
 inline GradWork grad_work(uint64_t n, uint64_t dim) {
     GradWork w;
-    w.chunk = grad_chunk(n, dim);
+    w.chunk = grad_chunk(n);
     w.chunks = (n + w.chunk - 1) / w.chunk;
     w.dim8 = (dim + 7) & ~7ull;
     uint64_t at = 0;
@@ -101,8 +105,16 @@ inline CacheWork cache_work(uint64_t n) {
 }
 
 constexpr int kVerifyChunk = 2048;   // entries of a row one workgroup adds up
-inline uint64_t verify_chunks(uint64_t vocab) { return (vocab + kVerifyChunk - 1) / kVerifyChunk; }
-inline uint64_t verify_work(uint64_t n, uint64_t vocab) { return n ? align256(n * verify_chunks(vocab) * 16) : 256; }
+struct VerifyVerdict { int32_t state; uint32_t a; uint64_t p_row, q_row; int32_t token; int32_t pad; };   // (l3_verify.hip)
+struct VerifyWork { uint64_t sums, verdicts, total, chunks; };
+inline VerifyWork verify_work(uint64_t n, uint64_t vocab) {
+    VerifyWork w;
+    w.chunks = (vocab + kVerifyChunk - 1) / kVerifyChunk;
+    w.sums = 0;
+    w.verdicts = align256(n * w.chunks * 16);
+    w.total = w.verdicts + align256((n ? n : 1) * sizeof(VerifyVerdict));
+    return w;
+}
 
 // ---- checks: null, or what is wrong -------------------------------------------------------------------------------
 inline bool bad_dtype(int t) { return t != kF32 && t != kF16 && t != kBF16; }
@@ -123,8 +135,8 @@ inline const char* check_embed(const EmbedArgs& A) {
 
 inline const char* check_embed_grad(const EmbedGradArgs& A) {
     if (bad_dtype(A.dtype) || bad_dtype(A.table_dtype)) return "unknown element type";
-    if (A.n > kMaxCount) return "more than 2^31 - 1 ids: split the call";
-    if (A.rows == 0 || A.rows > kMaxCount) return "n_rows must be 1 .. 2^31 - 1";
+    if (A.n > kMaxGradIds) return "more than 2^24 ids: split the call";
+    if (A.rows == 0 || A.rows > kMaxGradRows) return "n_rows must be 1 .. 2^29";
     if (A.dim == 0 || A.dim > kMaxDim) return "dim must be 1 .. 2^24";
     if (A.grad_stride < A.dim || A.table_stride < A.dim || A.grad_stride > kMaxStride || A.table_stride > kMaxStride)
         return "a row stride is smaller than dim or above 2^31 - 1";
@@ -177,7 +189,7 @@ inline const char* check_verify(const VerifyArgs& A) {
         misaligned(A.accepted, 4) || misaligned(A.target, dtype_size(A.dtype)) || misaligned(A.q, dtype_size(A.dtype)))
         return "a pointer is not aligned to its element";
     if (misaligned(A.work, 16)) return "the workspace must be aligned to 16 bytes";
-    if (A.work_bytes < verify_work(A.n, A.vocab)) return "workspace too small (l3_verify_workspace)";
+    if (A.work_bytes < verify_work(A.n, A.vocab).total) return "workspace too small (l3_verify_workspace)";
     return nullptr;
 }
 
