@@ -6,6 +6,8 @@
 // Products and sums are in 32 bits, rounded once where they are stored.
 #include "l3_token_kernels.h"
 
+#include <type_traits>
+
 #include "l3_dev.h"
 
 namespace l3 {
@@ -18,56 +20,72 @@ __device__ __forceinline__ uint64_t ids_that_count(uint64_t n, const uint64_t* n
     return m < n ? m : n;
 }
 
-// Eight columns from `col` on of a row of `dim`.
-template <class T>
-__device__ __forceinline__ void load_cols(const T* p, uint32_t col, uint32_t dim, float* v) {
-    if (col + 8 <= dim) { load8(p + col, v); return; }
+// A row is worked on in vectors of eight columns.  The last of a row whose width is no multiple of eight begins `skip` columns
+// early, so that every load has eight elements; those columns belong to the vector before.  Rows of fewer than eight columns
+// (SMALL) are loaded one element at a time.
+struct Cols { uint32_t col, skip; };
+__device__ __forceinline__ Cols cols_of(uint32_t vec, uint32_t dim) {
+    const uint32_t c = vec * 8;
+    if (c + 8 <= dim || dim < 8) return {c, 0};
+    return {dim - 8, c + 8 - dim};
+}
+template <bool SMALL, class T>
+__device__ __forceinline__ typename Eight<T>::V load_cols(const T* row, Cols c, uint32_t dim) {
+    if constexpr (SMALL) {
+        typename Eight<T>::V v = (T)0.f;
+        for (uint32_t i = 0; i < 8; i++) if (i < dim) v[i] = row[i];
+        return v;
+    } else {
+        return load8(row + c.col);
+    }
+}
+// The vector's own columns; SHARED: the skipped ones hold the same values as their owner stores.
+template <bool SMALL, bool SHARED, class T>
+__device__ __forceinline__ void store_cols(T* row, Cols c, uint32_t dim, F8 v) {
+    if constexpr (SMALL) {
+        for (uint32_t i = 0; i < 8; i++) if (i < dim) row[i] = (T)v[i];
+    } else if (SHARED || c.skip == 0) {
+        store8(row + c.col, v);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = col + i < dim ? (float)p[col + i] : 0.f;
+        for (uint32_t i = 1; i < 8; i++) if (i >= c.skip) row[c.col + i] = (T)v[i];
+    }
 }
-template <class T>
-__device__ __forceinline__ void store_cols(T* p, uint32_t col, uint32_t dim, const float* v) {
-    if (col + 8 <= dim) { store8(p + col, v); return; }
-    for (int i = 0; i < 8; i++) if (col + i < dim) p[col + i] = (T)v[i];
-}
-// ---- lookup -------------------------------------------------------------------------------------------------------
-// A thread has kEmbedPer times eight neighbouring columns, all loads in flight before the first store.  What is divided is a
-// workgroup's first vector (once) and 32-bit offsets from it.
-constexpr int kEmbedThreads = 256, kEmbedPer = 4, kEmbedTile = kEmbedThreads * kEmbedPer;
 
-template <class T, class O>
+// ---- lookup -------------------------------------------------------------------------------------------------------
+// A thread has PER times eight neighbouring columns, all loads in flight before the first store.  What is divided is a workgroup's
+// first vector (once) and 32-bit offsets from it.
+constexpr int kEmbedThreads = 256;
+constexpr uint64_t kEmbedMany = 1u << 20;   // vectors from which a thread has four
+
+template <class T, class O, int PER, bool SMALL>
 __global__ __launch_bounds__(kEmbedThreads) void embed_kernel(const int32_t* __restrict__ ids, uint64_t n, const uint64_t* __restrict__ n_dev,
                                                               const T* __restrict__ table, uint32_t rows, uint32_t dim, uint64_t stride,
                                                               O* __restrict__ out, uint64_t out_stride, float scale) {
+    constexpr uint32_t kTile = kEmbedThreads * PER;
     const uint32_t per_row = (dim + 7) / 8;
     const uint64_t count = ids_that_count(n, n_dev), total = count * per_row;
-    for (uint64_t g0 = (uint64_t)blockIdx.x * kEmbedTile; g0 < total; g0 += (uint64_t)gridDim.x * kEmbedTile) {
+    for (uint64_t g0 = (uint64_t)blockIdx.x * kTile; g0 < total; g0 += (uint64_t)gridDim.x * kTile) {
         const uint64_t t0 = g0 / per_row;
         const uint32_t r0 = (uint32_t)(g0 - t0 * per_row);
-        uint64_t t[kEmbedPer];
-        uint32_t col[kEmbedPer];
-        int32_t id[kEmbedPer];
-        float v[kEmbedPer][8];
+        uint64_t t[PER];
+        Cols c[PER];
+        int32_t id[PER];
+        typename Eight<T>::V v[PER];
 #pragma unroll
-        for (int k = 0; k < kEmbedPer; k++) {
+        for (int k = 0; k < PER; k++) {
             const uint32_t at = r0 + k * kEmbedThreads + threadIdx.x, row = at / per_row;
             t[k] = t0 + row;
-            col[k] = (at - row * per_row) * 8;
-            id[k] = t[k] < count ? ids[t[k]] : -1;
+            c[k] = cols_of(at - row * per_row, dim);
+            id[k] = ids[t[k] < count ? t[k] : count - 1];
         }
 #pragma unroll
-        for (int k = 0; k < kEmbedPer; k++) {
+        for (int k = 0; k < PER; k++)   // (an id that is no row loads row 0 and stores zeros)
+            v[k] = load_cols<SMALL>(table + (uint64_t)((uint32_t)id[k] < rows ? (uint32_t)id[k] : 0u) * stride, c[k], dim);
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[k][i] = 0.f;
-            if (id[k] >= 0 && (uint32_t)id[k] < rows) load_cols(table + (uint64_t)(uint32_t)id[k] * stride, col[k], dim, v[k]);
-        }
-#pragma unroll
-        for (int k = 0; k < kEmbedPer; k++) {
-            if (t[k] >= count) continue;
-            const bool there = id[k] >= 0 && (uint32_t)id[k] < rows;
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[k][i] = there ? v[k][i] * scale : 0.f;   // (a row of zeros whatever the scale is)
-            store_cols(out + t[k] * out_stride, col[k], dim, v[k]);
+        for (int k = 0; k < PER; k++) {
+            const F8 x = to_f8(v[k]) * scale;
+            if (t[k] < count) store_cols<SMALL, true>(out + t[k] * out_stride, c[k], dim, (uint32_t)id[k] < rows ? x : (F8)0.f);
         }
     }
 }
@@ -173,126 +191,106 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const int32_t*
 }
 
 // ---- gradient: runs of one id added up ----------------------------------------------------------------------------
-// A walker goes through `chunk` sorted positions for eight columns a thread, in order, four at a time: the four rows of the
-// gradient and, where a run of one id ends, the row of the table it is added to are loaded together.  A run that lies inside the
-// chunk is stored at once.  A run that crosses a border leaves its part in the workspace: part[2 c] of the run that came in
-// from the chunk before, part[2 c + 1] of the run that starts here and goes on; grad_join_kernel adds these up at the chunk
-// where the run starts.  Nothing is added by atomics: the same ids give the same bits.
-constexpr int kGradThreads = 256, kGradGroup = 4;
+// A wave walks through `chunk` sorted positions for 512 columns, in order, four at a time: the four rows of the gradient and, where
+// a run of one id ends, the row of the table it is added to are loaded together.  Keys and positions of the whole chunk are in
+// one register each (lane j has position j).  A run that lies inside the chunk is stored at once.  A run that crosses a border
+// leaves its part in the workspace: part[2 c] of the run that came in from the chunk before, part[2 c + 1] of the run that starts
+// here and goes on; grad_join_kernel adds these up at the chunk where the run starts.  Nothing is added by atomics: the same ids
+// give the same bits.
+constexpr int kGradThreads = 256, kGradWaves = kGradThreads / 64, kGradGroup = 4;
+constexpr uint32_t kGradCols = 512;
 constexpr uint32_t kZeroRows = 64;   // rows a workgroup looks after when the gradient is written whole
 
-// lanes of a row, a power of two
-inline uint32_t grad_lanes(uint64_t dim) {
-    const uint64_t v = (dim + 7) / 8;
-    uint32_t l = 1;
-    while (l < v && l < (uint32_t)kGradThreads) l *= 2;
-    return l;
-}
-
-template <class T>
-__device__ __forceinline__ void add_scaled(const float* old, const float* sum, float scale, float* v) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = old[i] + scale * sum[i];
-}
-
 // Rows [r0, r0 + kZeroRows) of which `named` has no bit become zero; by a whole workgroup.
-template <class T>
+template <bool SMALL, class T>
 __device__ __forceinline__ void zero_rows(T* table, uint64_t table_stride, uint64_t rows, uint32_t dim, uint64_t r0, u64 named) {
     static_assert(kZeroRows == 64, "a word of bits");
-    const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     const uint32_t per_row = (dim + 7) / 8;
-    for (uint32_t j = wave_id(); j < kZeroRows && r0 + j < rows; j += kGradThreads / 64) {
+    for (uint32_t j = wave_id(); j < kZeroRows && r0 + j < rows; j += kGradWaves) {
         if ((named >> j) & 1) continue;
-        for (uint32_t k = lane_id(); k < per_row; k += 64) store_cols(table + (r0 + j) * table_stride, k * 8, dim, zero);
+        for (uint32_t k = lane_id(); k < per_row; k += 64) store_cols<SMALL, true>(table + (r0 + j) * table_stride, cols_of(k, dim), dim, (F8)0.f);
     }
 }
 
 struct GradWalk {
-    const uint32_t* keys; const uint32_t* poss; uint64_t n; uint32_t rows;
-    uint32_t chunk; uint64_t chunks; uint32_t lanes, col_tiles; uint64_t walk_blocks;
-    const void* grad; uint64_t grad_stride; uint32_t dim;
-    void* table; uint64_t table_stride;
+    uint64_t n; uint32_t rows;
+    uint32_t chunk; uint64_t chunks; uint32_t tiles; uint64_t walk_blocks;
+    uint64_t grad_stride; uint32_t dim;
+    uint64_t table_stride;
     float scale; int accumulate;
-    float* part; uint64_t dim8;
+    uint64_t dim8;
 };
 
-template <class G, class T>
-__global__ __launch_bounds__(kGradThreads) void grad_walk_kernel(GradWalk P) {
-    const G* __restrict__ grad = (const G*)P.grad;
-    T* __restrict__ table = (T*)P.table;
-    const uint32_t* __restrict__ keys = P.keys;
-    const uint32_t* __restrict__ poss = P.poss;
+__device__ __forceinline__ uint32_t of_lane(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
+
+template <class G, class T, bool SMALL>
+__global__ __launch_bounds__(kGradThreads) void grad_walk_kernel(GradWalk P, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ poss,
+                                                                 const G* __restrict__ grad, T* __restrict__ table, float* __restrict__ part) {
     const uint32_t rows = P.rows, dim = P.dim;
     if (blockIdx.x >= P.walk_blocks) {   // rows that no id names, when the gradient is written whole: a binary search a row
         const uint64_t r0 = (uint64_t)(blockIdx.x - P.walk_blocks) * kZeroRows;
         const uint32_t r = (uint32_t)r0 + lane_id();
         uint64_t a = 0, b = P.n;
         while (a < b) { const uint64_t m = (a + b) / 2; if (keys[m] < r) a = m + 1; else b = m; }
-        zero_rows(table, P.table_stride, rows, dim, r0, __ballot(a < P.n && keys[a] == r));
+        zero_rows<SMALL>(table, P.table_stride, rows, dim, r0, __ballot(a < P.n && keys[a] == r));
         return;
     }
-    const uint32_t walkers = kGradThreads / P.lanes;
-    uint32_t me = threadIdx.x / P.lanes;
-    if (P.lanes >= 64) me = (uint32_t)__builtin_amdgcn_readfirstlane((int)me);   // keys and positions are the wave's: scalar loads
-    const uint64_t c = (uint64_t)(blockIdx.x / P.col_tiles) * walkers + me;
-    const uint32_t col = ((blockIdx.x % P.col_tiles) * P.lanes + threadIdx.x % P.lanes) * 8;
-    if (c >= P.chunks || col >= dim) return;
-    const uint64_t lo = c * P.chunk, hi = lo + P.chunk < P.n ? lo + P.chunk : P.n;
-    if (keys[lo] >= rows) return;
-    // the run that came in, if one did
-    const uint32_t came_in = lo > 0 && keys[lo - 1] == keys[lo] ? keys[lo] : ~0u;
-    float sum[8];
+    const uint64_t wave = (uint64_t)blockIdx.x * kGradWaves + (uint32_t)__builtin_amdgcn_readfirstlane((int)wave_id());
+    const uint64_t c = wave / P.tiles, lo = c * P.chunk;
+    if (c >= P.chunks) return;
+    const uint32_t vec = (uint32_t)(wave - c * P.tiles) * 64 + lane_id(), len = lo + P.chunk < P.n ? P.chunk : (uint32_t)(P.n - lo);
+    const uint32_t key = (uint32_t)lane_id() < len ? keys[lo + lane_id()] : ~0u, pos = (uint32_t)lane_id() < len ? poss[lo + lane_id()] : 0;
+    // the key behind the chunk, and the run that came in, if one did
+    const uint32_t behind = lo + len < P.n ? keys[lo + len] : ~0u, head = of_lane(key, 0), in_front = lo ? keys[lo - 1] : ~0u;
+    const uint32_t came_in = head == in_front ? head : ~0u;
+    const uint32_t used = (uint32_t)__popcll(__ballot(key < rows));   // ids that are no rows come last
+    if (used == 0) return;
+    const bool mine = vec * 8 < dim;
+    const Cols at = cols_of(mine ? vec : 0, dim);
+    F8 sum = 0.f;
+    for (uint32_t i = 0; i < used; i += kGradGroup) {
+        uint32_t k[kGradGroup + 1];
+        typename Eight<G>::V g[kGradGroup];
+        typename Eight<T>::V old[kGradGroup];
 #pragma unroll
-    for (int i = 0; i < 8; i++) sum[i] = 0.f;
-    for (uint64_t i = lo; i < hi; i += kGradGroup) {
-        uint32_t k[kGradGroup + 1], pos[kGradGroup];
-#pragma unroll
-        for (int j = 0; j <= kGradGroup; j++) k[j] = i + j < P.n ? keys[i + j] : ~0u;
-#pragma unroll
-        for (int j = 0; j < kGradGroup; j++) pos[j] = i + j < hi ? poss[i + j] : 0;
-        float g[kGradGroup][8], old[kGradGroup][8];
-        bool use[kGradGroup], end[kGradGroup];
+        for (int j = 0; j <= kGradGroup; j++) k[j] = i + j < len ? of_lane(key, i + j) : behind;
 #pragma unroll
         for (int j = 0; j < kGradGroup; j++) {
-            use[j] = i + j < hi && k[j] < rows;
-            end[j] = use[j] && k[j + 1] != k[j];
-            if (use[j]) load_cols(grad + (uint64_t)pos[j] * P.grad_stride, col, dim, g[j]);
-#pragma unroll
-            for (int x = 0; x < 8; x++) old[j][x] = 0.f;
-            if (end[j] && k[j] != came_in && P.accumulate) load_cols(table + (uint64_t)k[j] * P.table_stride, col, dim, old[j]);
+            const uint32_t x = i + j < used ? i + j : used - 1;
+            g[j] = load_cols<SMALL>(grad + (uint64_t)of_lane(pos, x) * P.grad_stride, at, dim);
         }
 #pragma unroll
         for (int j = 0; j < kGradGroup; j++) {
-            if (!use[j]) continue;
+            old[j] = (T)0.f;
+            if (i + j < used && k[j + 1] != k[j] && k[j] != came_in && P.accumulate) old[j] = load_cols<SMALL>(table + (uint64_t)k[j] * P.table_stride, at, dim);
+        }
 #pragma unroll
-            for (int x = 0; x < 8; x++) sum[x] += g[j][x];
-            if (!end[j]) continue;
-            if (k[j] == came_in) {
-                store8(P.part + (2 * c) * P.dim8 + col, sum);
-            } else {
-                float v[8];
-                add_scaled<T>(old[j], sum, P.scale, v);
-                store_cols(table + (uint64_t)k[j] * P.table_stride, col, dim, v);
+        for (int j = 0; j < kGradGroup; j++) {
+            if (i + j >= used) break;
+            sum += to_f8(g[j]);
+            if (k[j + 1] == k[j]) continue;
+            if (mine) {
+                if (k[j] == came_in) store8(part + (2 * c) * P.dim8 + vec * 8, sum);
+                else store_cols<SMALL, false>(table + (uint64_t)k[j] * P.table_stride, at, dim, to_f8(old[j]) + sum * P.scale);
             }
-#pragma unroll
-            for (int x = 0; x < 8; x++) sum[x] = 0.f;
+            sum = 0.f;
         }
     }
-    const uint32_t last = keys[hi - 1];
-    if (last < rows && hi < P.n && keys[hi] == last) store8(P.part + (2 * c + (last == came_in ? 0 : 1)) * P.dim8 + col, sum);
+    const uint32_t last = of_lane(key, len - 1);
+    if (mine && last < rows && last == behind) store8(part + (2 * c + (last == came_in ? 0 : 1)) * P.dim8 + vec * 8, sum);
 }
 
 // Parts of long runs: a workgroup per chunk and 512 columns, every wave a quarter of the parts, four loads in flight.
-template <class T>
-__global__ __launch_bounds__(kGradThreads) void grad_join_kernel(GradWalk P, uint32_t tiles) {
-    __shared__ float acc[kGradThreads / 64 - 1][64][8];
-    const uint32_t* __restrict__ keys = P.keys;
-    const uint64_t c = blockIdx.x / tiles;
-    const uint32_t col = (blockIdx.x % tiles) * 512 + lane_id() * 8;
+template <class T, bool SMALL>
+__global__ __launch_bounds__(kGradThreads) void grad_join_kernel(GradWalk P, const uint32_t* __restrict__ keys, T* __restrict__ table,
+                                                                 const float* __restrict__ part) {
+    __shared__ F8 acc[kGradWaves - 1][64];
+    const uint64_t c = blockIdx.x / P.tiles;
+    const uint32_t vec = (blockIdx.x % P.tiles) * 64 + lane_id();
     const uint64_t lo = c * P.chunk, hi = lo + P.chunk;
     if (hi >= P.n) return;
-    const uint32_t k = keys[hi - 1];
-    if (k >= P.rows || keys[hi] != k || (lo > 0 && keys[lo - 1] == k)) return;
+    const uint32_t k = keys[hi - 1], behind = keys[hi], in_front = lo ? keys[lo - 1] : ~0u;
+    if (k >= P.rows || behind != k || in_front == k) return;
     uint64_t more = 0;   // chunks behind c that the run comes into
     for (;;) {
         const uint64_t d = c + 1 + more + lane_id();
@@ -301,44 +299,30 @@ __global__ __launch_bounds__(kGradThreads) void grad_join_kernel(GradWalk P, uin
         more += (uint64_t)__builtin_ctzll(~m);
         break;
     }
-    const int w = wave_id();
-    T* row = (T*)P.table + (uint64_t)k * P.table_stride;
-    const bool in = col < P.dim;
-    float sum[8], old[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) sum[i] = old[i] = 0.f;
-    if (in) {
-        if (w == 0) {
-            if (P.accumulate) load_cols(row, col, P.dim, old);
-            load8(P.part + (2 * c + 1) * P.dim8 + col, sum);
-        }
-        const uint64_t d1 = c + 1 + more * (w + 1) / 4;
-        for (uint64_t d = c + 1 + more * w / 4; d < d1; d += 4) {
-            float v[4][8];
-#pragma unroll
-            for (int j = 0; j < 4; j++) if (d + j < d1) load8(P.part + 2 * (d + j) * P.dim8 + col, v[j]);
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if (d + j < d1) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) sum[i] += v[j][i];
-                }
-            }
-        }
+    const int w = __builtin_amdgcn_readfirstlane((int)wave_id());
+    const bool mine = vec * 8 < P.dim;
+    const Cols at = cols_of(mine ? vec : 0, P.dim);
+    T* row = table + (uint64_t)k * P.table_stride;
+    const float* from = part + (mine ? vec : 0) * 8;
+    typename Eight<T>::V old = (T)0.f;
+    F8 sum = 0.f;
+    if (w == 0) {
+        if (P.accumulate) old = load_cols<SMALL>(row, at, P.dim);
+        sum = load8(from + (2 * c + 1) * P.dim8);
     }
-    if (w) {
+    const uint64_t d1 = c + 1 + more * (w + 1) / kGradWaves;
+    for (uint64_t d = c + 1 + more * w / kGradWaves; d < d1; d += 4) {
+        F8 v[4];
 #pragma unroll
-        for (int i = 0; i < 8; i++) acc[w - 1][lane_id()][i] = sum[i];
+        for (int j = 0; j < 4; j++) v[j] = load8(from + 2 * (d + j < d1 ? d + j : d1 - 1) * P.dim8);
+#pragma unroll
+        for (int j = 0; j < 4; j++) if (d + j < d1) sum += v[j];
     }
+    if (w) acc[w - 1][lane_id()] = sum;
     __syncthreads();
-    if (w || !in) return;
-    for (int x = 0; x < kGradThreads / 64 - 1; x++) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) sum[i] += acc[x][lane_id()][i];
-    }
-    float v[8];
-    add_scaled<T>(old, sum, P.scale, v);
-    store_cols(row, col, P.dim, v);
+    if (w || !mine) return;
+    for (int x = 0; x < kGradWaves - 1; x++) sum += acc[x][lane_id()];
+    store_cols<SMALL, false>(row, at, P.dim, to_f8(old) + sum * P.scale);
 }
 
 // ---- gradient: few ids --------------------------------------------------------------------------------------------
@@ -347,43 +331,36 @@ __global__ __launch_bounds__(kGradThreads) void grad_join_kernel(GradWalk P, uin
 // positions and the waves' sums are added in order.
 constexpr int kDirectMany = 8, kDirectWords = (int)(kDirectIds / 64);
 
-template <class G>
-__device__ __forceinline__ void add_named(const G* __restrict__ grad, uint64_t stride, uint32_t col, uint32_t dim, const u64* words, int first, int step,
-                                          float* sum) {
+template <bool SMALL, class G>
+__device__ __forceinline__ F8 add_named(const G* __restrict__ grad, uint64_t stride, Cols at, uint32_t dim, const u64* words, int first, int step) {
+    F8 sum = 0.f;
     for (int x = first; x < kDirectWords; x += step) {
         u64 m = words[x];
         m = (u64)(uint32_t)__builtin_amdgcn_readfirstlane((int)(m >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)m);   // the wave's own
         while (m) {
-            float g[4][8];
-            bool on[4];
+            typename Eight<G>::V g[4];
+            uint32_t p = 0;
+            const int have = __popcll(m);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                on[j] = m != 0;
-                if (on[j]) {
-                    const uint32_t pos = (uint32_t)x * 64 + (uint32_t)__builtin_ctzll(m);
-                    m &= m - 1;
-                    load_cols(grad + (uint64_t)pos * stride, col, dim, g[j]);
-                }
+                if (m) { p = (uint32_t)x * 64 + (uint32_t)__builtin_ctzll(m); m &= m - 1; }
+                g[j] = load_cols<SMALL>(grad + (uint64_t)p * stride, at, dim);
             }
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if (on[j]) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) sum[i] += g[j][i];
-                }
-            }
+            for (int j = 0; j < 4; j++) if (j < have) sum += to_f8(g[j]);
         }
     }
+    return sum;
 }
 
-template <class G, class T>
+template <class G, class T, bool SMALL>
 __global__ __launch_bounds__(kGradThreads) void grad_direct_kernel(const int32_t* __restrict__ ids, uint32_t n, const uint64_t* n_dev, uint32_t rows,
                                                                    const G* __restrict__ grad, uint64_t grad_stride, uint32_t dim,
                                                                    T* __restrict__ table, uint64_t table_stride, float scale, int accumulate) {
     __shared__ u64 words[kDirectWords];
-    __shared__ float acc[kGradThreads / 64 - 1][64][8];
+    __shared__ F8 acc[kGradWaves - 1][64];
     const uint32_t valid = (uint32_t)ids_that_count(n, n_dev);
-    const int w = wave_id(), lane = lane_id();
+    const int w = __builtin_amdgcn_readfirstlane((int)wave_id()), lane = lane_id();
     if (blockIdx.x >= n) {   // rows that no id names, when the gradient is written whole
         const uint64_t r0 = (uint64_t)(blockIdx.x - n) * kZeroRows;
         if (threadIdx.x == 0) words[0] = 0;
@@ -393,75 +370,80 @@ __global__ __launch_bounds__(kGradThreads) void grad_direct_kernel(const int32_t
             if (d < kZeroRows) atomicOr(&words[0], 1ull << d);
         }
         __syncthreads();
-        zero_rows(table, table_stride, rows, dim, r0, words[0]);
+        zero_rows<SMALL>(table, table_stride, rows, dim, r0, words[0]);
         return;
     }
     const uint32_t t = blockIdx.x;
     if (t >= valid) return;
     const int32_t id = ids[t];
     if (id < 0 || (uint32_t)id >= rows) return;
+    int32_t other[kDirectWords / kGradWaves];
+#pragma unroll
+    for (int y = 0; y < kDirectWords / kGradWaves; y++) {
+        const uint32_t j = (uint32_t)(y * kGradWaves + w) * 64 + lane;
+        other[y] = j < valid ? ids[j] : -1;
+    }
     bool earlier = false;
     int many = 0;
 #pragma unroll
-    for (int x0 = 0; x0 < kDirectWords; x0 += kGradThreads / 64) {
-        const int x = x0 + w;
-        const uint32_t j = (uint32_t)x * 64 + lane;
-        const u64 m = __ballot(j < valid && ids[j] == id);
+    for (int y = 0; y < kDirectWords / kGradWaves; y++) {
+        const int x = y * kGradWaves + w;
+        const u64 m = __ballot(other[y] == id);
         if (lane == 0) words[x] = m;
         if (m && (uint32_t)x * 64 + (uint32_t)__builtin_ctzll(m) < t) earlier = true;
         many += __popcll(m);
     }
     if (__syncthreads_or(earlier)) return;
+    T* row = table + (uint64_t)(uint32_t)id * table_stride;
+    const uint32_t per_row = (dim + 7) / 8;
     if (!__syncthreads_or(many > kDirectMany)) {   // (of one wave's words: at most four times as many in all)
-        for (uint32_t col = (uint32_t)threadIdx.x * 8; col < dim; col += kGradThreads * 8) {
-            float sum[8], old[8], v[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) sum[i] = old[i] = 0.f;
-            T* row = table + (uint64_t)(uint32_t)id * table_stride;
-            if (accumulate) load_cols(row, col, dim, old);
-            add_named(grad, grad_stride, col, dim, words, 0, 1, sum);
-            add_scaled<T>(old, sum, scale, v);
-            store_cols(row, col, dim, v);
+        for (uint32_t vec = threadIdx.x; vec < per_row; vec += kGradThreads) {
+            const Cols at = cols_of(vec, dim);
+            typename Eight<T>::V old = (T)0.f;
+            if (accumulate) old = load_cols<SMALL>(row, at, dim);
+            const F8 sum = add_named<SMALL>(grad, grad_stride, at, dim, words, 0, 1);
+            store_cols<SMALL, false>(row, at, dim, to_f8(old) + sum * scale);
         }
         return;
     }
-    for (uint32_t c0 = 0; c0 < dim; c0 += 512) {
-        const uint32_t col = c0 + (uint32_t)lane * 8;
-        const bool in = col < dim;
-        float sum[8], old[8], v[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) sum[i] = old[i] = 0.f;
-        T* row = table + (uint64_t)(uint32_t)id * table_stride;
-        if (in && w == 0 && accumulate) load_cols(row, col, dim, old);
-        if (in) add_named(grad, grad_stride, col, dim, words, w, kGradThreads / 64, sum);
-        if (w) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) acc[w - 1][lane][i] = sum[i];
-        }
+    for (uint32_t v0 = 0; v0 < per_row; v0 += 64) {
+        const uint32_t vec = v0 + (uint32_t)lane;
+        const bool mine = vec < per_row;
+        const Cols at = cols_of(mine ? vec : 0, dim);
+        typename Eight<T>::V old = (T)0.f;
+        if (w == 0 && accumulate) old = load_cols<SMALL>(row, at, dim);
+        F8 sum = add_named<SMALL>(grad, grad_stride, at, dim, words, w, kGradWaves);
+        if (w) acc[w - 1][lane] = sum;
         __syncthreads();
-        if (w == 0 && in) {
-            for (int x = 0; x < kGradThreads / 64 - 1; x++) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) sum[i] += acc[x][lane][i];
-            }
-            add_scaled<T>(old, sum, scale, v);
-            store_cols(row, col, dim, v);
+        if (w == 0 && mine) {
+            for (int x = 0; x < kGradWaves - 1; x++) sum += acc[x][lane];
+            store_cols<SMALL, false>(row, at, dim, to_f8(old) + sum * scale);
         }
         __syncthreads();
     }
+}
+
+// f(std::true_type / false_type): rows of fewer than eight columns, or not
+template <class F>
+hipError_t with_small(uint64_t dim, F f) {
+    return dim < 8 ? f(std::true_type()) : f(std::false_type());
 }
 
 }  // namespace
 
 hipError_t launch_embed(const EmbedArgs& A, hipStream_t stream) {
     if (A.n == 0) return hipSuccess;
-    const uint64_t blocks = capped((A.n * ((A.dim + 7) / 8) + kEmbedTile - 1) / kEmbedTile);
+    const uint64_t vectors = A.n * ((A.dim + 7) / 8);
     return with_dtype(A.dtype, [&](auto t) {
         typedef decltype(t) T;
         return with_dtype(A.out_dtype, [&](auto o) {
             typedef decltype(o) O;
-            return launch(embed_kernel<T, O>, blocks, kEmbedThreads, stream, A.ids, A.n, A.n_dev, (const T*)A.table, (uint32_t)A.rows, (uint32_t)A.dim, A.stride,
-                          (O*)A.out, A.out_stride, A.scale);
+            return with_small(A.dim, [&](auto small) {
+                const bool many = vectors >= kEmbedMany;
+                const uint64_t tile = kEmbedThreads * (many ? 4 : 1);
+                return launch(many ? embed_kernel<T, O, 4, small.value> : embed_kernel<T, O, 1, small.value>, capped((vectors + tile - 1) / tile), kEmbedThreads, stream,
+                              A.ids, A.n, A.n_dev, (const T*)A.table, (uint32_t)A.rows, (uint32_t)A.dim, A.stride, (O*)A.out, A.out_stride, A.scale);
+            });
         });
     });
 }
@@ -469,15 +451,18 @@ hipError_t launch_embed(const EmbedArgs& A, hipStream_t stream) {
 hipError_t launch_embed_grad(const EmbedGradArgs& A, hipStream_t stream) {
     const uint32_t rows = (uint32_t)A.rows, dim = (uint32_t)A.dim;
     const uint64_t zero_blocks = A.accumulate ? 0 : (A.rows + kZeroRows - 1) / kZeroRows;
+    auto with_types = [&](auto f) {
+        return with_dtype(A.table_dtype, [&](auto t) {
+            return with_dtype(A.dtype, [&](auto g) { return with_small(A.dim, [&](auto small) { return f(g, t, small); }); });
+        });
+    };
     if (A.n <= kDirectIds) {
         if (A.n + zero_blocks == 0) return hipSuccess;
-        return with_dtype(A.table_dtype, [&](auto t) {
+        return with_types([&](auto g, auto t, auto small) {
+            typedef decltype(g) G;
             typedef decltype(t) T;
-            return with_dtype(A.dtype, [&](auto g) {
-                typedef decltype(g) G;
-                return launch(grad_direct_kernel<G, T>, A.n + zero_blocks, kGradThreads, stream, A.ids, (uint32_t)A.n, A.n_dev, rows, (const G*)A.grad, A.grad_stride, dim,
-                              (T*)A.table, A.table_stride, A.scale, A.accumulate);
-            });
+            return launch(grad_direct_kernel<G, T, small.value>, A.n + zero_blocks, kGradThreads, stream, A.ids, (uint32_t)A.n, A.n_dev, rows, (const G*)A.grad,
+                          A.grad_stride, dim, (T*)A.table, A.table_stride, A.scale, A.accumulate);
         });
     }
     const GradWork W = grad_work(A.n, A.dim);
@@ -499,19 +484,17 @@ hipError_t launch_embed_grad(const EmbedGradArgs& A, hipStream_t stream) {
         if (e != hipSuccess) return e;
     }
     const int to = (passes - 1) & 1;
-    const uint32_t lanes = grad_lanes(A.dim), walkers = kGradThreads / lanes, col_tiles = (uint32_t)(((A.dim + 7) / 8 + lanes - 1) / lanes);
-    const uint64_t walk_blocks = (W.chunks + walkers - 1) / walkers * col_tiles;
-    GradWalk P{kb[to], pb[to], A.n, rows, W.chunk, W.chunks, lanes, col_tiles, walk_blocks, A.grad, A.grad_stride, dim, A.table, A.table_stride, A.scale,
-               A.accumulate, (float*)(base + W.part), W.dim8};
-    const uint32_t join_tiles = (uint32_t)((A.dim + 511) / 512);
-    return with_dtype(A.table_dtype, [&](auto t) {
+    const uint32_t *keys = kb[to], *poss = pb[to];
+    const uint32_t col_tiles = (dim + kGradCols - 1) / kGradCols;
+    const uint64_t walk_blocks = (W.chunks * col_tiles + kGradWaves - 1) / kGradWaves;
+    const GradWalk P{A.n, rows, W.chunk, W.chunks, col_tiles, walk_blocks, A.grad_stride, dim, A.table_stride, A.scale, A.accumulate, W.dim8};
+    float* part = (float*)(base + W.part);
+    return with_types([&](auto g, auto t, auto small) {
+        typedef decltype(g) G;
         typedef decltype(t) T;
-        hipError_t e = with_dtype(A.dtype, [&](auto g) {
-            typedef decltype(g) G;
-            return launch(grad_walk_kernel<G, T>, walk_blocks + zero_blocks, kGradThreads, stream, P);
-        });
+        hipError_t e = launch(grad_walk_kernel<G, T, small.value>, walk_blocks + zero_blocks, kGradThreads, stream, P, keys, poss, (const G*)A.grad, (T*)A.table, part);
         if (e != hipSuccess) return e;
-        return launch(grad_join_kernel<T>, W.chunks * join_tiles, kGradThreads, stream, P, join_tiles);
+        return launch(grad_join_kernel<T, small.value>, W.chunks * col_tiles, kGradThreads, stream, P, keys, (T*)A.table, (const float*)part);
     });
 }
 

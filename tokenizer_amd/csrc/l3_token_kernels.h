@@ -31,21 +31,18 @@ hipError_t with_dtype(int code, F f) {
     return code == kF32 ? f(float()) : code == kF16 ? f(_Float16()) : f((__bf16)0.f);
 }
 
-// Eight neighbouring elements.  The copies carry no alignment beyond the element's, so any row start and stride is fine: gfx950
-// takes unaligned 16-byte accesses.
+// Eight neighbouring elements, aligned like one of them: any row start and stride is fine, gfx950 takes unaligned 16-byte accesses.
+template <class T> struct Eight {
+    typedef T V __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+};
+typedef float F8 __attribute__((ext_vector_type(8)));
 template <class T>
-__device__ __forceinline__ void load8(const T* p, float* v) {
-    T t[8];
-    __builtin_memcpy(t, p, sizeof t);
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = (float)t[i];
-}
+__device__ __forceinline__ typename Eight<T>::V load8(const T* p) { return *reinterpret_cast<const typename Eight<T>::V*>(p); }
+template <class V>
+__device__ __forceinline__ F8 to_f8(V v) { return __builtin_convertvector(v, F8); }
 template <class T>
-__device__ __forceinline__ void store8(T* p, const float* v) {
-    T t[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) t[i] = (T)v[i];   // round to nearest, ties to even
-    __builtin_memcpy(p, t, sizeof t);
+__device__ __forceinline__ void store8(T* p, F8 v) {   // rounded to nearest, ties to even
+    *reinterpret_cast<typename Eight<T>::V*>(p) = __builtin_convertvector(v, typename Eight<T>::V);
 }
 
 }  // namespace

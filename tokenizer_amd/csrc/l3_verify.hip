@@ -59,10 +59,10 @@ template <class T>
 __device__ __forceinline__ void weights8(const VerifyArgs& A, const Verdict& R, uint64_t col, double* rest, double* full) {
     const T* p = (const T*)A.target + R.p_row * A.target_stride;
     const T* q = R.state == kDrawRest && A.q ? (const T*)A.q + R.q_row * A.q_stride : nullptr;
-    float pv[8], qv[8];
+    F8 pv = 0.f, qv = 0.f;
     if (col + 8 <= A.vocab) {
-        load8(p + col, pv);
-        if (q) load8(q + col, qv);
+        pv = to_f8(load8(p + col));
+        if (q) qv = to_f8(load8(q + col));
     } else {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
