@@ -29,23 +29,23 @@ __device__ __forceinline__ Cols cols_of(uint32_t vec, uint32_t dim) {
     if (c + 8 <= dim || dim < 8) return {c, 0};
     return {dim - 8, c + 8 - dim};
 }
-template <bool SMALL, class T>
+template <bool SMALL, bool ONCE = false, class T>
 __device__ __forceinline__ typename Eight<T>::V load_cols(const T* row, Cols c, uint32_t dim) {
     if constexpr (SMALL) {
         typename Eight<T>::V v = (T)0.f;
         for (uint32_t i = 0; i < 8; i++) if (i < dim) v[i] = row[i];
         return v;
     } else {
-        return load8(row + c.col);
+        return ONCE ? load8_once(row + c.col) : load8(row + c.col);
     }
 }
 // The vector's own columns; SHARED: the skipped ones hold the same values as their owner stores.
-template <bool SMALL, bool SHARED, class T>
+template <bool SMALL, bool SHARED, bool ONCE = false, class T>
 __device__ __forceinline__ void store_cols(T* row, Cols c, uint32_t dim, F8 v) {
     if constexpr (SMALL) {
         for (uint32_t i = 0; i < 8; i++) if (i < dim) row[i] = (T)v[i];
     } else if (SHARED || c.skip == 0) {
-        store8(row + c.col, v);
+        ONCE ? store8_once(row + c.col, v) : store8(row + c.col, v);
     } else {
 #pragma unroll
         for (uint32_t i = 1; i < 8; i++) if (i >= c.skip) row[c.col + i] = (T)v[i];
@@ -56,9 +56,9 @@ __device__ __forceinline__ void store_cols(T* row, Cols c, uint32_t dim, F8 v) {
 // A thread has PER times eight neighbouring columns, all loads in flight before the first store.  What is divided is a workgroup's
 // first vector (once) and 32-bit offsets from it.
 constexpr int kEmbedThreads = 256;
-constexpr uint64_t kEmbedMany = 1u << 20;   // vectors from which a thread has four
+constexpr uint64_t kEmbedOnce = 1u << 20, kEmbedMany = 1u << 24;   // vectors (launch_embed)
 
-template <class T, class O, int PER, bool SMALL>
+template <class T, class O, int PER, bool ONCE, bool SMALL>
 __global__ __launch_bounds__(kEmbedThreads) void embed_kernel(const int32_t* __restrict__ ids, uint64_t n, const uint64_t* __restrict__ n_dev,
                                                               const T* __restrict__ table, uint32_t rows, uint32_t dim, uint64_t stride,
                                                               O* __restrict__ out, uint64_t out_stride, float scale) {
@@ -85,7 +85,7 @@ __global__ __launch_bounds__(kEmbedThreads) void embed_kernel(const int32_t* __r
 #pragma unroll
         for (int k = 0; k < PER; k++) {
             const F8 x = to_f8(v[k]) * scale;
-            if (t[k] < count) store_cols<SMALL, true>(out + t[k] * out_stride, c[k], dim, (uint32_t)id[k] < rows ? x : (F8)0.f);
+            if (t[k] < count) store_cols<SMALL, true, ONCE>(out + t[k] * out_stride, c[k], dim, (uint32_t)id[k] < rows ? x : (F8)0.f);
         }
     }
 }
@@ -190,15 +190,52 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const int32_t*
     }
 }
 
+// ---- gradient: ids ranked -----------------------------------------------------------------------------------------
+// Up to kRankIds ids in one launch: the place of position i is the number of positions j with key_j < key_i, or key_j = key_i and
+// j < i.  A workgroup has kRankMine positions and all keys in LDS; each of its 32 half waves counts over a part of them, four keys
+// a load.
+constexpr uint32_t kRankMine = 32;
+
+__global__ __launch_bounds__(kSortThreads) void sort_rank_kernel(const int32_t* __restrict__ ids, uint32_t n, const uint64_t* __restrict__ n_dev, uint32_t rows,
+                                                                 uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out) {
+    __shared__ __align__(16) uint32_t key[kRankIds];
+    __shared__ uint32_t rank[kRankMine];
+    const uint32_t valid = (uint32_t)ids_that_count(n, n_dev), i0 = blockIdx.x * kRankMine;
+    constexpr uint32_t kParts = kSortThreads / kRankMine;
+    const uint32_t quads = (n + 4 * kParts - 1) / (4 * kParts), all = quads * 4 * kParts;   // (kRankIds is a multiple of 4 kParts)
+    for (uint32_t j = threadIdx.x; j < all; j += kSortThreads) key[j] = j < n ? sort_key(ids, j, valid, rows) : ~0u;
+    if (threadIdx.x < kRankMine) rank[threadIdx.x] = 0;
+    __syncthreads();
+    const uint32_t i = i0 + threadIdx.x % kRankMine, part = threadIdx.x / kRankMine, k = key[i];   // (i < all: all is a multiple of kRankMine)
+    uint32_t count = 0;
+    const uint32_t lo = part * quads * 4;
+#pragma unroll 4
+    for (uint32_t q = 0; q < quads; q++) {
+        const uint32_t j = lo + q * 4, bound = k + (j < i0 ? 1u : 0u);   // before the workgroup's own positions an equal key counts
+        const uint4 v = *reinterpret_cast<const uint4*>(&key[j]);
+        count += (v.x < bound) + (v.y < bound) + (v.z < bound) + (v.w < bound);
+    }
+    if (part == 0) for (uint32_t j = i0; j < i0 + kRankMine; j++) count += j < i && key[j] == k ? 1u : 0u;
+    atomicAdd(&rank[threadIdx.x % kRankMine], count);
+    __syncthreads();
+    if (part == 0 && i < n) {
+        keys_out[rank[threadIdx.x]] = k;
+        pos_out[rank[threadIdx.x]] = i;
+    }
+}
+
 // ---- gradient: runs of one id added up ----------------------------------------------------------------------------
 // A wave walks through `chunk` sorted positions for 512 columns, in order, four at a time: the four rows of the gradient and, where
 // a run of one id ends, the row of the table it is added to are loaded together.  Keys and positions of the whole chunk are in
-// one register each (lane j has position j).  A run that lies inside the chunk is stored at once.  A run that crosses a border
-// leaves its part in the workspace: part[2 c] of the run that came in from the chunk before, part[2 c + 1] of the run that starts
-// here and goes on; grad_join_kernel adds these up at the chunk where the run starts.  Nothing is added by atomics: the same ids
-// give the same bits.
-constexpr int kGradThreads = 256, kGradWaves = kGradThreads / 64, kGradGroup = 4;
+// one register each (lane j has position j).  A run that lies inside the chunk is stored at once.  The parts of a run that crosses
+// from one wave of a workgroup to the next meet in LDS; a run that crosses the workgroup's border leaves its part in the
+// workspace: part[2 b] of the run that came in from the workgroup before, part[2 b + 1] of the run that starts here and goes
+// on; grad_join_kernel adds these up at the workgroup where the run starts.  Nothing is added by atomics: the same ids give the
+// same bits.
+constexpr int kGradThreads = 64 * kGradWaves;
+constexpr int kGradGroup = 4;
 constexpr uint32_t kGradCols = 512;
+constexpr uint64_t kGradOnce = 256ull << 20;   // bytes of gradient (launch_embed_grad)
 constexpr uint32_t kZeroRows = 64;   // rows a workgroup looks after when the gradient is written whole
 
 // Rows [r0, r0 + kZeroRows) of which `named` has no bit become zero; by a whole workgroup.
@@ -214,7 +251,7 @@ __device__ __forceinline__ void zero_rows(T* table, uint64_t table_stride, uint6
 
 struct GradWalk {
     uint64_t n; uint32_t rows;
-    uint32_t chunk; uint64_t chunks; uint32_t tiles; uint64_t walk_blocks;
+    uint32_t chunk, tiles; uint64_t walk_blocks;
     uint64_t grad_stride; uint32_t dim;
     uint64_t table_stride;
     float scale; int accumulate;
@@ -223,7 +260,7 @@ struct GradWalk {
 
 __device__ __forceinline__ uint32_t of_lane(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
 
-template <class G, class T, bool SMALL>
+template <class G, class T, bool ONCE, bool SMALL>
 __global__ __launch_bounds__(kGradThreads) void grad_walk_kernel(GradWalk P, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ poss,
                                                                  const G* __restrict__ grad, T* __restrict__ table, float* __restrict__ part) {
     const uint32_t rows = P.rows, dim = P.dim;
@@ -235,19 +272,20 @@ __global__ __launch_bounds__(kGradThreads) void grad_walk_kernel(GradWalk P, con
         zero_rows<SMALL>(table, P.table_stride, rows, dim, r0, __ballot(a < P.n && keys[a] == r));
         return;
     }
-    const uint64_t wave = (uint64_t)blockIdx.x * kGradWaves + (uint32_t)__builtin_amdgcn_readfirstlane((int)wave_id());
-    const uint64_t c = wave / P.tiles, lo = c * P.chunk;
-    if (c >= P.chunks) return;
-    const uint32_t vec = (uint32_t)(wave - c * P.tiles) * 64 + lane_id(), len = lo + P.chunk < P.n ? P.chunk : (uint32_t)(P.n - lo);
+    __shared__ F8 heads[kGradWaves][64];
+    __shared__ bool goes_through[kGradWaves];
+    const uint64_t block = blockIdx.x / P.tiles;
+    const uint32_t w = (uint32_t)__builtin_amdgcn_readfirstlane((int)wave_id());
+    const uint64_t c = block * kGradWaves + w, lo = c * P.chunk < P.n ? c * P.chunk : P.n;
+    const uint32_t vec = (uint32_t)(blockIdx.x - block * P.tiles) * 64 + lane_id(), len = lo + P.chunk < P.n ? P.chunk : (uint32_t)(P.n - lo);
     const uint32_t key = (uint32_t)lane_id() < len ? keys[lo + lane_id()] : ~0u, pos = (uint32_t)lane_id() < len ? poss[lo + lane_id()] : 0;
     // the key behind the chunk, and the run that came in, if one did
-    const uint32_t behind = lo + len < P.n ? keys[lo + len] : ~0u, head = of_lane(key, 0), in_front = lo ? keys[lo - 1] : ~0u;
-    const uint32_t came_in = head == in_front ? head : ~0u;
+    const uint32_t behind = lo + len < P.n ? keys[lo + len] : ~0u, first = of_lane(key, 0), in_front = lo && len ? keys[lo - 1] : ~0u;
+    const uint32_t came_in = first == in_front && first < rows ? first : ~0u;
     const uint32_t used = (uint32_t)__popcll(__ballot(key < rows));   // ids that are no rows come last
-    if (used == 0) return;
     const bool mine = vec * 8 < dim;
     const Cols at = cols_of(mine ? vec : 0, dim);
-    F8 sum = 0.f;
+    F8 sum = 0.f, head = 0.f;
     for (uint32_t i = 0; i < used; i += kGradGroup) {
         uint32_t k[kGradGroup + 1];
         typename Eight<G>::V g[kGradGroup];
@@ -257,7 +295,7 @@ __global__ __launch_bounds__(kGradThreads) void grad_walk_kernel(GradWalk P, con
 #pragma unroll
         for (int j = 0; j < kGradGroup; j++) {
             const uint32_t x = i + j < used ? i + j : used - 1;
-            g[j] = load_cols<SMALL>(grad + (uint64_t)of_lane(pos, x) * P.grad_stride, at, dim);
+            g[j] = load_cols<SMALL, ONCE>(grad + (uint64_t)of_lane(pos, x) * P.grad_stride, at, dim);
         }
 #pragma unroll
         for (int j = 0; j < kGradGroup; j++) {
@@ -269,32 +307,62 @@ __global__ __launch_bounds__(kGradThreads) void grad_walk_kernel(GradWalk P, con
             if (i + j >= used) break;
             sum += to_f8(g[j]);
             if (k[j + 1] == k[j]) continue;
-            if (mine) {
-                if (k[j] == came_in) store8(part + (2 * c) * P.dim8 + vec * 8, sum);
-                else store_cols<SMALL, false>(table + (uint64_t)k[j] * P.table_stride, at, dim, to_f8(old[j]) + sum * P.scale);
-            }
+            if (k[j] == came_in) head = sum;
+            else if (mine) store_cols<SMALL, false>(table + (uint64_t)k[j] * P.table_stride, at, dim, to_f8(old[j]) + sum * P.scale);
             sum = 0.f;
         }
     }
-    const uint32_t last = of_lane(key, len - 1);
-    if (mine && last < rows && last == behind) store8(part + (2 * c + (last == came_in ? 0 : 1)) * P.dim8 + vec * 8, sum);
+    const uint32_t last = len ? of_lane(key, (int)len - 1) : ~0u;
+    const bool goes_on = last < rows && last == behind, through = goes_on && last == came_in, starts = goes_on && !through;
+    if (through) head = sum;
+    if (w && came_in != ~0u) {
+        heads[w][lane_id()] = head;
+        goes_through[w] = through;
+    }
+    __syncthreads();
+    // the run that this wave has to look after: the one that starts here and goes on or, in the first wave, the one that came in
+    F8 x = starts ? sum : head;
+    uint32_t v = w;
+    bool on = goes_on;
+    if (starts || (w == 0 && came_in != ~0u)) {
+        while (on && ++v < kGradWaves) {
+            x += heads[v][lane_id()];
+            on = goes_through[v];
+        }
+        if (mine) {
+            if (!starts) {
+                store8(part + (2 * block) * P.dim8 + vec * 8, x);
+            } else if (on) {
+                store8(part + (2 * block + 1) * P.dim8 + vec * 8, x);
+            } else {
+                typename Eight<T>::V old = (T)0.f;
+                T* row = table + (uint64_t)last * P.table_stride;
+                if (P.accumulate) old = load_cols<SMALL>(row, at, dim);
+                store_cols<SMALL, false>(row, at, dim, to_f8(old) + x * P.scale);
+            }
+        }
+    }
+    // (the first wave may have both: a run that came in and ended, and one that starts and goes on)
+    if (w == 0 && starts && came_in != ~0u && mine) store8(part + (2 * block) * P.dim8 + vec * 8, head);
 }
 
-// Parts of long runs: a workgroup per chunk and 512 columns, every wave a quarter of the parts, four loads in flight.
+// Parts of long runs: a workgroup per walking workgroup and 512 columns, every wave a share of the parts, eight loads in flight.
+constexpr int kJoinGroup = 8;
+
 template <class T, bool SMALL>
 __global__ __launch_bounds__(kGradThreads) void grad_join_kernel(GradWalk P, const uint32_t* __restrict__ keys, T* __restrict__ table,
                                                                  const float* __restrict__ part) {
     __shared__ F8 acc[kGradWaves - 1][64];
-    const uint64_t c = blockIdx.x / P.tiles;
-    const uint32_t vec = (blockIdx.x % P.tiles) * 64 + lane_id();
-    const uint64_t lo = c * P.chunk, hi = lo + P.chunk;
+    const uint64_t b = blockIdx.x / P.tiles, span = (uint64_t)P.chunk * kGradWaves;
+    const uint32_t vec = (blockIdx.x - (uint32_t)b * P.tiles) * 64 + lane_id();
+    const uint64_t lo = b * span, hi = lo + span;
     if (hi >= P.n) return;
     const uint32_t k = keys[hi - 1], behind = keys[hi], in_front = lo ? keys[lo - 1] : ~0u;
     if (k >= P.rows || behind != k || in_front == k) return;
-    uint64_t more = 0;   // chunks behind c that the run comes into
+    uint64_t more = 0;   // workgroups behind b that the run comes into
     for (;;) {
-        const uint64_t d = c + 1 + more + lane_id();
-        const u64 m = __ballot(d < P.chunks && keys[d * P.chunk] == k);
+        const uint64_t at = hi + (more + lane_id()) * span;
+        const u64 m = __ballot(at < P.n && keys[at] == k);
         if (m == ~0ull) { more += 64; continue; }
         more += (uint64_t)__builtin_ctzll(~m);
         break;
@@ -303,20 +371,20 @@ __global__ __launch_bounds__(kGradThreads) void grad_join_kernel(GradWalk P, con
     const bool mine = vec * 8 < P.dim;
     const Cols at = cols_of(mine ? vec : 0, P.dim);
     T* row = table + (uint64_t)k * P.table_stride;
-    const float* from = part + (mine ? vec : 0) * 8;
+    const float* from = part + (uint64_t)(mine ? vec : 0) * 8;
     typename Eight<T>::V old = (T)0.f;
     F8 sum = 0.f;
     if (w == 0) {
         if (P.accumulate) old = load_cols<SMALL>(row, at, P.dim);
-        sum = load8(from + (2 * c + 1) * P.dim8);
+        sum = load8(from + (2 * b + 1) * P.dim8);
     }
-    const uint64_t d1 = c + 1 + more * (w + 1) / kGradWaves;
-    for (uint64_t d = c + 1 + more * w / kGradWaves; d < d1; d += 4) {
-        F8 v[4];
+    const uint64_t end = b + 1 + more * (w + 1) / kGradWaves;
+    for (uint64_t d = b + 1 + more * w / kGradWaves; d < end; d += kJoinGroup) {
+        F8 v[kJoinGroup];
 #pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = load8(from + 2 * (d + j < d1 ? d + j : d1 - 1) * P.dim8);
+        for (int j = 0; j < kJoinGroup; j++) v[j] = load8(from + 2 * (d + j < end ? d + j : end - 1) * P.dim8);
 #pragma unroll
-        for (int j = 0; j < 4; j++) if (d + j < d1) sum += v[j];
+        for (int j = 0; j < kJoinGroup; j++) if (d + j < end) sum += v[j];
     }
     if (w) acc[w - 1][lane_id()] = sum;
     __syncthreads();
@@ -326,43 +394,23 @@ __global__ __launch_bounds__(kGradThreads) void grad_join_kernel(GradWalk P, con
 }
 
 // ---- gradient: few ids --------------------------------------------------------------------------------------------
-// One launch.  A workgroup per position: it compares all ids with its own, leaves if one before it is the same, and else adds up
-// the rows of those that are -- with few of them every wave has columns of its own, with many every wave has a quarter of the
-// positions and the waves' sums are added in order.
-constexpr int kDirectMany = 8, kDirectWords = (int)(kDirectIds / 64);
-
-template <bool SMALL, class G>
-__device__ __forceinline__ F8 add_named(const G* __restrict__ grad, uint64_t stride, Cols at, uint32_t dim, const u64* words, int first, int step) {
-    F8 sum = 0.f;
-    for (int x = first; x < kDirectWords; x += step) {
-        u64 m = words[x];
-        m = (u64)(uint32_t)__builtin_amdgcn_readfirstlane((int)(m >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)m);   // the wave's own
-        while (m) {
-            typename Eight<G>::V g[4];
-            uint32_t p = 0;
-            const int have = __popcll(m);
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if (m) { p = (uint32_t)x * 64 + (uint32_t)__builtin_ctzll(m); m &= m - 1; }
-                g[j] = load_cols<SMALL>(grad + (uint64_t)p * stride, at, dim);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; j++) if (j < have) sum += to_f8(g[j]);
-        }
-    }
-    return sum;
-}
+// One launch, nothing sorted.  A workgroup per position and 512 columns: it compares all ids with its own, leaves if one before it
+// is the same, and else adds up the rows of those that are, every wave a quarter of them.  Its own row and the table's are on
+// their way while it compares.
+constexpr int kDirectWords = (int)(kDirectIds / 64), kDirectGroup = 8;
 
 template <class G, class T, bool SMALL>
 __global__ __launch_bounds__(kGradThreads) void grad_direct_kernel(const int32_t* __restrict__ ids, uint32_t n, const uint64_t* n_dev, uint32_t rows,
                                                                    const G* __restrict__ grad, uint64_t grad_stride, uint32_t dim,
-                                                                   T* __restrict__ table, uint64_t table_stride, float scale, int accumulate) {
+                                                                   T* __restrict__ table, uint64_t table_stride, float scale, int accumulate,
+                                                                   uint32_t tiles) {
     __shared__ u64 words[kDirectWords];
+    __shared__ uint32_t list[kDirectIds];
     __shared__ F8 acc[kGradWaves - 1][64];
     const uint32_t valid = (uint32_t)ids_that_count(n, n_dev);
     const int w = __builtin_amdgcn_readfirstlane((int)wave_id()), lane = lane_id();
-    if (blockIdx.x >= n) {   // rows that no id names, when the gradient is written whole
-        const uint64_t r0 = (uint64_t)(blockIdx.x - n) * kZeroRows;
+    if (blockIdx.x >= n * tiles) {   // rows that no id names, when the gradient is written whole
+        const uint64_t r0 = (uint64_t)(blockIdx.x - n * tiles) * kZeroRows;
         if (threadIdx.x == 0) words[0] = 0;
         __syncthreads();
         for (uint32_t j = threadIdx.x; j < valid; j += kGradThreads) {
@@ -373,54 +421,63 @@ __global__ __launch_bounds__(kGradThreads) void grad_direct_kernel(const int32_t
         zero_rows<SMALL>(table, table_stride, rows, dim, r0, words[0]);
         return;
     }
-    const uint32_t t = blockIdx.x;
+    const uint32_t t = blockIdx.x / tiles;
     if (t >= valid) return;
-    const int32_t id = ids[t];
-    if (id < 0 || (uint32_t)id >= rows) return;
     int32_t other[kDirectWords / kGradWaves];
 #pragma unroll
     for (int y = 0; y < kDirectWords / kGradWaves; y++) {
         const uint32_t j = (uint32_t)(y * kGradWaves + w) * 64 + lane;
-        other[y] = j < valid ? ids[j] : -1;
+        other[y] = ids[j < valid ? j : 0];
+    }
+    const int32_t id = ids[t];
+    if (id < 0 || (uint32_t)id >= rows) return;
+    const uint32_t vec = (blockIdx.x - t * tiles) * 64 + lane;
+    const bool mine = vec * 8 < dim;
+    const Cols at = cols_of(mine ? vec : 0, dim);
+    T* row = table + (uint64_t)(uint32_t)id * table_stride;
+    typename Eight<T>::V old = (T)0.f;
+    F8 sum = 0.f;
+    if (w == 0) {
+        if (accumulate) old = load_cols<SMALL>(row, at, dim);
+        sum = to_f8(load_cols<SMALL>(grad + (uint64_t)t * grad_stride, at, dim));
     }
     bool earlier = false;
-    int many = 0;
 #pragma unroll
     for (int y = 0; y < kDirectWords / kGradWaves; y++) {
         const int x = y * kGradWaves + w;
-        const u64 m = __ballot(other[y] == id);
+        const uint32_t j = (uint32_t)x * 64 + lane;
+        const u64 m = __ballot(j < valid && j != t && other[y] == id);
         if (lane == 0) words[x] = m;
         if (m && (uint32_t)x * 64 + (uint32_t)__builtin_ctzll(m) < t) earlier = true;
-        many += __popcll(m);
     }
     if (__syncthreads_or(earlier)) return;
-    T* row = table + (uint64_t)(uint32_t)id * table_stride;
-    const uint32_t per_row = (dim + 7) / 8;
-    if (!__syncthreads_or(many > kDirectMany)) {   // (of one wave's words: at most four times as many in all)
-        for (uint32_t vec = threadIdx.x; vec < per_row; vec += kGradThreads) {
-            const Cols at = cols_of(vec, dim);
-            typename Eight<T>::V old = (T)0.f;
-            if (accumulate) old = load_cols<SMALL>(row, at, dim);
-            const F8 sum = add_named<SMALL>(grad, grad_stride, at, dim, words, 0, 1);
-            store_cols<SMALL, false>(row, at, dim, to_f8(old) + sum * scale);
+    // the others, in order: every wave knows how many there are in the words before its own
+    static_assert(kDirectWords <= 64, "a lane a word");
+    const u64 mine_word = lane < kDirectWords ? words[lane] : 0;
+    const uint32_t upto = wave_iscan((uint32_t)__popcll(mine_word)), count = of_lane(upto, 63);
+    if (count) {
+        for (int x = w; x < kDirectWords; x += kGradWaves) {
+            const u64 m = words[x];
+            if ((m >> lane) & 1) list[of_lane(upto, x) - (uint32_t)__popcll(m) + (uint32_t)__popcll(m & ((1ull << lane) - 1))] = (uint32_t)x * 64 + lane;
         }
-        return;
-    }
-    for (uint32_t v0 = 0; v0 < per_row; v0 += 64) {
-        const uint32_t vec = v0 + (uint32_t)lane;
-        const bool mine = vec < per_row;
-        const Cols at = cols_of(mine ? vec : 0, dim);
-        typename Eight<T>::V old = (T)0.f;
-        if (w == 0 && accumulate) old = load_cols<SMALL>(row, at, dim);
-        F8 sum = add_named<SMALL>(grad, grad_stride, at, dim, words, w, kGradWaves);
+        __syncthreads();
+        const uint32_t hi = count * (w + 1) / kGradWaves;
+        for (uint32_t i = count * w / kGradWaves; i < hi; i += kDirectGroup) {
+            typename Eight<G>::V g[kDirectGroup];
+#pragma unroll
+            for (int j = 0; j < kDirectGroup; j++) {
+                const uint32_t p = (uint32_t)__builtin_amdgcn_readfirstlane((int)list[i + j < hi ? i + j : hi - 1]);
+                g[j] = load_cols<SMALL>(grad + (uint64_t)p * grad_stride, at, dim);
+            }
+#pragma unroll
+            for (int j = 0; j < kDirectGroup; j++) if (i + j < hi) sum += to_f8(g[j]);
+        }
         if (w) acc[w - 1][lane] = sum;
         __syncthreads();
-        if (w == 0 && mine) {
-            for (int x = 0; x < kGradWaves - 1; x++) sum += acc[x][lane];
-            store_cols<SMALL, false>(row, at, dim, to_f8(old) + sum * scale);
-        }
-        __syncthreads();
     }
+    if (w || !mine) return;
+    if (count) for (int x = 0; x < kGradWaves - 1; x++) sum += acc[x][lane];
+    store_cols<SMALL, false>(row, at, dim, to_f8(old) + sum * scale);
 }
 
 // f(std::true_type / false_type): rows of fewer than eight columns, or not
@@ -439,10 +496,13 @@ hipError_t launch_embed(const EmbedArgs& A, hipStream_t stream) {
         return with_dtype(A.out_dtype, [&](auto o) {
             typedef decltype(o) O;
             return with_small(A.dim, [&](auto small) {
-                const bool many = vectors >= kEmbedMany;
-                const uint64_t tile = kEmbedThreads * (many ? 4 : 1);
-                return launch(many ? embed_kernel<T, O, 4, small.value> : embed_kernel<T, O, 1, small.value>, capped((vectors + tile - 1) / tile), kEmbedThreads, stream,
-                              A.ids, A.n, A.n_dev, (const T*)A.table, (uint32_t)A.rows, (uint32_t)A.dim, A.stride, (O*)A.out, A.out_stride, A.scale);
+                const int per = vectors >= kEmbedMany ? 4 : 1;
+                auto* kernel = vectors >= kEmbedMany   ? embed_kernel<T, O, 4, true, small.value>
+                               : vectors >= kEmbedOnce ? embed_kernel<T, O, 1, true, small.value>
+                                                       : embed_kernel<T, O, 1, false, small.value>;
+                const uint64_t tile = (uint64_t)kEmbedThreads * per;
+                return launch(kernel, capped((vectors + tile - 1) / tile), kEmbedThreads, stream, A.ids, A.n, A.n_dev, (const T*)A.table, (uint32_t)A.rows,
+                              (uint32_t)A.dim, A.stride, (O*)A.out, A.out_stride, A.scale);
             });
         });
     });
@@ -456,13 +516,14 @@ hipError_t launch_embed_grad(const EmbedGradArgs& A, hipStream_t stream) {
             return with_dtype(A.dtype, [&](auto g) { return with_small(A.dim, [&](auto small) { return f(g, t, small); }); });
         });
     };
-    if (A.n <= kDirectIds) {
+    const uint32_t col_tiles = (dim + kGradCols - 1) / kGradCols;
+    if (grad_direct(A.n, A.dim)) {
         if (A.n + zero_blocks == 0) return hipSuccess;
         return with_types([&](auto g, auto t, auto small) {
             typedef decltype(g) G;
             typedef decltype(t) T;
-            return launch(grad_direct_kernel<G, T, small.value>, A.n + zero_blocks, kGradThreads, stream, A.ids, (uint32_t)A.n, A.n_dev, rows, (const G*)A.grad,
-                          A.grad_stride, dim, (T*)A.table, A.table_stride, A.scale, A.accumulate);
+            return launch(grad_direct_kernel<G, T, small.value>, A.n * col_tiles + zero_blocks, kGradThreads, stream, A.ids, (uint32_t)A.n, A.n_dev, rows, (const G*)A.grad,
+                          A.grad_stride, dim, (T*)A.table, A.table_stride, A.scale, A.accumulate, col_tiles);
         });
     }
     const GradWork W = grad_work(A.n, A.dim);
@@ -470,31 +531,37 @@ hipError_t launch_embed_grad(const EmbedGradArgs& A, hipStream_t stream) {
     uint32_t* const kb[2] = {(uint32_t*)(base + W.keys0), (uint32_t*)(base + W.keys1)};
     uint32_t* const pb[2] = {(uint32_t*)(base + W.pos0), (uint32_t*)(base + W.pos1)};
     uint32_t* hist = (uint32_t*)(base + W.hist);
-    int bits = 1;
-    while (bits < 32 && (rows >> bits)) bits++;            // keys are 0 .. rows
-    const int passes = (bits + kSortBits - 1) / kSortBits, per = (bits + passes - 1) / passes;
-    const uint64_t tiles = (A.n + kSortTile - 1) / kSortTile;
-    const uint32_t mask = (1u << per) - 1;
-    for (int p = 0; p < passes; p++) {
-        const int shift = p * per, from = (p + 1) & 1, to = p & 1;
-        const uint32_t *k = kb[from], *q = pb[from], *h = hist;
-        hipError_t e = launch(p ? sort_count_kernel<false> : sort_count_kernel<true>, tiles, kSortThreads, stream, A.ids, k, A.n, A.n_dev, rows, shift, mask, hist);
+    const uint32_t *keys = kb[0], *poss = pb[0];
+    if (A.n <= kRankIds) {
+        const hipError_t e = launch(sort_rank_kernel, (A.n + kRankMine - 1) / kRankMine, kSortThreads, stream, A.ids, (uint32_t)A.n, A.n_dev, rows, kb[0], pb[0]);
         if (e != hipSuccess) return e;
-        e = launch(p ? sort_place_kernel<false> : sort_place_kernel<true>, tiles, kSortThreads, stream, A.ids, k, q, A.n, A.n_dev, rows, shift, mask, per, h, kb[to], pb[to]);
-        if (e != hipSuccess) return e;
+    } else {
+        int bits = 1;
+        while (bits < 32 && (rows >> bits)) bits++;            // keys are 0 .. rows
+        const int passes = (bits + kSortBits - 1) / kSortBits, per = (bits + passes - 1) / passes;
+        const uint64_t tiles = (A.n + kSortTile - 1) / kSortTile;
+        const uint32_t mask = (1u << per) - 1;
+        for (int p = 0; p < passes; p++) {
+            const int shift = p * per, from = (p + 1) & 1, to = p & 1;
+            const uint32_t *k = kb[from], *q = pb[from], *h = hist;
+            hipError_t e = launch(p ? sort_count_kernel<false> : sort_count_kernel<true>, tiles, kSortThreads, stream, A.ids, k, A.n, A.n_dev, rows, shift, mask, hist);
+            if (e != hipSuccess) return e;
+            e = launch(p ? sort_place_kernel<false> : sort_place_kernel<true>, tiles, kSortThreads, stream, A.ids, k, q, A.n, A.n_dev, rows, shift, mask, per, h, kb[to], pb[to]);
+            if (e != hipSuccess) return e;
+            keys = kb[to];
+            poss = pb[to];
+        }
     }
-    const int to = (passes - 1) & 1;
-    const uint32_t *keys = kb[to], *poss = pb[to];
-    const uint32_t col_tiles = (dim + kGradCols - 1) / kGradCols;
-    const uint64_t walk_blocks = (W.chunks * col_tiles + kGradWaves - 1) / kGradWaves;
-    const GradWalk P{A.n, rows, W.chunk, W.chunks, col_tiles, walk_blocks, A.grad_stride, dim, A.table_stride, A.scale, A.accumulate, W.dim8};
+    const uint64_t walk_blocks = W.blocks * col_tiles;
+    const GradWalk P{A.n, rows, W.chunk, col_tiles, walk_blocks, A.grad_stride, dim, A.table_stride, A.scale, A.accumulate, W.dim8};
     float* part = (float*)(base + W.part);
     return with_types([&](auto g, auto t, auto small) {
         typedef decltype(g) G;
         typedef decltype(t) T;
-        hipError_t e = launch(grad_walk_kernel<G, T, small.value>, walk_blocks + zero_blocks, kGradThreads, stream, P, keys, poss, (const G*)A.grad, (T*)A.table, part);
+        const bool once = A.n * A.dim * sizeof(G) > kGradOnce;
+        hipError_t e = launch(once ? grad_walk_kernel<G, T, true, small.value> : grad_walk_kernel<G, T, false, small.value>, walk_blocks + zero_blocks, kGradThreads, stream, P, keys, poss, (const G*)A.grad, (T*)A.table, part);
         if (e != hipSuccess) return e;
-        return launch(grad_join_kernel<T, small.value>, W.chunks * col_tiles, kGradThreads, stream, P, keys, (T*)A.table, (const float*)part);
+        return launch(grad_join_kernel<T, small.value>, walk_blocks, kGradThreads, stream, P, keys, (T*)A.table, (const float*)part);
     });
 }
 

@@ -38,6 +38,13 @@ template <class T> struct Eight {
 typedef float F8 __attribute__((ext_vector_type(8)));
 template <class T>
 __device__ __forceinline__ typename Eight<T>::V load8(const T* p) { return *reinterpret_cast<const typename Eight<T>::V*>(p); }
+// The same for data that is used once: it need not stay in the caches.
+template <class T>
+__device__ __forceinline__ typename Eight<T>::V load8_once(const T* p) { return __builtin_nontemporal_load(reinterpret_cast<const typename Eight<T>::V*>(p)); }
+template <class T>
+__device__ __forceinline__ void store8_once(T* p, F8 v) {
+    __builtin_nontemporal_store(__builtin_convertvector(v, typename Eight<T>::V), reinterpret_cast<typename Eight<T>::V*>(p));
+}
 template <class V>
 __device__ __forceinline__ F8 to_f8(V v) { return __builtin_convertvector(v, F8); }
 template <class T>

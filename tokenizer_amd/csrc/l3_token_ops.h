@@ -65,21 +65,30 @@ constexpr uint64_t align256(uint64_t b) { return (b + 255) & ~255ull; }
 
 // Ids are sorted in tiles of kSortTile by digits of at most kSortBits bits.
 constexpr int kSortTile = 2048, kSortBits = 9, kSortBins = 1 << kSortBits;
-// Up to kDirectIds ids are not sorted: every position looks for the others of its id by itself.
-constexpr uint64_t kDirectIds = 2048;
-// Sorted positions one walker adds up.
-inline uint32_t grad_chunk(uint64_t n) { return n >= 32768 ? 64 : n >= 8192 ? 16 : 8; }
-struct GradWork { uint64_t keys0, pos0, keys1, pos1, hist, part, total; uint32_t chunk; uint64_t chunks, dim8; };
+// Few ids are not sorted: every position looks for the others of its id by itself, a workgroup for each and 512 columns.  Up to
+// kRankIds ids are sorted in one launch by counting, more digit by digit.
+constexpr uint64_t kDirectIds = 2048, kDirectBlocks = 4096, kRankIds = 8192;
+inline bool grad_direct(uint64_t n, uint64_t dim) { return n <= kDirectIds && n * ((dim + 511) / 512) <= kDirectBlocks; }
+// Sorted positions one wave adds up: few enough that there are about kGradWalkers waves, and 8 .. 64.
+constexpr uint64_t kGradWalkers = 2048;
+constexpr int kGradWaves = 4;        // waves of a workgroup
+inline uint32_t grad_chunk(uint64_t n, uint64_t dim) {
+    const uint64_t want = n * ((dim + 511) / 512) / kGradWalkers;
+    uint32_t c = 8;
+    while (c < 64 && c < want) c *= 2;
+    return c;
+}
+struct GradWork { uint64_t keys0, pos0, keys1, pos1, hist, part, total; uint32_t chunk; uint64_t blocks, dim8; };
 inline GradWork grad_work(uint64_t n, uint64_t dim) {
     GradWork w;
-    w.chunk = grad_chunk(n);
-    w.chunks = (n + w.chunk - 1) / w.chunk;
+    w.chunk = grad_chunk(n, dim);
+    w.blocks = (n + kGradWaves * w.chunk - 1) / (kGradWaves * w.chunk);
     w.dim8 = (dim + 7) & ~7ull;
     uint64_t at = 0;
     auto take = [&](uint64_t b) { const uint64_t p = at; at += align256(b); return p; };
     w.keys0 = take(4 * n); w.pos0 = take(4 * n); w.keys1 = take(4 * n); w.pos1 = take(4 * n);
     w.hist = take(((n + kSortTile - 1) / kSortTile) * kSortBins * 4);
-    w.part = take(2 * w.chunks * w.dim8 * 4);
+    w.part = take(2 * w.blocks * w.dim8 * 4);
     w.total = at ? at : 256;
     return w;
 }
@@ -212,8 +221,8 @@ L3_HD PlanRec plan_slots(int32_t len, int32_t held, uint64_t a, uint64_t b, uint
     const uint64_t end = (uint64_t)len + (b - a);
     if (b == a) return r;
     if (end > max_pages * page || end > kMaxCount) { r.flags = kCacheRow; return r; }
-    const uint64_t pages = (end + page - 1) / page;
-    r.delta = pages > (uint64_t)held ? (int32_t)(pages - (uint64_t)held) : 0;
+    const uint32_t pages = ((uint32_t)end + page - 1) / page;   // (below 2^31 + 2^20)
+    r.delta = pages > (uint32_t)held ? (int32_t)(pages - (uint32_t)held) : 0;
     r.new_len = (int32_t)end;
     return r;
 }
@@ -224,7 +233,7 @@ L3_HD PlanRec plan_trim(int32_t len, int32_t held, int32_t keep, uint32_t page, 
     if (keep < 0) return r;
     if (!sane_request(len, held, page, max_pages)) { r.flags = kCacheBad; return r; }
     r.new_len = keep < len ? keep : len;
-    r.delta = held - (int32_t)(((uint64_t)r.new_len + page - 1) / page);
+    r.delta = held - (int32_t)(((uint32_t)r.new_len + page - 1) / page);
     return r;
 }
 // Is it served?  `before`: pages the requests before it ask for / give back; `left`: pages in the pool.

@@ -78,18 +78,35 @@ __device__ __forceinline__ void weights8(const VerifyArgs& A, const Verdict& R, 
     }
 }
 
-__device__ __forceinline__ double wave_sum_f64(double v) {
-    for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d, 64);
+// Inclusive sums over the wave's lanes, by DPP as wave_iscan (l3_dev.h) has them.
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ double dpp_move_f64(double v) {
+    const u64 b = (u64)__double_as_longlong(v);
+    return __longlong_as_double((long long)((u64)dpp_move<CTRL, ROWS>((uint32_t)(b >> 32)) << 32 | dpp_move<CTRL, ROWS>((uint32_t)b)));
+}
+__device__ __forceinline__ double wave_iscan_f64(double v) {
+    v += dpp_move_f64<0x111>(v);
+    v += dpp_move_f64<0x112>(v);
+    v += dpp_move_f64<0x114>(v);
+    v += dpp_move_f64<0x118>(v);
+    v += dpp_move_f64<0x142, 0xA>(v);
+    v += dpp_move_f64<0x143, 0xC>(v);
     return v;
 }
+__device__ __forceinline__ double of_lane_f64(double v, int lane) {
+    const u64 b = (u64)__double_as_longlong(v);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), lane), lo = (uint32_t)__builtin_amdgcn_readlane((int)b, lane);
+    return __longlong_as_double((long long)((u64)hi << 32 | lo));
+}
+__device__ __forceinline__ double wave_sum_f64(double v) { return of_lane_f64(wave_iscan_f64(v), 63); }
 
 // Sums of kVerifyChunk entries: sums[i][chunk] = {rest, full}.  A workgroup per request and chunk; that of chunk 0 leaves the
-// verdict too.
+// verdict, and all of the answer but the drawn token.
 template <class T>
 __global__ __launch_bounds__(kVerifyThreads) void verify_sum_kernel(VerifyArgs A, uint64_t chunks, double2* sums, Verdict* verdicts) {
-    __shared__ double tmp[2][kVerifyThreads / 64];
+    __shared__ double2 tmp[kVerifyThreads / 64];
     for (uint64_t g = blockIdx.x; g < A.n * chunks; g += gridDim.x) {
-        const uint64_t i = g / chunks, c = g % chunks;
+        const uint64_t i = g / chunks, c = g - i * chunks;
         const Verdict R = verdict_of<T>(A, i);
         double sr = 0, sf = 0;
         const uint64_t col = c * kVerifyChunk + (uint64_t)threadIdx.x * 8;
@@ -101,26 +118,28 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_sum_kernel(VerifyArgs A
         }
         sr = wave_sum_f64(sr);
         sf = wave_sum_f64(sf);
-        if (lane_id() == 0) { tmp[0][wave_id()] = sr; tmp[1][wave_id()] = sf; }
+        if (lane_id() == 0) tmp[wave_id()] = make_double2(sr, sf);
         __syncthreads();
         if (threadIdx.x == 0) {
-            sr = sf = 0;
-            for (int w = 0; w < kVerifyThreads / 64; w++) { sr += tmp[0][w]; sf += tmp[1][w]; }
-            sums[g] = make_double2(sr, sf);
-            if (c == 0) verdicts[i] = R;
+            double2 s = tmp[0];
+            for (int w = 1; w < kVerifyThreads / 64; w++) { s.x += tmp[w].x; s.y += tmp[w].y; }
+            sums[g] = s;
+        }
+        if (c == 0) {
+            int32_t* out = A.out + i * (A.max_draft + 1ull);
+            for (uint32_t j = threadIdx.x; j <= A.max_draft; j += kVerifyThreads) out[j] = R.state != kBadRequest && j < R.a ? A.draft[R.q_row - R.a + j] : -1;
+            if (threadIdx.x == 0) {
+                A.accepted[i] = R.state == kBadRequest ? -1 : (int32_t)R.a;
+                verdicts[i] = R;
+            }
         }
         __syncthreads();
     }
 }
 
-__device__ __forceinline__ double wave_iscan_f64(double v) {
-    for (int d = 1; d < 64; d <<= 1) { const double o = __shfl_up(v, d, 64); if (lane_id() >= d) v += o; }
-    return v;
-}
-
 // A workgroup per request: the chunk the border falls into (every wave finds it by itself, 64 chunks at a time), then the entry.
-// What bounds it is the chain of loads -- verdict and sums, then the chunk's entries -- so nothing else is loaded on the way: with
-// the verdict worked out again and the chunks walked by one thread it took 21 us for 128 requests over 128,256 entries.
+// What bounds it is the chain of loads -- verdict and sums, then the chunk's entries -- so nothing else is on the way: with the
+// verdict worked out again and the chunks walked by one thread it took 21 us for 128 requests over 128,256 entries.
 template <class T>
 __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs A, uint64_t chunks, const double2* sums, const Verdict* verdicts) {
     __shared__ double tmp[kVerifyThreads / 64];
@@ -130,31 +149,29 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
         const double2* S = sums + i * chunks;
         const Verdict R = verdicts[i];
         const double u = (double)A.u_draw[i];
-        int32_t* out = A.out + i * (A.max_draft + 1ull);
-        double rest = 0, full = 0;
-        for (uint64_t c = lane; c < chunks; c += 64) { const double2 w = S[c]; rest += w.x; full += w.y; }
-        rest = wave_sum_f64(rest);
-        full = wave_sum_f64(full);
+        const double2 first = (uint64_t)lane < chunks ? S[lane] : make_double2(0, 0);   // (most vocabularies have no more chunks)
+        if (threadIdx.x == 0) { s_token = 0x7FFFFFFF; s_last = -1; }
+        double2 mine2 = first;
+        for (uint64_t c = 64 + lane; c < chunks; c += 64) { const double2 w = S[c]; mine2.x += w.x; mine2.y += w.y; }
+        const double rest = wave_sum_f64(mine2.x), full = wave_sum_f64(mine2.y);
         const bool use_rest = R.state == kDrawRest && rest > 0;
         const double border = u * (use_rest ? rest : full);
         long long at = -1, last = -1;
         double before = 0, before_last = 0, run = 0;
         for (uint64_t c0 = 0; c0 < chunks && at < 0; c0 += 64) {
             const uint64_t c = c0 + lane;
-            double w = 0;
-            if (c < chunks) w = use_rest ? S[c].x : S[c].y;
-            const double inc = run + wave_iscan_f64(w);
+            const double2 s = c0 == 0 ? first : c < chunks ? S[c] : make_double2(0, 0);
+            const double w = use_rest ? s.x : s.y, inc = run + wave_iscan_f64(w);
             const u64 some = __ballot(w > 0), over = __ballot(w > 0 && inc > border);
             if (some) {
                 const int f = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
-                const double b = __shfl(inc - w, f, 64);
+                const double b = of_lane_f64(inc - w, f);
                 if (over) { at = (long long)c0 + f; before = b; } else { last = (long long)c0 + f; before_last = b; }
             }
-            run = __shfl(inc, 63, 64);
+            run = of_lane_f64(inc, 63);
         }
         // (a border that rounding has put behind all sums falls into the last chunk with weight)
         if (at < 0) { at = last; before = before_last; }
-        if (threadIdx.x == 0) { s_token = 0x7FFFFFFF; s_last = -1; }
         double w8[8], mine = 0;
 #pragma unroll
         for (int j = 0; j < 8; j++) w8[j] = 0;
@@ -183,10 +200,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
         if (found != 0x7FFFFFFF) atomicMin(&s_token, found);
         if (mine_last >= 0) atomicMax(&s_last, mine_last);
         __syncthreads();
-        const int32_t token = s_token != 0x7FFFFFFF ? s_token : s_last;
-        for (uint32_t j = threadIdx.x; j <= A.max_draft; j += kVerifyThreads)
-            out[j] = R.state == kBadRequest ? -1 : j < R.a ? A.draft[R.q_row - R.a + j] : j == R.a ? token : -1;
-        if (threadIdx.x == 0) A.accepted[i] = R.state == kBadRequest ? -1 : (int32_t)R.a;
+        if (threadIdx.x == 0 && R.state != kBadRequest) A.out[i * (A.max_draft + 1ull) + R.a] = s_token != 0x7FFFFFFF ? s_token : s_last;
         __syncthreads();
     }
 }
