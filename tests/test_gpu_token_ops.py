@@ -185,13 +185,31 @@ def test_grad_types_strides_alignment(ctx, torch, G, T):
 
 
 @pytest.mark.parametrize("rows", [1, 2, 255, 511, 512, 513, 128256, 262143, 262144, 262145])
-def test_grad_numbers_of_digits(ctx, torch, rows):
+@pytest.mark.parametrize("n", [5000, 9000])
+def test_grad_numbers_of_digits(ctx, torch, rows, n):
     """Keys of one to three digits; the first and last rows among them."""
     rng = np.random.default_rng(rows)
-    ids = _ids(rng, 5000, rows)
+    ids = _ids(rng, n, rows)
     ids[:4] = [0, rows - 1, 0, rows - 1]
     _grad_case(ctx, torch, rng, ids, 8, F32, F32, rows, False)
     _grad_case(ctx, torch, rng, ids, 8, F32, F32, rows, True)
+
+
+@pytest.mark.parametrize("n", [2047, 2048, 2049, 8191, 8192, 8193, 65536, 65537, 262144, 262145, 300001])
+def test_grad_where_the_sort_changes(ctx, torch, n):
+    """Every way of bringing equal ids together, next to the sizes at which another begins."""
+    rng = np.random.default_rng(n)
+    _grad_case(ctx, torch, rng, _ids(rng, n, 3000), 16, BF16, F32, 3000, True, n_dev=n - 5)
+
+
+@pytest.mark.parametrize("n, dim", [(2048, 520), (600, 4096), (257, 8200)])
+def test_grad_few_ids_wide_rows(ctx, torch, n, dim):
+    """Few ids, one of them in half of the positions: with and without a sort (the number of workgroups decides)."""
+    rng = np.random.default_rng(dim)
+    ids = _ids(rng, n, 50)
+    ids[rng.random(n) < 0.5] = 7
+    _grad_case(ctx, torch, rng, ids, dim, BF16, F32, 50, True)
+    _grad_case(ctx, torch, rng, ids, dim, BF16, BF16, 50, False)
 
 
 @pytest.mark.parametrize("n", [64, 1000, 8192, 40000])
@@ -346,6 +364,15 @@ def test_cache_one_long_request(ctx, torch, tokens):
     rng = np.random.default_rng(tokens)
     _cache_round(ctx, torch, rng, 1, 16, 1300, 2700, [tokens], True)
     _cache_round(ctx, torch, rng, 3, 16, 1300, 7000, [0, tokens, 0], False)
+
+
+@pytest.mark.parametrize("n, every", [(1500, 1), (3000, 1), (5000, 7), (70000, 30)])
+def test_cache_many_requests_few_tokens(ctx, torch, n, every):
+    """More requests than one workgroup plans, most of them without a new token."""
+    rng = np.random.default_rng(n)
+    new = (np.arange(n) % every == 0).astype(int) * rng.integers(1, 3, n)
+    _cache_round(ctx, torch, rng, n, 4, 3, n * 3 + 10, new, True)
+    _cache_round(ctx, torch, rng, n, 4, 3, n * 3 + 10, new, False, tight=True, odd=True)
 
 
 def test_cache_single_tokens_step_after_step(ctx, torch):

@@ -19,12 +19,14 @@ namespace {
 
 struct CacheHead { uint64_t left; uint32_t bad, pad; };
 
-__device__ __forceinline__ u64 block_escan64(u64 v, u64* tmp, u64* total) {   // kPlanThreads threads; tmp: one word per wave
+template <int THREADS>
+__device__ __forceinline__ u64 block_escan64(u64 v, u64* tmp, u64* total) {   // tmp: one word per wave
     const u64 inc = wave_iscan64(v);
     if (lane_id() == 63) tmp[wave_id()] = inc;
     __syncthreads();
     u64 base = 0, tot = 0;
-    for (int i = 0; i < kPlanThreads / 64; i++) {
+#pragma unroll
+    for (int i = 0; i < THREADS / 64; i++) {
         if (i < wave_id()) base += tmp[i];
         tot += tmp[i];
     }
@@ -42,7 +44,7 @@ __global__ __launch_bounds__(kPlanThreads) void cache_plan_kernel(CacheArgs A, P
         r = TRIM ? plan_trim(A.len[i], A.held[i], A.keep[i], A.page, A.max_pages)
                  : plan_slots(A.len[i], A.held[i], A.off[i], A.off[i + 1], A.cap, A.page, A.max_pages);
     u64 total;
-    r.before = block_escan64((u64)r.delta, tmp, &total);
+    r.before = block_escan64<kPlanThreads>((u64)r.delta, tmp, &total);
     if (i < A.n) recs[i] = r;
     if (threadIdx.x == 0) {
         if (blockIdx.x * (uint64_t)kPlanThreads < A.n) blocks[blockIdx.x] = total;
@@ -107,18 +109,24 @@ __device__ u64 pages_served(const PlanRec* recs, const u64* blocks, uint64_t n, 
     return ~block_min64<kApplyThreads / 64>(~best, tmp);
 }
 
-// The last i < n with off[i] <= t, 64 places at a time, by a whole wave (for offsets that are not in order: some i < n).
-__device__ __forceinline__ uint64_t request_of(const uint64_t* off, uint64_t n, uint64_t t) {
-    uint64_t lo = 0, len = n;
-    while (len > 1) {
-        const uint64_t step = (len + 63) / 64, at = lo + (uint64_t)lane_id() * step;
-        const bool ok = (uint64_t)lane_id() * step < len && off[at] <= t;
-        const u64 m = __ballot(ok);
+// The last i < n with off[i] <= t, 64 places at a time, by a whole wave (for offsets that are not in order: some i < n).  The first
+// 64 places are the same for every t: what stands there is loaded by request_probe, before t is known.
+__device__ __forceinline__ uint64_t request_probe(const uint64_t* off, uint64_t n) {
+    const uint64_t at = (uint64_t)lane_id() * ((n + 63) / 64);
+    return at < n ? off[at] : ~0ull;
+}
+__device__ __forceinline__ uint64_t request_of(const uint64_t* off, uint64_t n, uint64_t t, uint64_t probe) {
+    uint64_t lo = 0, len = n, step = (n + 63) / 64;
+    u64 m = __ballot(probe <= t && (uint64_t)lane_id() * step < n);
+    for (;;) {
         const uint64_t k = m ? 63 - __builtin_clzll(m) : 0;
         lo += k * step;
         len = len - k * step < step ? len - k * step : step;
+        if (len <= 1) return lo;
+        step = (len + 63) / 64;
+        const uint64_t at = (uint64_t)lane_id() * step;
+        m = __ballot(at < len && off[lo + (at < len ? at : 0)] <= t);
     }
-    return lo;
 }
 
 // What a token needs of its request.
@@ -146,14 +154,16 @@ __device__ __forceinline__ uint32_t place_token(const CacheArgs& A, const Owner&
     return *slot < 0 ? (uint32_t)kCachePage : 0u;
 }
 
-// Tokens in blocks of 1,024, four neighbours a thread; the requests of a block are found once and kept in LDS (more than
-// kOwners of them only where many requests have no new token: then every token looks for its own).
-constexpr int kTokensPer = 4, kTokenBlock = kApplyThreads * kTokensPer, kOwners = 1024;
+// Tokens in blocks of 512, two neighbours a thread; the requests of a block are found once and kept in LDS (more than kOwners of
+// them only where many requests have no new token: then every token looks for its own).
+constexpr int kTokensPer = 2, kTokenBlock = kApplyThreads * kTokensPer, kOwners = 512, kMaxPlans = (int)(kMaxSeqs / kPlanThreads);
+constexpr uint64_t kRequestBlock = 4 * kApplyWaves;   // requests of a workgroup, four a wave (it divides kPlanThreads)
 
 __global__ __launch_bounds__(kApplyThreads) void cache_slots_kernel(CacheArgs A, const PlanRec* recs, const u64* blocks,
                                                                     const CacheHead* head, uint64_t request_blocks) {
-    __shared__ u64 tmp[kApplyThreads / 64];
+    __shared__ u64 tmp[kApplyWaves];
     __shared__ Owner owners[kOwners];
+    __shared__ uint64_t ends[2];
     const uint64_t left = head->left;
     uint32_t bits = 0;
     if (blockIdx.x == 0) {
@@ -162,38 +172,54 @@ __global__ __launch_bounds__(kApplyThreads) void cache_slots_kernel(CacheArgs A,
         return;
     }
     if (blockIdx.x <= request_blocks) {  // a wave per request: its new state, and its new pages into the table
-        const uint64_t i0 = (uint64_t)(blockIdx.x - 1) * kApplyWaves, i = i0 + wave_id();   // (kApplyWaves divides kPlanThreads)
+        const uint64_t i0 = (blockIdx.x - 1) * kRequestBlock;
         const u64 base = pages_before(blocks, i0 / kPlanThreads, tmp);
-        if (i >= A.n) return;
-        const PlanRec r = recs[i];
-        const u64 before = base + r.before;
-        const bool served = slots_served(r, before, left);
-        if (lane_id() == 0) {
-            A.len_out[i] = served ? r.new_len : r.len;
-            A.held_out[i] = served ? r.held + r.delta : r.held;
-            bits = served ? 0u : r.flags ? r.flags : (uint32_t)kCachePool;
-        }
-        if (served) {
-            int32_t* to = A.table + i * A.table_stride + r.held;
-            const int32_t* from = A.free_pages + (left - before) - 1;
-            for (int32_t j = lane_id(); j < r.delta; j += 64) to[j] = *(from - j);
+#pragma unroll
+        for (uint64_t i = i0 + wave_id(); i < i0 + kRequestBlock; i += kApplyWaves) {
+            if (i >= A.n) break;
+            const PlanRec r = recs[i];
+            const u64 before = base + r.before;
+            const bool served = slots_served(r, before, left);
+            if (lane_id() == 0) {
+                A.len_out[i] = served ? r.new_len : r.len;
+                A.held_out[i] = served ? r.held + r.delta : r.held;
+                bits |= served ? 0u : r.flags ? r.flags : (uint32_t)kCachePool;
+            }
+            if (served) {
+                int32_t* to = A.table + i * A.table_stride + r.held;
+                const int32_t* from = A.free_pages + (left - before) - 1;
+                for (int32_t j = lane_id(); j < r.delta; j += 64) to[j] = *(from - j);
+            }
         }
     } else {
         const uint64_t t0 = (uint64_t)(blockIdx.x - 1 - request_blocks) * kTokenBlock;
         uint64_t total = A.off[A.n];
+        const uint64_t probe = request_probe(A.off, A.n);
         if (total > A.cap) total = A.cap;
         if (t0 >= total) return;
         const uint64_t last = (t0 + kTokenBlock < total ? t0 + kTokenBlock : total) - 1;
-        const uint64_t a0 = request_of(A.off, A.n, t0), a1 = request_of(A.off, A.n, last);
-        const uint64_t b0 = a0 / kPlanThreads;
-        const u64 before0 = pages_before(blocks, b0, tmp);
+        constexpr int kPer = kMaxPlans / kApplyThreads;
+        const uint64_t n_plans = (A.n + kPlanThreads - 1) / kPlanThreads;
+        u64 sums[kPer], base = 0;              // (on their way while the requests are looked for)
+#pragma unroll
+        for (int k = 0; k < kPer; k++) {
+            const uint64_t b = (uint64_t)k * kApplyThreads + threadIdx.x;
+            sums[k] = b < n_plans ? blocks[b] : 0;
+        }
+        // the first two waves find the first and the last request of the block
+        if (wave_id() < 2) ends[wave_id()] = request_of(A.off, A.n, wave_id() ? last : t0, probe);
+        __syncthreads();
+        const uint64_t a0 = ends[0], a1 = ends[1], many = a1 >= a0 ? a1 - a0 + 1 : kOwners + 1;
+        const uint64_t b0 = many <= kOwners ? a0 / kPlanThreads : 0;
+#pragma unroll
+        for (int k = 0; k < kPer; k++) if ((uint64_t)k * kApplyThreads + threadIdx.x < b0) base += sums[k];
+        if (b0) base = apply_sum64(base, tmp);
         auto load_owner = [&](uint64_t i) {
-            u64 before = before0;
+            u64 before = base;
             for (uint64_t b = b0; b < i / kPlanThreads; b++) before += blocks[b];
             const PlanRec r = recs[i];
             return owner_of(A, r, A.off[i], A.off[i + 1], before + r.before, left);
         };
-        const uint64_t many = a1 >= a0 ? a1 - a0 + 1 : kOwners + 1;
         const uint64_t t = t0 + (uint64_t)threadIdx.x * kTokensPer;
         int64_t slot[kTokensPer];
         int32_t pos[kTokensPer];
@@ -211,10 +237,7 @@ __global__ __launch_bounds__(kApplyThreads) void cache_slots_kernel(CacheArgs A,
             for (int j = 0; j < kTokensPer; j++) {
                 uint64_t a = 0, b = A.n;
                 while (b - a > 1) { const uint64_t m = (a + b) / 2; if (A.off[m] <= t + j) a = m; else b = m; }
-                if (t + j <= last) {
-                    if (a / kPlanThreads < b0) { slot[j] = -1; pos[j] = -1; continue; }   // (offsets out of order only)
-                    bits |= place_token(A, load_owner(a), a, t + j, &slot[j], &pos[j]);
-                }
+                if (t + j <= last) bits |= place_token(A, load_owner(a), a, t + j, &slot[j], &pos[j]);
             }
         }
         if (t + kTokensPer <= last + 1) {
@@ -236,13 +259,23 @@ __device__ __forceinline__ uint32_t request_of_page(const uint32_t* before, uint
     return k;
 }
 
-// The whole step in one workgroup: at most kPlanThreads requests and kOneTokens tokens.
-constexpr uint64_t kOneTokens = 4096;
+// The sums up to and with each request ascend: the wave's last request that is served has its largest.  (One atomic a wave: with one
+// from every lane on the same word the compiler walks through the lanes.)
+__device__ __forceinline__ void pages_of_wave(bool served, u64 upto, uint32_t* most) {
+    const u64 m = __ballot(served);
+    if (m && lane_id() == 63 - __builtin_clzll(m)) atomicMax(most, (uint32_t)upto);
+}
 
-__global__ __launch_bounds__(kPlanThreads) void cache_slots_one_kernel(CacheArgs A) {
-    __shared__ u64 tmp[kPlanThreads / 64];
-    __shared__ Owner owners[kPlanThreads];
-    __shared__ uint32_t s_before[kPlanThreads], s_status, s_taken;
+// The whole step in one workgroup: a thread for each request, and at most kOneTokens tokens.  What bounds it is
+// latency -- three dependent loads and two barriers -- so no more waves are started than the requests need.
+constexpr uint64_t kOneTokens = 4096;
+constexpr int kOneSmall = 256;
+
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void cache_slots_one_kernel(CacheArgs A) {
+    __shared__ u64 tmp[THREADS / 64];
+    __shared__ Owner owners[THREADS];
+    __shared__ uint32_t s_before[THREADS], s_status, s_taken;
     const uint64_t i = threadIdx.x;
     const int32_t n_free = *A.n_free;
     const bool bad = n_free < 0 || (uint32_t)n_free > A.n_pages;
@@ -257,24 +290,26 @@ __global__ __launch_bounds__(kPlanThreads) void cache_slots_one_kernel(CacheArgs
         r = plan_slots(A.len[i], A.held[i], first, end, A.cap, A.page, A.max_pages);
     }
     u64 all;
-    const u64 before = block_escan64((u64)r.delta, tmp, &all);   // (barriers inside: nobody's state is read behind it)
+    const u64 before = block_escan64<THREADS>((u64)r.delta, tmp, &all);   // (barriers inside: nobody's state is read behind it)
+    bool takes = false;
     if (i < A.n) {
         const bool served = slots_served(r, before, left);
+        takes = served && r.delta;
         owners[i] = owner_of(A, r, first, end, before, left);
         s_before[i] = (uint32_t)before;   // (a request asks for at most kOneTokens pages)
         A.len_out[i] = served ? r.new_len : r.len;
         A.held_out[i] = served ? r.held + r.delta : r.held;
         if (!served) atomicOr(&s_status, r.flags ? r.flags : (uint32_t)kCachePool);
-        else if (r.delta) atomicMax(&s_taken, (uint32_t)(before + (u64)r.delta));
     }
+    pages_of_wave(takes, before + (u64)r.delta, &s_taken);
     __syncthreads();
     const uint32_t taken = s_taken;
-    for (uint32_t g = threadIdx.x; g < taken; g += kPlanThreads) {   // new pages into the table
+    for (uint32_t g = threadIdx.x; g < taken; g += THREADS) {   // new pages into the table
         const uint32_t k = request_of_page(s_before, (uint32_t)A.n, g);
         A.table[k * A.table_stride + (uint32_t)owners[k].held + (g - s_before[k])] = A.free_pages[left - 1 - g];
     }
     if (total > A.cap) total = A.cap;
-    for (uint64_t t = threadIdx.x; t < total; t += kPlanThreads) {
+    for (uint64_t t = threadIdx.x; t < total; t += THREADS) {
         uint32_t k = 0, e = (uint32_t)A.n;
         while (e - k > 1) { const uint32_t m = (k + e) / 2; if (owners[m].first <= t) k = m; else e = m; }
         int64_t slot;
@@ -317,13 +352,14 @@ __global__ __launch_bounds__(kApplyThreads) void cache_trim_kernel(CacheArgs A, 
     for (int32_t j = lane_id(); j < r.delta; j += 64) to[j] = from[j];
 }
 
-// The whole call in one workgroup: at most kPlanThreads requests that hold kOnePages pages at the very most.
+// The whole call in one workgroup: a thread for each request, which hold kOnePages pages at the very most.
 constexpr uint64_t kOnePages = 16384;
 
-__global__ __launch_bounds__(kPlanThreads) void cache_trim_one_kernel(CacheArgs A) {
-    __shared__ u64 tmp[kPlanThreads / 64];
-    __shared__ uint32_t s_before[kPlanThreads], s_status, s_given;
-    __shared__ int32_t s_first[kPlanThreads];
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void cache_trim_one_kernel(CacheArgs A) {
+    __shared__ u64 tmp[THREADS / 64];
+    __shared__ uint32_t s_before[THREADS], s_status, s_given;
+    __shared__ int32_t s_first[THREADS];
     const uint64_t i = threadIdx.x;
     const int32_t n_free = *A.n_free;
     const bool bad = n_free < 0 || (uint32_t)n_free > A.n_pages;
@@ -332,19 +368,21 @@ __global__ __launch_bounds__(kPlanThreads) void cache_trim_one_kernel(CacheArgs 
     PlanRec r{};
     if (i < A.n) r = plan_trim(A.len[i], A.held[i], A.keep[i], A.page, A.max_pages);
     u64 all;
-    const u64 before = block_escan64((u64)r.delta, tmp, &all);   // (at most kOnePages pages)
+    const u64 before = block_escan64<THREADS>((u64)r.delta, tmp, &all);   // (at most kOnePages pages)
     s_before[i] = (uint32_t)before;
     s_first[i] = r.held - r.delta;
+    bool gives = false;
     if (i < A.n) {
         const bool served = trim_served(r, before, left, A.n_pages);
+        gives = served && r.delta;
         A.len_out[i] = served ? r.new_len : r.len;
         A.held_out[i] = served ? r.held - r.delta : r.held;
         if (!served) atomicOr(&s_status, r.flags ? r.flags : (uint32_t)kCachePool);
-        else if (r.delta) atomicMax(&s_given, (uint32_t)(before + (u64)r.delta));
     }
+    pages_of_wave(gives, before + (u64)r.delta, &s_given);
     __syncthreads();
     const uint32_t given = s_given;
-    for (uint32_t g = threadIdx.x; g < given; g += kPlanThreads) {
+    for (uint32_t g = threadIdx.x; g < given; g += THREADS) {
         const uint32_t k = request_of_page(s_before, (uint32_t)A.n, g);
         A.free_pages[left + g] = A.table[k * A.table_stride + (uint32_t)s_first[k] + (g - s_before[k])];
     }
@@ -364,17 +402,19 @@ Parts parts_of(const CacheArgs& A) {
 }  // namespace
 
 hipError_t launch_cache_slots(const CacheArgs& A, hipStream_t stream) {
-    if (A.n <= (uint64_t)kPlanThreads && A.cap <= kOneTokens) return launch(cache_slots_one_kernel, 1, kPlanThreads, stream, A);
+    if (A.n <= kOneSmall && A.cap <= kOneTokens / 4) return launch(cache_slots_one_kernel<kOneSmall>, 1, kOneSmall, stream, A);
+    if (A.n <= kPlanThreads && A.cap <= kOneTokens) return launch(cache_slots_one_kernel<kPlanThreads>, 1, kPlanThreads, stream, A);
     const Parts P = parts_of(A);
     hipError_t e = launch(cache_plan_kernel<false>, P.plan_blocks, kPlanThreads, stream, A, P.recs, P.blocks, P.head);
     if (e != hipSuccess) return e;
-    const uint64_t request_blocks = (A.n + kApplyWaves - 1) / kApplyWaves, token_blocks = A.n ? (A.cap + kTokenBlock - 1) / kTokenBlock : 0;
+    const uint64_t request_blocks = (A.n + kRequestBlock - 1) / kRequestBlock, token_blocks = A.n ? (A.cap + kTokenBlock - 1) / kTokenBlock : 0;
     return launch(cache_slots_kernel, 1 + request_blocks + token_blocks, kApplyThreads, stream, A, (const PlanRec*)P.recs, (const u64*)P.blocks, (const CacheHead*)P.head,
                   request_blocks);
 }
 
 hipError_t launch_cache_trim(const CacheArgs& A, hipStream_t stream) {
-    if (A.n <= (uint64_t)kPlanThreads && A.n * A.max_pages <= kOnePages) return launch(cache_trim_one_kernel, 1, kPlanThreads, stream, A);
+    if (A.n <= kOneSmall && A.n * A.max_pages <= kOnePages / 4) return launch(cache_trim_one_kernel<kOneSmall>, 1, kOneSmall, stream, A);
+    if (A.n <= kPlanThreads && A.n * A.max_pages <= kOnePages) return launch(cache_trim_one_kernel<kPlanThreads>, 1, kPlanThreads, stream, A);
     const Parts P = parts_of(A);
     hipError_t e = launch(cache_plan_kernel<true>, P.plan_blocks, kPlanThreads, stream, A, P.recs, P.blocks, P.head);
     if (e != hipSuccess) return e;

@@ -92,10 +92,10 @@ __global__ __launch_bounds__(kEmbedThreads) void embed_kernel(const int32_t* __r
 
 // ---- gradient: ids sorted -----------------------------------------------------------------------------------------
 // Stable counting sort of (id, position) by digits, the lowest first.  An id that is no row, and a position that does not
-// count, has the key n_rows and ends up behind all others.  A tile of kSortTile ids per workgroup:
+// count, has the key n_rows and ends up behind all others.  A tile of ids per workgroup:
 //   sort_count_kernel    how often each digit occurs in the tile
 //   sort_place_kernel    adds up the counts of the tiles before it, ranks the tile's ids and writes them to their places
-constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64, kSortRounds = kSortTile / kSortThreads;
+constexpr int kSortWaves = kSortThreads / 64;
 static_assert(kSortThreads == 2 * kSortBins, "two threads a digit add up the tiles' counts");
 
 __device__ __forceinline__ uint32_t sort_key(const int32_t* ids, uint64_t i, uint64_t valid, uint32_t rows) {
@@ -104,15 +104,15 @@ __device__ __forceinline__ uint32_t sort_key(const int32_t* ids, uint64_t i, uin
     return id < 0 || (uint32_t)id >= rows ? rows : (uint32_t)id;
 }
 
-template <bool FIRST>
+template <bool FIRST, int ROUNDS>
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(const int32_t* ids, const uint32_t* keys, uint64_t n, const uint64_t* n_dev,
                                                                   uint32_t rows, int shift, uint32_t mask, uint32_t* hist) {
     __shared__ uint32_t cnt[kSortBins];
     if (threadIdx.x < kSortBins) cnt[threadIdx.x] = 0;
     __syncthreads();
-    const uint64_t valid = FIRST ? ids_that_count(n, n_dev) : n, lo = (uint64_t)blockIdx.x * kSortTile;
+    const uint64_t valid = FIRST ? ids_that_count(n, n_dev) : n, lo = (uint64_t)blockIdx.x * kSortThreads * ROUNDS;
 #pragma unroll
-    for (int k = 0; k < kSortRounds; k++) {
+    for (int k = 0; k < ROUNDS; k++) {
         const uint64_t i = lo + (uint64_t)k * kSortThreads + threadIdx.x;
         if (i < n) atomicAdd(&cnt[((FIRST ? sort_key(ids, i, valid, rows) : keys[i]) >> shift) & mask], 1u);
     }
@@ -120,7 +120,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(const int32_t*
     if (threadIdx.x < kSortBins) hist[(uint64_t)blockIdx.x * kSortBins + threadIdx.x] = cnt[threadIdx.x];
 }
 
-template <bool FIRST>
+template <bool FIRST, int ROUNDS>
 __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const int32_t* ids, const uint32_t* keys, const uint32_t* poss, uint64_t n,
                                                                   const uint64_t* n_dev, uint32_t rows, int shift, uint32_t mask, int bits,
                                                                   const uint32_t* hist, uint32_t* keys_out, uint32_t* pos_out) {
@@ -129,10 +129,10 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const int32_t*
     __shared__ uint32_t tmp[kSortWaves];
     const int tid = threadIdx.x, w = wave_id(), lane = lane_id();
     const uint64_t valid = FIRST ? ids_that_count(n, n_dev) : n;
-    const uint64_t lo = (uint64_t)blockIdx.x * kSortTile + (uint64_t)w * (kSortTile / kSortWaves);
-    uint32_t key[kSortRounds], rank[kSortRounds];
+    const uint64_t lo = ((uint64_t)blockIdx.x * kSortThreads + (uint64_t)w * 64) * ROUNDS;
+    uint32_t key[ROUNDS], rank[ROUNDS];
 #pragma unroll
-    for (int k = 0; k < kSortRounds; k++) {
+    for (int k = 0; k < ROUNDS; k++) {
         const uint64_t i = lo + (uint64_t)k * 64 + lane;
         key[k] = i < n ? (FIRST ? sort_key(ids, i, valid, rows) : keys[i]) : 0;
     }
@@ -153,9 +153,9 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const int32_t*
     if (tid < kSortBins) { all += half_all[digit]; before += half_before[digit]; } else all = 0;
     uint32_t total;
     uint32_t start = block_escan<kSortWaves>(all, tmp, &total) + before;   // (of the first kSortBins threads)
-    // ranks: a wave has kSortTile / kSortWaves ids in a row, 64 at a time
+    // ranks: a wave has 64 ROUNDS ids in a row, 64 at a time
 #pragma unroll
-    for (int k = 0; k < kSortRounds; k++) {
+    for (int k = 0; k < ROUNDS; k++) {
         const bool in = lo + (uint64_t)k * 64 + lane < n;
         const uint32_t d = (key[k] >> shift) & mask;
         u64 same = __ballot(in);
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const int32_t*
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kSortRounds; k++) {
+    for (int k = 0; k < ROUNDS; k++) {
         const uint64_t i = lo + (uint64_t)k * 64 + lane;
         if (i < n) {
             const uint32_t at = cnt[w][(key[k] >> shift) & mask] + rank[k];
@@ -216,7 +216,8 @@ __global__ __launch_bounds__(kSortThreads) void sort_rank_kernel(const int32_t* 
         count += (v.x < bound) + (v.y < bound) + (v.z < bound) + (v.w < bound);
     }
     if (part == 0) for (uint32_t j = i0; j < i0 + kRankMine; j++) count += j < i && key[j] == k ? 1u : 0u;
-    atomicAdd(&rank[threadIdx.x % kRankMine], count);
+    count += __shfl_xor(count, 32, 64);
+    if (!(threadIdx.x & 32)) atomicAdd(&rank[threadIdx.x % kRankMine], count);
     __syncthreads();
     if (part == 0 && i < n) {
         keys_out[rank[threadIdx.x]] = k;
@@ -225,7 +226,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_rank_kernel(const int32_t* 
 }
 
 // ---- gradient: runs of one id added up ----------------------------------------------------------------------------
-// A wave walks through `chunk` sorted positions for 512 columns, in order, four at a time: the four rows of the gradient and, where
+// A wave walks through `chunk` sorted positions for 512 columns, in order, eight at a time: the eight rows of the gradient and, where
 // a run of one id ends, the row of the table it is added to are loaded together.  Keys and positions of the whole chunk are in
 // one register each (lane j has position j).  A run that lies inside the chunk is stored at once.  The parts of a run that crosses
 // from one wave of a workgroup to the next meet in LDS; a run that crosses the workgroup's border leaves its part in the
@@ -233,7 +234,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_rank_kernel(const int32_t* 
 // on; grad_join_kernel adds these up at the workgroup where the run starts.  Nothing is added by atomics: the same ids give the
 // same bits.
 constexpr int kGradThreads = 64 * kGradWaves;
-constexpr int kGradGroup = 4;
+constexpr int kGradGroup = 8;
 constexpr uint32_t kGradCols = 512;
 constexpr uint64_t kGradOnce = 256ull << 20;   // bytes of gradient (launch_embed_grad)
 constexpr uint32_t kZeroRows = 64;   // rows a workgroup looks after when the gradient is written whole
@@ -539,17 +540,27 @@ hipError_t launch_embed_grad(const EmbedGradArgs& A, hipStream_t stream) {
         int bits = 1;
         while (bits < 32 && (rows >> bits)) bits++;            // keys are 0 .. rows
         const int passes = (bits + kSortBits - 1) / kSortBits, per = (bits + passes - 1) / passes;
-        const uint64_t tiles = (A.n + kSortTile - 1) / kSortTile;
+        const uint64_t tiles = sort_tiles(A.n);
         const uint32_t mask = (1u << per) - 1;
+        auto pass = [&](auto first, auto rounds, int shift, const uint32_t* k, const uint32_t* q, uint32_t* k_out, uint32_t* q_out) {
+            const hipError_t e = launch(sort_count_kernel<first.value, rounds.value>, tiles, kSortThreads, stream, A.ids, k, A.n, A.n_dev, rows, shift, mask, hist);
+            if (e != hipSuccess) return e;
+            return launch(sort_place_kernel<first.value, rounds.value>, tiles, kSortThreads, stream, A.ids, k, q, A.n, A.n_dev, rows, shift, mask, per,
+                          (const uint32_t*)hist, k_out, q_out);
+        };
+        auto pass_of = [&](auto rounds, int p) {
+            const int from = (p + 1) & 1, to = p & 1;
+            return p ? pass(std::false_type(), rounds, p * per, kb[from], pb[from], kb[to], pb[to])
+                     : pass(std::true_type(), rounds, 0, kb[from], pb[from], kb[to], pb[to]);
+        };
         for (int p = 0; p < passes; p++) {
-            const int shift = p * per, from = (p + 1) & 1, to = p & 1;
-            const uint32_t *k = kb[from], *q = pb[from], *h = hist;
-            hipError_t e = launch(p ? sort_count_kernel<false> : sort_count_kernel<true>, tiles, kSortThreads, stream, A.ids, k, A.n, A.n_dev, rows, shift, mask, hist);
+            const int r = sort_rounds(A.n);
+            const hipError_t e = r == 1   ? pass_of(std::integral_constant<int, 1>(), p)
+                                 : r == 2 ? pass_of(std::integral_constant<int, 2>(), p)
+                                          : pass_of(std::integral_constant<int, 4>(), p);
             if (e != hipSuccess) return e;
-            e = launch(p ? sort_place_kernel<false> : sort_place_kernel<true>, tiles, kSortThreads, stream, A.ids, k, q, A.n, A.n_dev, rows, shift, mask, per, h, kb[to], pb[to]);
-            if (e != hipSuccess) return e;
-            keys = kb[to];
-            poss = pb[to];
+            keys = kb[p & 1];
+            poss = pb[p & 1];
         }
     }
     const uint64_t walk_blocks = W.blocks * col_tiles;

@@ -63,8 +63,12 @@ struct VerifyArgs {
 // ---- workspaces ---------------------------------------------------------------------------------------------------
 constexpr uint64_t align256(uint64_t b) { return (b + 255) & ~255ull; }
 
-// Ids are sorted in tiles of kSortTile by digits of at most kSortBits bits.
-constexpr int kSortTile = 2048, kSortBits = 9, kSortBins = 1 << kSortBits;
+// Ids are sorted by digits of at most kSortBits bits, in tiles of kSortThreads times 1, 2 or 4: small tiles are more workgroups,
+// but each adds up the counts of all of them.  Whole gradients of 64 columns by tile (us): 16,384 ids 26 / 30 / 38, 65,536 40 / 42 /
+// 50, 262,144 90 / 83 / 86, 2^20 353 / 207 / 173.
+constexpr int kSortThreads = 1024, kSortBits = 9, kSortBins = 1 << kSortBits;
+inline int sort_rounds(uint64_t n) { return n <= 65536 ? 1 : n <= 262144 ? 2 : 4; }
+inline uint64_t sort_tiles(uint64_t n) { const uint64_t t = (uint64_t)kSortThreads * sort_rounds(n); return (n + t - 1) / t; }
 // Few ids are not sorted: every position looks for the others of its id by itself, a workgroup for each and 512 columns.  Up to
 // kRankIds ids are sorted in one launch by counting, more digit by digit.
 constexpr uint64_t kDirectIds = 2048, kDirectBlocks = 4096, kRankIds = 8192;
@@ -87,7 +91,7 @@ inline GradWork grad_work(uint64_t n, uint64_t dim) {
     uint64_t at = 0;
     auto take = [&](uint64_t b) { const uint64_t p = at; at += align256(b); return p; };
     w.keys0 = take(4 * n); w.pos0 = take(4 * n); w.keys1 = take(4 * n); w.pos1 = take(4 * n);
-    w.hist = take(((n + kSortTile - 1) / kSortTile) * kSortBins * 4);
+    w.hist = take(sort_tiles(n) * kSortBins * 4);
     w.part = take(2 * w.blocks * w.dim8 * 4);
     w.total = at ? at : 256;
     return w;

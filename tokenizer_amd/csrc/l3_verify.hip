@@ -197,8 +197,10 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
                 if (sum > border && found == 0x7FFFFFFF) found = mine_last;
             }
         }
-        if (found != 0x7FFFFFFF) atomicMin(&s_token, found);
-        if (mine_last >= 0) atomicMax(&s_last, mine_last);
+        // columns ascend with the lanes: a wave's first found entry is its first lane's, its last entry with weight its last lane's
+        const u64 any_found = __ballot(found != 0x7FFFFFFF), any_last = __ballot(mine_last >= 0);
+        if (any_found && lane == __builtin_ctzll(any_found)) atomicMin(&s_token, found);
+        if (any_last && lane == 63 - __builtin_clzll(any_last)) atomicMax(&s_last, mine_last);
         __syncthreads();
         if (threadIdx.x == 0 && R.state != kBadRequest) A.out[i * (A.max_draft + 1ull) + R.a] = s_token != 0x7FFFFFFF ? s_token : s_last;
         __syncthreads();
