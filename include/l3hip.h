@@ -176,7 +176,7 @@ int l3_embed(l3_ctx* ctx, const int32_t* d_ids, uint64_t n_ids, const uint64_t* 
  * summed in 32 bits in a fixed order (the same inputs give the same bits).
  * accumulate = 1: table[v] = table[v] + G[v] for the rows that occur, rounded once; other rows are not touched.
  * accumulate = 0: table = G, rows that do not occur become zero.
- * Ids outside [0, n_rows) and ids behind *d_n_ids take no part.  n_ids <= 2^24, n_rows <= 2^29.  d_work:
+ * Ids outside [0, n_rows) and ids behind *d_n_ids take no part.  n_ids <= 2^24, n_rows <= 2^28.  d_work:
  * l3_embed_grad_workspace(n_ids, dim) bytes (0: the sizes are out of range). */
 uint64_t l3_embed_grad_workspace(uint64_t n_ids, uint64_t dim);
 int l3_embed_grad(l3_ctx* ctx, const int32_t* d_ids, uint64_t n_ids, const uint64_t* d_n_ids, const void* d_grad, int grad_type,

@@ -89,7 +89,7 @@ REFUSED = [
     ("embed", dict(ids=None), "null"), ("embed", dict(table=None), "null"), ("embed", dict(out=None), "null"), ("embed", dict(ids=AT + 2), "aligned"),
     ("embed", dict(n_dev=AT + 4), "aligned"), ("embed", dict(table=AT + 1), "aligned"), ("embed", dict(dtype=0, table=AT + 2), "aligned"),
     ("embed", dict(out_dtype=0, out=AT + 2), "aligned"),
-    ("grad", dict(dtype=7), "type"), ("grad", dict(table_dtype=3), "type"), ("grad", dict(n=2 ** 24 + 1), "split"), ("grad", dict(rows=0), "n_rows"), ("grad", dict(rows=2 ** 29 + 1), "n_rows"),
+    ("grad", dict(dtype=7), "type"), ("grad", dict(table_dtype=3), "type"), ("grad", dict(n=2 ** 24 + 1), "split"), ("grad", dict(rows=0), "n_rows"), ("grad", dict(rows=2 ** 28 + 1), "n_rows"),
     ("grad", dict(dim=0), "dim"), ("grad", dict(grad_stride=10), "stride"), ("grad", dict(table_stride=10), "stride"), ("grad", dict(accumulate=2), "accumulate"),
     ("grad", dict(table=None), "null"), ("grad", dict(ids=None), "null"), ("grad", dict(grad=None), "null"), ("grad", dict(work=None), "null"),
     ("grad", dict(table=AT + 2), "aligned"), ("grad", dict(grad=AT + 1), "aligned"), ("grad", dict(work=AT + 8), "16 bytes"),

@@ -353,7 +353,7 @@ __global__ __launch_bounds__(kApplyThreads) void cache_trim_kernel(CacheArgs A, 
 }
 
 // The whole call in one workgroup: a thread for each request, which hold kOnePages pages at the very most.
-constexpr uint64_t kOnePages = 16384;
+constexpr uint64_t kOnePages = 4096;
 
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void cache_trim_one_kernel(CacheArgs A) {
@@ -382,9 +382,15 @@ __global__ __launch_bounds__(THREADS) void cache_trim_one_kernel(CacheArgs A) {
     pages_of_wave(gives, before + (u64)r.delta, &s_given);
     __syncthreads();
     const uint32_t given = s_given;
-    for (uint32_t g = threadIdx.x; g < given; g += THREADS) {
-        const uint32_t k = request_of_page(s_before, (uint32_t)A.n, g);
-        A.free_pages[left + g] = A.table[k * A.table_stride + (uint32_t)s_first[k] + (g - s_before[k])];
+    for (uint32_t g = threadIdx.x; g < given; g += 4 * THREADS) {
+        int32_t page[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint32_t x = g + j * THREADS < given ? g + j * THREADS : g, k = request_of_page(s_before, (uint32_t)A.n, x);
+            page[j] = A.table[k * A.table_stride + (uint32_t)s_first[k] + (x - s_before[k])];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) if (g + j * THREADS < given) A.free_pages[left + g + j * THREADS] = page[j];
     }
     if (threadIdx.x == 0) {
         *A.n_free_out = bad ? n_free : n_free + (int32_t)given;

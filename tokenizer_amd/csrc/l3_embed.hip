@@ -20,41 +20,42 @@ __device__ __forceinline__ uint64_t ids_that_count(uint64_t n, const uint64_t* n
     return m < n ? m : n;
 }
 
-// A row is worked on in vectors of eight columns.  The last of a row whose width is no multiple of eight begins `skip` columns
-// early, so that every load has eight elements; those columns belong to the vector before.  Rows of fewer than eight columns
-// (SMALL) are loaded one element at a time.
+// A row is worked on in vectors of N columns.  The last of a row whose width is no multiple of N begins `skip` columns early, so that
+// every load has N elements; those columns belong to the vector before.  Rows of fewer than eight columns (SMALL) are loaded one
+// element at a time.
 struct Cols { uint32_t col, skip; };
+template <uint32_t N = 8>
 __device__ __forceinline__ Cols cols_of(uint32_t vec, uint32_t dim) {
-    const uint32_t c = vec * 8;
-    if (c + 8 <= dim || dim < 8) return {c, 0};
-    return {dim - 8, c + 8 - dim};
+    const uint32_t c = vec * N;
+    if (c + N <= dim || dim < 8) return {c, 0};
+    return {dim - N, c + N - dim};
 }
-template <bool SMALL, bool ONCE = false, class T>
-__device__ __forceinline__ typename Eight<T>::V load_cols(const T* row, Cols c, uint32_t dim) {
+template <bool SMALL, bool ONCE = false, int N = 8, class T>
+__device__ __forceinline__ typename Few<T, N>::V load_cols(const T* row, Cols c, uint32_t dim) {
     if constexpr (SMALL) {
-        typename Eight<T>::V v = (T)0.f;
-        for (uint32_t i = 0; i < 8; i++) if (i < dim) v[i] = row[i];
+        typename Few<T, N>::V v = (T)0.f;
+        for (uint32_t i = 0; i < N; i++) if (c.col + i < dim) v[i] = row[c.col + i];
         return v;
     } else {
-        return ONCE ? load8_once(row + c.col) : load8(row + c.col);
+        return ONCE ? load8_once<N>(row + c.col) : load8<N>(row + c.col);
     }
 }
 // The vector's own columns; SHARED: the skipped ones hold the same values as their owner stores.
-template <bool SMALL, bool SHARED, bool ONCE = false, class T>
-__device__ __forceinline__ void store_cols(T* row, Cols c, uint32_t dim, F8 v) {
+template <bool SMALL, bool SHARED, bool ONCE = false, int N = 8, class T>
+__device__ __forceinline__ void store_cols(T* row, Cols c, uint32_t dim, typename Few<T, N>::F v) {
     if constexpr (SMALL) {
-        for (uint32_t i = 0; i < 8; i++) if (i < dim) row[i] = (T)v[i];
+        for (uint32_t i = 0; i < N; i++) if (c.col + i < dim) row[c.col + i] = (T)v[i];
     } else if (SHARED || c.skip == 0) {
-        ONCE ? store8_once(row + c.col, v) : store8(row + c.col, v);
+        ONCE ? store8_once<N>(row + c.col, v) : store8<N>(row + c.col, v);
     } else {
 #pragma unroll
-        for (uint32_t i = 1; i < 8; i++) if (i >= c.skip) row[c.col + i] = (T)v[i];
+        for (uint32_t i = 1; i < N; i++) if (i >= c.skip) row[c.col + i] = (T)v[i];
     }
 }
 
 // ---- lookup -------------------------------------------------------------------------------------------------------
-// A thread has PER times eight neighbouring columns, all loads in flight before the first store.  What is divided is a workgroup's
-// first vector (once) and 32-bit offsets from it.
+// A thread has PER times as many neighbouring columns as make 16 bytes of the output, all loads in flight before the first store.
+// What is divided is a workgroup's first vector (once) and 32-bit offsets from it.
 constexpr int kEmbedThreads = 256;
 constexpr uint64_t kEmbedOnce = 1u << 20, kEmbedMany = 1u << 24;   // vectors (launch_embed)
 
@@ -63,7 +64,9 @@ __global__ __launch_bounds__(kEmbedThreads) void embed_kernel(const int32_t* __r
                                                               const T* __restrict__ table, uint32_t rows, uint32_t dim, uint64_t stride,
                                                               O* __restrict__ out, uint64_t out_stride, float scale) {
     constexpr uint32_t kTile = kEmbedThreads * PER;
-    const uint32_t per_row = (dim + 7) / 8;
+    constexpr int N = 16 / sizeof(O);
+    typedef typename Few<T, N>::F F;
+    const uint32_t per_row = (dim + N - 1) / N;
     const uint64_t count = ids_that_count(n, n_dev), total = count * per_row;
     for (uint64_t g0 = (uint64_t)blockIdx.x * kTile; g0 < total; g0 += (uint64_t)gridDim.x * kTile) {
         const uint64_t t0 = g0 / per_row;
@@ -71,21 +74,21 @@ __global__ __launch_bounds__(kEmbedThreads) void embed_kernel(const int32_t* __r
         uint64_t t[PER];
         Cols c[PER];
         int32_t id[PER];
-        typename Eight<T>::V v[PER];
+        typename Few<T, N>::V v[PER];
 #pragma unroll
         for (int k = 0; k < PER; k++) {
             const uint32_t at = r0 + k * kEmbedThreads + threadIdx.x, row = at / per_row;
             t[k] = t0 + row;
-            c[k] = cols_of(at - row * per_row, dim);
+            c[k] = cols_of<N>(at - row * per_row, dim);
             id[k] = ids[t[k] < count ? t[k] : count - 1];
         }
 #pragma unroll
         for (int k = 0; k < PER; k++)   // (an id that is no row loads row 0 and stores zeros)
-            v[k] = load_cols<SMALL>(table + (uint64_t)((uint32_t)id[k] < rows ? (uint32_t)id[k] : 0u) * stride, c[k], dim);
+            v[k] = load_cols<SMALL, false, N>(table + (uint64_t)((uint32_t)id[k] < rows ? (uint32_t)id[k] : 0u) * stride, c[k], dim);
 #pragma unroll
         for (int k = 0; k < PER; k++) {
-            const F8 x = to_f8(v[k]) * scale;
-            if (t[k] < count) store_cols<SMALL, true, ONCE>(out + t[k] * out_stride, c[k], dim, (uint32_t)id[k] < rows ? x : (F8)0.f);
+            const F x = __builtin_convertvector(v[k], F) * scale;
+            if (t[k] < count) store_cols<SMALL, true, ONCE, N>(out + t[k] * out_stride, c[k], dim, (uint32_t)id[k] < rows ? x : (F)0.f);
         }
     }
 }
@@ -203,7 +206,18 @@ __global__ __launch_bounds__(kSortThreads) void sort_rank_kernel(const int32_t* 
     const uint32_t valid = (uint32_t)ids_that_count(n, n_dev), i0 = blockIdx.x * kRankMine;
     constexpr uint32_t kParts = kSortThreads / kRankMine;
     const uint32_t quads = (n + 4 * kParts - 1) / (4 * kParts), all = quads * 4 * kParts;   // (kRankIds is a multiple of 4 kParts)
-    for (uint32_t j = threadIdx.x; j < all; j += kSortThreads) key[j] = j < n ? sort_key(ids, j, valid, rows) : ~0u;
+    constexpr int kPer = (int)(kRankIds / kSortThreads);
+    int32_t id[kPer];
+#pragma unroll
+    for (int x = 0; x < kPer; x++) {
+        const uint32_t j = (uint32_t)x * kSortThreads + threadIdx.x;
+        id[x] = j < valid ? ids[j] : -1;
+    }
+#pragma unroll
+    for (int x = 0; x < kPer; x++) {
+        const uint32_t j = (uint32_t)x * kSortThreads + threadIdx.x;
+        if (j < all) key[j] = j >= n ? ~0u : id[x] < 0 || (uint32_t)id[x] >= rows ? rows : (uint32_t)id[x];
+    }
     if (threadIdx.x < kRankMine) rank[threadIdx.x] = 0;
     __syncthreads();
     const uint32_t i = i0 + threadIdx.x % kRankMine, part = threadIdx.x / kRankMine, k = key[i];   // (i < all: all is a multiple of kRankMine)
@@ -237,17 +251,32 @@ constexpr int kGradThreads = 64 * kGradWaves;
 constexpr int kGradGroup = 8;
 constexpr uint32_t kGradCols = 512;
 constexpr uint64_t kGradOnce = 256ull << 20;   // bytes of gradient (launch_embed_grad)
-constexpr uint32_t kZeroRows = 64;   // rows a workgroup looks after when the gradient is written whole
+constexpr uint32_t kZeroRows = 32;   // rows a workgroup looks after when the gradient is written whole
 
-// Rows [r0, r0 + kZeroRows) of which `named` has no bit become zero; by a whole workgroup.
+// Rows [r0, r0 + kZeroRows) of which `named` has no mark become zero; by a whole workgroup.  16 bytes a lane, the last ones of a row
+// overlapping those before.
 template <bool SMALL, class T>
-__device__ __forceinline__ void zero_rows(T* table, uint64_t table_stride, uint64_t rows, uint32_t dim, uint64_t r0, u64 named) {
-    static_assert(kZeroRows == 64, "a word of bits");
-    const uint32_t per_row = (dim + 7) / 8;
+__device__ __forceinline__ void zero_rows(T* table, uint64_t table_stride, uint64_t rows, uint32_t dim, uint64_t r0, const uint32_t* named) {
+    constexpr int N = 16 / sizeof(T);
+    const uint32_t per_row = (dim + N - 1) / N;
     for (uint32_t j = wave_id(); j < kZeroRows && r0 + j < rows; j += kGradWaves) {
-        if ((named >> j) & 1) continue;
-        for (uint32_t k = lane_id(); k < per_row; k += 64) store_cols<SMALL, true>(table + (r0 + j) * table_stride, cols_of(k, dim), dim, (F8)0.f);
+        if (named[j]) continue;
+        for (uint32_t k = lane_id(); k < per_row; k += 64)
+            store_cols<SMALL, true, false, N>(table + (r0 + j) * table_stride, cols_of<N>(k, dim), dim, (typename Few<T, N>::F)0.f);
     }
+}
+
+// The first position of the sorted keys that is not below r, 64 places at a time, by a whole wave.
+__device__ __forceinline__ uint64_t first_key(const uint32_t* __restrict__ keys, uint64_t n, uint64_t r) {
+    uint64_t lo = 0, len = n;                // the keys before lo are below r, key lo + len is not
+    while (len) {
+        const uint64_t step = (len + 63) / 64, at = lo + ((uint64_t)lane_id() + 1) * step - 1;
+        const u64 below = __ballot(at < lo + len && keys[at < lo + len ? at : lo] < r);
+        const uint64_t k = (uint64_t)__popcll(below);                     // (keys ascend: the low lanes)
+        lo += k * step;
+        len = len - k * step < step ? len - k * step : step - 1;
+    }
+    return lo;
 }
 
 struct GradWalk {
@@ -265,12 +294,16 @@ template <class G, class T, bool ONCE, bool SMALL>
 __global__ __launch_bounds__(kGradThreads) void grad_walk_kernel(GradWalk P, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ poss,
                                                                  const G* __restrict__ grad, T* __restrict__ table, float* __restrict__ part) {
     const uint32_t rows = P.rows, dim = P.dim;
-    if (blockIdx.x >= P.walk_blocks) {   // rows that no id names, when the gradient is written whole: a binary search a row
+    if (blockIdx.x >= P.walk_blocks) {   // rows that no id names, when the gradient is written whole
+        __shared__ uint32_t named[kZeroRows];
+        __shared__ uint64_t ends[2];
         const uint64_t r0 = (uint64_t)(blockIdx.x - P.walk_blocks) * kZeroRows;
-        const uint32_t r = (uint32_t)r0 + lane_id();
-        uint64_t a = 0, b = P.n;
-        while (a < b) { const uint64_t m = (a + b) / 2; if (keys[m] < r) a = m + 1; else b = m; }
-        zero_rows<SMALL>(table, P.table_stride, rows, dim, r0, __ballot(a < P.n && keys[a] == r));
+        if (threadIdx.x < kZeroRows) named[threadIdx.x] = 0;
+        if (wave_id() < 2) ends[wave_id()] = first_key(keys, P.n, r0 + wave_id() * kZeroRows);
+        __syncthreads();
+        for (uint64_t i = ends[0] + threadIdx.x; i < ends[1]; i += kGradThreads) named[keys[i] - r0] = 1;
+        __syncthreads();
+        zero_rows<SMALL>(table, P.table_stride, rows, dim, r0, named);
         return;
     }
     __shared__ F8 heads[kGradWaves][64];
@@ -412,14 +445,14 @@ __global__ __launch_bounds__(kGradThreads) void grad_direct_kernel(const int32_t
     const int w = __builtin_amdgcn_readfirstlane((int)wave_id()), lane = lane_id();
     if (blockIdx.x >= n * tiles) {   // rows that no id names, when the gradient is written whole
         const uint64_t r0 = (uint64_t)(blockIdx.x - n * tiles) * kZeroRows;
-        if (threadIdx.x == 0) words[0] = 0;
+        if (threadIdx.x < kZeroRows) list[threadIdx.x] = 0;
         __syncthreads();
         for (uint32_t j = threadIdx.x; j < valid; j += kGradThreads) {
             const uint64_t d = (uint64_t)(int64_t)ids[j] - r0;   // (below kZeroRows for these rows only)
-            if (d < kZeroRows) atomicOr(&words[0], 1ull << d);
+            if (d < kZeroRows) list[d] = 1;
         }
         __syncthreads();
-        zero_rows<SMALL>(table, table_stride, rows, dim, r0, words[0]);
+        zero_rows<SMALL>(table, table_stride, rows, dim, r0, list);
         return;
     }
     const uint32_t t = blockIdx.x / tiles;
@@ -491,17 +524,17 @@ hipError_t with_small(uint64_t dim, F f) {
 
 hipError_t launch_embed(const EmbedArgs& A, hipStream_t stream) {
     if (A.n == 0) return hipSuccess;
-    const uint64_t vectors = A.n * ((A.dim + 7) / 8);
+    const uint64_t per = 16 / dtype_size(A.out_dtype), vectors = A.n * ((A.dim + per - 1) / per);
     return with_dtype(A.dtype, [&](auto t) {
         typedef decltype(t) T;
         return with_dtype(A.out_dtype, [&](auto o) {
             typedef decltype(o) O;
             return with_small(A.dim, [&](auto small) {
-                const int per = vectors >= kEmbedMany ? 4 : 1;
+                const int many = vectors >= kEmbedMany ? 4 : 1;
                 auto* kernel = vectors >= kEmbedMany   ? embed_kernel<T, O, 4, true, small.value>
                                : vectors >= kEmbedOnce ? embed_kernel<T, O, 1, true, small.value>
                                                        : embed_kernel<T, O, 1, false, small.value>;
-                const uint64_t tile = (uint64_t)kEmbedThreads * per;
+                const uint64_t tile = (uint64_t)kEmbedThreads * many;
                 return launch(kernel, capped((vectors + tile - 1) / tile), kEmbedThreads, stream, A.ids, A.n, A.n_dev, (const T*)A.table, (uint32_t)A.rows,
                               (uint32_t)A.dim, A.stride, (O*)A.out, A.out_stride, A.scale);
             });

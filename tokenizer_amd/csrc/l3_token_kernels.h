@@ -31,25 +31,29 @@ hipError_t with_dtype(int code, F f) {
     return code == kF32 ? f(float()) : code == kF16 ? f(_Float16()) : f((__bf16)0.f);
 }
 
-// Eight neighbouring elements, aligned like one of them: any row start and stride is fine, gfx950 takes unaligned 16-byte accesses.
-template <class T> struct Eight {
-    typedef T V __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+// N neighbouring elements, aligned like one of them: any row start and stride is fine, gfx950 takes unaligned 16-byte accesses.
+template <class T, int N = 8> struct Few {
+    typedef T V __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+    typedef float F __attribute__((ext_vector_type(N)));
 };
+template <class T> using Eight = Few<T, 8>;
 typedef float F8 __attribute__((ext_vector_type(8)));
-template <class T>
-__device__ __forceinline__ typename Eight<T>::V load8(const T* p) { return *reinterpret_cast<const typename Eight<T>::V*>(p); }
-// The same for data that is used once: it need not stay in the caches.
-template <class T>
-__device__ __forceinline__ typename Eight<T>::V load8_once(const T* p) { return __builtin_nontemporal_load(reinterpret_cast<const typename Eight<T>::V*>(p)); }
-template <class T>
-__device__ __forceinline__ void store8_once(T* p, F8 v) {
-    __builtin_nontemporal_store(__builtin_convertvector(v, typename Eight<T>::V), reinterpret_cast<typename Eight<T>::V*>(p));
-}
+template <int N = 8, class T>
+__device__ __forceinline__ typename Few<T, N>::V load8(const T* p) { return *reinterpret_cast<const typename Few<T, N>::V*>(p); }
 template <class V>
 __device__ __forceinline__ F8 to_f8(V v) { return __builtin_convertvector(v, F8); }
-template <class T>
-__device__ __forceinline__ void store8(T* p, F8 v) {   // rounded to nearest, ties to even
-    *reinterpret_cast<typename Eight<T>::V*>(p) = __builtin_convertvector(v, typename Eight<T>::V);
+// Stores round to nearest, ties to even.
+template <int N = 8, class T>
+__device__ __forceinline__ void store8(T* p, typename Few<T, N>::F v) {
+    *reinterpret_cast<typename Few<T, N>::V*>(p) = __builtin_convertvector(v, typename Few<T, N>::V);
+}
+// The same for data that is used once: it need not stay in the caches.  (Stores: 16 bytes a lane, neighbouring lanes side by side --
+// what a wave's store leaves open of a cache line is not put together with the next store's.)
+template <int N = 8, class T>
+__device__ __forceinline__ typename Few<T, N>::V load8_once(const T* p) { return __builtin_nontemporal_load(reinterpret_cast<const typename Few<T, N>::V*>(p)); }
+template <int N = 8, class T>
+__device__ __forceinline__ void store8_once(T* p, typename Few<T, N>::F v) {
+    __builtin_nontemporal_store(__builtin_convertvector(v, typename Few<T, N>::V), reinterpret_cast<typename Few<T, N>::V*>(p));
 }
 
 }  // namespace

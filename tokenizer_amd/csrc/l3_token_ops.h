@@ -15,7 +15,7 @@ L3_HD int dtype_size(int t) { return t == kF32 ? 4 : 2; }
 constexpr uint64_t kMaxCount = 0x7FFFFFFFull;    // ids, rows, tokens, pages: 31 bits
 constexpr uint64_t kMaxDim = 1ull << 24;
 constexpr uint64_t kMaxGradIds = 1ull << 24;     // ids sorted in one call: every tile adds up the counts of all tiles before it
-constexpr uint64_t kMaxGradRows = 1ull << 29;    // rows of a gradient: one workgroup for 64 of them
+constexpr uint64_t kMaxGradRows = 1ull << 28;    // rows of a gradient: one workgroup for 32 of them
 constexpr uint64_t kMaxSeqs = 1ull << 20;
 constexpr uint64_t kMaxStride = kMaxCount;       // elements: (2^31 - 1) rows of (2^31 - 1) elements of 4 bytes stay inside 64 bits
 
@@ -149,7 +149,7 @@ inline const char* check_embed(const EmbedArgs& A) {
 inline const char* check_embed_grad(const EmbedGradArgs& A) {
     if (bad_dtype(A.dtype) || bad_dtype(A.table_dtype)) return "unknown element type";
     if (A.n > kMaxGradIds) return "more than 2^24 ids: split the call";
-    if (A.rows == 0 || A.rows > kMaxGradRows) return "n_rows must be 1 .. 2^29";
+    if (A.rows == 0 || A.rows > kMaxGradRows) return "n_rows must be 1 .. 2^28";
     if (A.dim == 0 || A.dim > kMaxDim) return "dim must be 1 .. 2^24";
     if (A.grad_stride < A.dim || A.table_stride < A.dim || A.grad_stride > kMaxStride || A.table_stride > kMaxStride)
         return "a row stride is smaller than dim or above 2^31 - 1";
