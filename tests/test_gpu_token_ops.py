@@ -130,6 +130,19 @@ def test_embed_offsets_beyond_32_bits(ctx, torch):
     assert (out[dim:dim + 64] == -7).all() and (out[stride - 64:stride] == -7).all()
 
 
+@pytest.mark.parametrize("n, dim, T, O", [(2100, 4096, BF16, BF16), (4097, 1024, F32, F32), (2500, 4001, F16, F32), (33000, 4096, F16, BF16)])
+def test_embed_outputs_that_pass_the_caches(ctx, torch, n, dim, T, O):
+    """Large outputs take other kernels; the rows and types of the whole output against torch's own conversion."""
+    rows = 70
+    table = torch.randn(rows, dim, device="cuda").to(_t(torch, T))
+    ids = torch.randint(-1, rows + 1, (n,), device="cuda", dtype=torch.int32)
+    out = torch.full((n + 1, dim), -7.0, dtype=_t(torch, O), device="cuda")
+    ctx.embed(ids.data_ptr(), n, table.data_ptr(), T, rows, dim, dim, out.data_ptr(), O, dim, 0.5)
+    there = ((ids >= 0) & (ids < rows))[:, None]
+    want = torch.where(there, table[ids.clamp(0, rows - 1).long()].float() * 0.5, torch.zeros(1, device="cuda")).to(_t(torch, O))
+    assert torch.equal(out[:n], want) and (out[n] == -7).all()
+
+
 # ---- gradient -----------------------------------------------------------------------------------------------------
 def _grad_case(ctx, torch, rng, ids, dim, G, T, rows, accumulate, scale=1.0, grad_stride=None, table_stride=None, shift=0, n_dev=None, whole=False):
     n = len(ids)
@@ -230,6 +243,28 @@ def test_grad_counts_on_the_device(ctx, torch, count):
     rng = np.random.default_rng(5)
     for accumulate in (False, True):
         _grad_case(ctx, torch, rng, _ids(rng, 1000, 50), 16, F32, F32, 50, accumulate, n_dev=count)
+
+
+@pytest.mark.parametrize("n", [5, 3000])
+def test_grad_offsets_beyond_32_bits(ctx, torch, n):
+    """Element offsets pass 2^32 in the gradient and in the table (rows far apart); with and without a sort."""
+    dim, rows = 16, 3
+    gs, ts = 2 ** 32 // (n - 1) + 3, (1 << 30) + 5
+    grad = torch.zeros((n - 1) * gs + dim, dtype=torch.float16, device="cuda")             # 8 GiB
+    table = torch.zeros(2 * ts + dim, dtype=torch.float16, device="cuda")                  # 4 GiB
+    at = (torch.arange(n, device="cuda")[:, None] * gs + torch.arange(dim, device="cuda")).reshape(-1)
+    g = torch.randint(-4, 5, (n, dim), device="cuda").half()
+    grad[at] = g.reshape(-1)
+    ids = (torch.arange(n, device="cuda") % 3).int()
+    need = capi.embed_grad_workspace(n, dim)
+    work = torch.empty(need, dtype=torch.uint8, device="cuda")
+    for accumulate in (False, True):
+        ctx.embed_grad(ids.data_ptr(), n, grad.data_ptr(), F16, gs, rows, dim, table.data_ptr(), F16, ts, work.data_ptr(), need, 1.0, accumulate)
+        for r in range(rows):
+            want = g[ids == r].float().sum(0)                                               # whole numbers: exact in 32 bits ...
+            want = want.half() if not accumulate else (want.half().float() + want).half()   # ... rounded where they are stored
+            assert torch.equal(table[r * ts:r * ts + dim], want)
+        assert (table[dim:dim + 64] == 0).all()
 
 
 def test_grad_without_ids(ctx, torch):
@@ -434,6 +469,47 @@ def test_cache_counts_that_cannot_be(ctx, torch, n_free):
     assert int(dev.status[0]) == status and dev.state() == (model.length, model.held, model.table, model.free, model.n_free)
 
 
+def test_cache_slots_beyond_32_bits(ctx, torch):
+    """Slots of pages at the end of a pool of 2^42 tokens; one launch and two."""
+    page, n_pages = 4096, 2 ** 30
+    for n, cap in ((2, 8), (1100, 1100)):
+        length, held = [page - 1] + [0] * (n - 1), [1] + [0] * (n - 1)
+        table = [[n_pages - 1, -5]] + [[-5, -5]] * (n - 1)
+        free = torch.tensor([n_pages - 5, n_pages - 4, n_pages - 3, n_pages - 2], dtype=torch.int32, device="cuda")
+        off = [0, 2, 5] + [5] * (n - 2)
+        state = (length, held, table, [], 4, page, n_pages, 2)
+        dev = DeviceCache(torch, state)
+        dev.free = free
+        slots = torch.full((cap,), -7, dtype=torch.int64, device="cuda")
+        pos = torch.full((cap,), -7, dtype=torch.int32, device="cuda")
+        dev.slots(ctx, torch.tensor(off, dtype=torch.int64, device="cuda"), slots, pos, cap)
+        P = n_pages * page
+        assert slots[:6].tolist() == [P - 1, P - 2 * page, P - 3 * page, P - 3 * page + 1, P - 3 * page + 2, -7]
+        assert pos[:6].tolist() == [page - 1, page, 0, 1, 2, -7] and int(dev.n_free[0]) == 2 and int(dev.status[0]) == 0
+
+
+@pytest.mark.parametrize("n, most", [(3, 1300), (256, 4), (300, 13), (1024, 4), (1024, 5)])
+def test_cache_trims_of_many_pages(ctx, torch, n, most):
+    """Everything given back at once, in one launch and in two; the next step takes the pages again, the last ones first."""
+    pages = torch.randperm(n * most)
+    state = ([most * 2] * n, [most] * n, pages.view(n, most).tolist(), [-5] * (n * most), 0, 2, n * most, most)
+    dev = DeviceCache(torch, state)
+    keep = [0 if i % 3 else 3 for i in range(n)]
+    dev.trim(ctx, torch.tensor(keep, dtype=torch.int32, device="cuda"))
+    model = ref.Cache(*state)
+    assert model.trim(keep) == 0 == int(dev.status[0])
+    assert dev.state() == (model.length, model.held, model.table, model.free, model.n_free)
+    new = [5] * n
+    off = [0] + np.cumsum(new).tolist()
+    d = torch.full((off[-1],), -7, dtype=torch.int64, device="cuda")
+    p = torch.full((off[-1],), -7, dtype=torch.int32, device="cuda")
+    slots, pos = [-7] * off[-1], [-7] * off[-1]
+    dev.slots(ctx, torch.tensor(off, dtype=torch.int64, device="cuda"), d, p, off[-1])
+    assert model.slots(off, off[-1], slots, pos) == int(dev.status[0])
+    assert dev.state() == (model.length, model.held, model.table, model.free, model.n_free)
+    assert d.tolist() == slots and p.tolist() == pos
+
+
 def test_cache_without_requests(ctx, torch):
     dev = DeviceCache(torch, ([], [], [], [1, 2, 3, 4], 3, 8, 4, 2))
     z = torch.full((4,), -7, dtype=torch.int64, device="cuda")
@@ -559,6 +635,26 @@ def test_verify_offsets_that_cannot_be(ctx, torch):
     want, acc = _verify(ctx, torch, np.arange(8, dtype=np.int32), off, 8, 3, p, q, F32, vocab, [0.5] * 8, [0.5] * 6, vocab, vocab)
     assert acc.tolist() == [2, -1, 3, -1, -1, -1]
     assert (want[[1, 3, 4, 5]] == -1).all()
+
+
+def test_verify_offsets_beyond_32_bits(ctx, torch):
+    """Rows of probabilities so far apart that element offsets pass 2^32."""
+    vocab, stride = 16, 2 ** 30 + 7
+    target = torch.zeros(4 * stride + vocab, dtype=torch.float16, device="cuda")            # 8 GiB
+    q = torch.zeros(3 * stride + vocab, dtype=torch.float16, device="cuda")                 # 6 GiB
+    for r, v in enumerate((3, 5, 7, 9, 11)):
+        target[r * stride + v] = 1.0
+        if r < 4:
+            q[r * stride + v] = 1.0
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    off = torch.tensor([0, 4], dtype=torch.int64, device="cuda")
+    u, out, acc = torch.full((4,), 0.5, device="cuda"), i32([[-7] * 5]), i32([-7])
+    need = capi.verify_workspace(1, vocab)
+    work = torch.empty(need, dtype=torch.uint8, device="cuda")
+    for draft, want, k in (([3, 5, 7, 9], [3, 5, 7, 9, 11], 4), ([3, 5, 7, 8], [3, 5, 7, 9, -1], 3)):
+        ctx.verify_draft(i32(draft).data_ptr(), off.data_ptr(), 1, 4, 4, target.data_ptr(), F16, stride, q.data_ptr(), stride, vocab, u.data_ptr(),
+                         u.data_ptr(), out.data_ptr(), acc.data_ptr(), work.data_ptr(), need)
+        assert out.tolist() == [want] and int(acc[0]) == k
 
 
 def test_verify_draws_what_the_target_says(ctx, torch):
@@ -705,6 +801,22 @@ def test_two_threads(ctx, torch):
     for t in threads:
         t.join()
     assert not errors, errors
+
+
+def test_two_contexts_and_the_current_device(ctx, torch):
+    """Two contexts on one GPU take turns on one stream; the current device stays what it was."""
+    other = capi.Context(device=0)
+    try:
+        table = torch.randn(9, 24, device="cuda")
+        ids = torch.tensor([8, 0, 3], dtype=torch.int32, device="cuda")
+        mid, out = torch.zeros(3, 24, device="cuda"), torch.zeros(3, 24, device="cuda")
+        again = torch.tensor([2, 1, 0], dtype=torch.int32, device="cuda")
+        for _ in range(20):
+            ctx.embed(ids.data_ptr(), 3, table.data_ptr(), F32, 9, 24, 24, mid.data_ptr(), F32, 24)
+            other.embed(again.data_ptr(), 3, mid.data_ptr(), F32, 3, 24, 24, out.data_ptr(), F32, 24)
+        assert torch.equal(out, table[[3, 0, 8]]) and torch.cuda.current_device() == 0
+    finally:
+        other.close()
 
 
 def test_refusals_leave_the_context_usable(ctx, torch):

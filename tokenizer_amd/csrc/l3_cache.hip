@@ -9,6 +9,9 @@
 //          sums of the workgroups.  What a request was is copied to the workspace.
 //   apply  adds up the workgroups' sums, decides who is served, writes table, slots, positions and the new state.
 // A step that one workgroup has through in the time of a launch does both in one (cache_slots_one_kernel, cache_trim_one_kernel).
+// All of it is bound by latency: chains of dependent loads, and launches.  Measured, us a call among others: 256 requests of one
+// token 5.2 (one launch; 4.6 on the GPU), 2,048 prompts with a million tokens 12.9 (3.8 + 9.5 on the GPU; 12.6 MB written, 2.5 us at a
+// copy's rate), a trim of 256 or 2,048 requests 8.0 (3.4 + 3.0).
 #include "l3_token_kernels.h"
 
 #include "l3_dev.h"
@@ -268,7 +271,7 @@ __device__ __forceinline__ void pages_of_wave(bool served, u64 upto, uint32_t* m
 
 // The whole step in one workgroup: a thread for each request, and at most kOneTokens tokens.  What bounds it is
 // latency -- three dependent loads and two barriers -- so no more waves are started than the requests need.
-constexpr uint64_t kOneTokens = 4096;
+constexpr uint64_t kOneTokens = 4096;   // (a workgroup of 1,024 has them in four turns, which take less than a second launch)
 constexpr int kOneSmall = 256;
 
 template <int THREADS>
@@ -352,7 +355,8 @@ __global__ __launch_bounds__(kApplyThreads) void cache_trim_kernel(CacheArgs A, 
     for (int32_t j = lane_id(); j < r.delta; j += 64) to[j] = from[j];
 }
 
-// The whole call in one workgroup: a thread for each request, which hold kOnePages pages at the very most.
+// The whole call in one workgroup: a thread for each request, which hold kOnePages pages at the very most: 2.4 .. 2.9 us where few
+// pages go, as against 4.6 .. 5.5 in two launches, but 3 us more for every 4,096 pages, which two launches move in 0.3.
 constexpr uint64_t kOnePages = 4096;
 
 template <int THREADS>

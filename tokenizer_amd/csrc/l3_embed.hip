@@ -55,9 +55,15 @@ __device__ __forceinline__ void store_cols(T* row, Cols c, uint32_t dim, typenam
 
 // ---- lookup -------------------------------------------------------------------------------------------------------
 // A thread has PER times as many neighbouring columns as make 16 bytes of the output, all loads in flight before the first store.
-// What is divided is a workgroup's first vector (once) and 32-bit offsets from it.
+// What is divided is a workgroup's first vector (once) and 32-bit offsets from it.  Bound by memory: 16,384 rows of 4,096 in 16 bits
+// take 31 us (186 MB of distinct rows read and rows written: 6.0 TB/s; a copy of 1 GiB reaches 5.1), 64 rows a launch (2.5 us).
+//
+// Outputs of 16 MiB and more (kEmbedOnce) pass the caches: stored the usual way, the output drives the table's rows out of them
+// (44 us instead of 32 at the size above; 16,384 rows of 2,048 in 32 bits 46 and 32).  A smaller output stays in them for the
+// kernel that reads it next.  One vector a thread is best up to 2^24 vectors (16,384 x 4,096: 32 us, with four 35), four above
+// (65,536 x 4,096: 169 and 144).
 constexpr int kEmbedThreads = 256;
-constexpr uint64_t kEmbedOnce = 1u << 20, kEmbedMany = 1u << 24;   // vectors (launch_embed)
+constexpr uint64_t kEmbedOnce = 1u << 20, kEmbedMany = 1u << 24;   // vectors of 16 bytes
 
 template <class T, class O, int PER, bool ONCE, bool SMALL>
 __global__ __launch_bounds__(kEmbedThreads) void embed_kernel(const int32_t* __restrict__ ids, uint64_t n, const uint64_t* __restrict__ n_dev,
@@ -98,6 +104,8 @@ __global__ __launch_bounds__(kEmbedThreads) void embed_kernel(const int32_t* __r
 // count, has the key n_rows and ends up behind all others.  A tile of ids per workgroup:
 //   sort_count_kernel    how often each digit occurs in the tile
 //   sort_place_kernel    adds up the counts of the tiles before it, ranks the tile's ids and writes them to their places
+// Bound by latency: 4.9 and 7.9 us a pass for 65,536 ids, two passes for up to 2^18 - 1 rows.  (Adding the counts up in every workgroup
+// saves a launch for their scan; a look-back from tile to tile would need cleared flags.)
 constexpr int kSortWaves = kSortThreads / 64;
 static_assert(kSortThreads == 2 * kSortBins, "two threads a digit add up the tiles' counts");
 
@@ -196,7 +204,8 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const int32_t*
 // ---- gradient: ids ranked -----------------------------------------------------------------------------------------
 // Up to kRankIds ids in one launch: the place of position i is the number of positions j with key_j < key_i, or key_j = key_i and
 // j < i.  A workgroup has kRankMine positions and all keys in LDS; each of its 32 half waves counts over a part of them, four keys
-// a load.
+// a load.  Bound by the n^2 comparisons: 7 us for 5,003 ids.  Whole gradients of 64 .. 256 columns, ranked / sorted by digits (us):
+// 8,192 ids 20 / 28, 12,288 34 / 33, 16,384 40 / 33.
 constexpr uint32_t kRankMine = 32;
 
 __global__ __launch_bounds__(kSortThreads) void sort_rank_kernel(const int32_t* __restrict__ ids, uint32_t n, const uint64_t* __restrict__ n_dev, uint32_t rows,
@@ -247,11 +256,20 @@ __global__ __launch_bounds__(kSortThreads) void sort_rank_kernel(const int32_t* 
 // workspace: part[2 b] of the run that came in from the workgroup before, part[2 b + 1] of the run that starts here and goes
 // on; grad_join_kernel adds these up at the workgroup where the run starts.  Nothing is added by atomics: the same ids give the
 // same bits.
+//
+// Bound by memory: 65,536 ids onto 32-bit gradients of 128,256 x 4,096 read 0.81 GB and write 0.32 GB (counters: the distinct rows,
+// each once, and 4 % for the parts) in 250 us, 4.5 TB/s; a copy of 4 GiB reaches 4.7.  Rows in flight, us of the whole call: two 308,
+// four 279, eight 265; loading the next eight while these are added up gains nothing more (268).  Keys and positions in
+// registers instead of a load each, and no loads by element at the row's end: 346 -> 272 us.
 constexpr int kGradThreads = 64 * kGradWaves;
 constexpr int kGradGroup = 8;
 constexpr uint32_t kGradCols = 512;
-constexpr uint64_t kGradOnce = 256ull << 20;   // bytes of gradient (launch_embed_grad)
-constexpr uint32_t kZeroRows = 32;   // rows a workgroup looks after when the gradient is written whole
+// A gradient above the last cache's 256 MiB is loaded past the caches (65,536 x 4,096 in 16 bits: 288 us instead of 313); a smaller one
+// may still be in them from the kernel that made it (8,192 x 4,096: 55 instead of 48 us if it is loaded past them).
+constexpr uint64_t kGradOnce = 256ull << 20;
+// Rows a workgroup looks after when the gradient is written whole.  128,256 rows of 4,096 in 32 bits / of 64 in 16 bits, us: 8 rows
+// 397 / 36, 16 rows 401 / 28, 32 rows 409 / 25, 64 rows 415 / 24.
+constexpr uint32_t kZeroRows = 32;
 
 // Rows [r0, r0 + kZeroRows) of which `named` has no mark become zero; by a whole workgroup.  16 bytes a lane, the last ones of a row
 // overlapping those before.
@@ -380,7 +398,9 @@ __global__ __launch_bounds__(kGradThreads) void grad_walk_kernel(GradWalk P, con
     if (w == 0 && starts && came_in != ~0u && mine) store8(part + (2 * block) * P.dim8 + vec * 8, head);
 }
 
-// Parts of long runs: a workgroup per walking workgroup and 512 columns, every wave a share of the parts, eight loads in flight.
+// Parts of long runs: a workgroup per walking workgroup and 512 columns, every wave a share of the parts, eight loads in flight.  Most
+// workgroups find no run to join and leave after one load; 65,536 ids of which 6 % are the same: 7.5 us (26 us with one wave for
+// all parts of a run and parts of single waves).
 constexpr int kJoinGroup = 8;
 
 template <class T, bool SMALL>
@@ -430,7 +450,8 @@ __global__ __launch_bounds__(kGradThreads) void grad_join_kernel(GradWalk P, con
 // ---- gradient: few ids --------------------------------------------------------------------------------------------
 // One launch, nothing sorted.  A workgroup per position and 512 columns: it compares all ids with its own, leaves if one before it
 // is the same, and else adds up the rows of those that are, every wave a quarter of them.  Its own row and the table's are on
-// their way while it compares.
+// their way while it compares.  Bound by the chain ids -> rows -> store: 7 us for 512 ids of 2,048 columns, 6.5 us a call among others
+// (sorted: 16 us).
 constexpr int kDirectWords = (int)(kDirectIds / 64), kDirectGroup = 8;
 
 template <class G, class T, bool SMALL>

@@ -69,11 +69,13 @@ constexpr uint64_t align256(uint64_t b) { return (b + 255) & ~255ull; }
 constexpr int kSortThreads = 1024, kSortBits = 9, kSortBins = 1 << kSortBits;
 inline int sort_rounds(uint64_t n) { return n <= 65536 ? 1 : n <= 262144 ? 2 : 4; }
 inline uint64_t sort_tiles(uint64_t n) { const uint64_t t = (uint64_t)kSortThreads * sort_rounds(n); return (n + t - 1) / t; }
-// Few ids are not sorted: every position looks for the others of its id by itself, a workgroup for each and 512 columns.  Up to
-// kRankIds ids are sorted in one launch by counting, more digit by digit.
+// Few ids are not sorted: every position looks for the others of its id by itself, a workgroup for each and 512 columns (kDirectBlocks
+// of them fit the GPU twice; 2,048 ids of 1,024 columns take 10 us so, 16 sorted).  Up to kRankIds ids are sorted in one launch by
+// counting, more digit by digit (l3_embed.hip has the times of both).
 constexpr uint64_t kDirectIds = 2048, kDirectBlocks = 4096, kRankIds = 8192;
 inline bool grad_direct(uint64_t n, uint64_t dim) { return n <= kDirectIds && n * ((dim + 511) / 512) <= kDirectBlocks; }
-// Sorted positions one wave adds up: few enough that there are about kGradWalkers waves, and 8 .. 64.
+// Sorted positions one wave adds up: few enough that there are about kGradWalkers waves, and 8 .. 64.  By kGradWalkers = 8,192 /
+// 4,096 / 2,048 / 1,024, us: 16,384 ids of 2,048 columns 72 / 60 / 56 / 60, 65,536 of 1,024 98 / 86 / 84 / 84 (more waves leave more parts).
 constexpr uint64_t kGradWalkers = 2048;
 constexpr int kGradWaves = 4;        // waves of a workgroup
 inline uint32_t grad_chunk(uint64_t n, uint64_t dim) {
@@ -155,10 +157,10 @@ inline const char* check_embed_grad(const EmbedGradArgs& A) {
         return "a row stride is smaller than dim or above 2^31 - 1";
     if (A.accumulate != 0 && A.accumulate != 1) return "accumulate must be 0 or 1";
     if (!A.table) return "null pointer argument";
-    if (misaligned(A.table, dtype_size(A.table_dtype))) return "a pointer is not aligned to its element";
+    if (misaligned(A.table, dtype_size(A.table_dtype)) || misaligned(A.n_dev, 8)) return "a pointer is not aligned to its element";
     if (A.n == 0) return nullptr;
     if (!A.ids || !A.grad || !A.work) return "null pointer argument";
-    if (misaligned(A.ids, 4) || misaligned(A.n_dev, 8) || misaligned(A.grad, dtype_size(A.dtype))) return "a pointer is not aligned to its element";
+    if (misaligned(A.ids, 4) || misaligned(A.grad, dtype_size(A.dtype))) return "a pointer is not aligned to its element";
     if (misaligned(A.work, 16)) return "the workspace must be aligned to 16 bytes";
     if (A.work_bytes < grad_work(A.n, A.dim).total) return "workspace too small (l3_embed_grad_workspace)";
     return nullptr;
