@@ -215,6 +215,30 @@ def test_grad_where_the_sort_changes(ctx, torch, n):
     _grad_case(ctx, torch, rng, _ids(rng, n, 3000), 16, BF16, F32, 3000, True, n_dev=n - 5)
 
 
+@pytest.mark.parametrize("n, rows", [(3000, 11999), (3000, 12000), (8500, 33999), (8500, 34000)])
+@pytest.mark.parametrize("dim, T", [(1, F16), (1, F32), (5, F16), (7, BF16), (8, F16), (9, F32), (40, BF16)])
+def test_grad_whole_names_few_rows(ctx, torch, n, rows, dim, T):
+    """Most rows are zeros; rows of two bytes and more, on any alignment."""
+    rng = np.random.default_rng(n + dim)
+    _grad_case(ctx, torch, rng, _ids(rng, n, rows), dim, BF16, T, rows, False, 0.5, dim + 2, dim + 3, 1)
+
+
+@pytest.mark.parametrize("n", [300, 5000, 9000])
+def test_grad_of_the_most_rows(ctx, torch, n):
+    """2^28 rows: keys of four digits."""
+    rows = 2 ** 28
+    table = torch.ones(rows, dtype=torch.float16, device="cuda")
+    ids = torch.randint(0, rows, (n,), dtype=torch.int32, device="cuda")
+    ids[:3] = torch.tensor([0, rows - 1, rows - 1], dtype=torch.int32)
+    g = torch.randint(-4, 5, (n, 1), device="cuda").half()
+    need = capi.embed_grad_workspace(n, 1)
+    work = torch.empty(need, dtype=torch.uint8, device="cuda")
+    want = torch.zeros(rows, device="cuda").index_add_(0, ids.long(), g[:, 0].float())
+    for accumulate in (False, True):
+        ctx.embed_grad(ids.data_ptr(), n, g.data_ptr(), F16, 1, rows, 1, table.data_ptr(), F16, 1, work.data_ptr(), need, 1.0, accumulate)
+        assert torch.equal(table, (want * (2 if accumulate else 1)).half())
+
+
 @pytest.mark.parametrize("n, dim", [(2048, 520), (600, 4096), (257, 8200)])
 def test_grad_few_ids_wide_rows(ctx, torch, n, dim):
     """Few ids, one of them in half of the positions: with and without a sort (the number of workgroups decides)."""
@@ -467,6 +491,33 @@ def test_cache_counts_that_cannot_be(ctx, torch, n_free):
     status = model.trim([0, 0])
     dev.trim(ctx, torch.zeros(2, dtype=torch.int32, device="cuda"))
     assert int(dev.status[0]) == status and dev.state() == (model.length, model.held, model.table, model.free, model.n_free)
+
+
+@pytest.mark.parametrize("n_free", [2 ** 20, 700001, 1024 * 600, 5, 0])
+def test_cache_of_the_most_requests(ctx, torch, n_free):
+    """2^20 requests of one new token each, on a pool that may run short; then every page back."""
+    n, page = 2 ** 20, 16
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    free = torch.arange(n, dtype=torch.int32, device="cuda")
+    table, length, held, status = torch.full((n, 1), -5, dtype=torch.int32, device="cuda"), i32(n), i32(n), i32(1)
+    left = torch.tensor([n_free], dtype=torch.int32, device="cuda")
+    off = torch.arange(n + 1, dtype=torch.int64, device="cuda")
+    slots, pos = torch.full((n,), -7, dtype=torch.int64, device="cuda"), torch.full((n,), -7, dtype=torch.int32, device="cuda")
+    need = capi.cache_workspace(n)
+    work = torch.empty(need, dtype=torch.uint8, device="cuda")
+    p = lambda *a: [x.data_ptr() for x in a]  # noqa: E731
+    ctx.cache_slots(off.data_ptr(), n, *p(length, held), page, n, table.data_ptr(), 1, 1, *p(free, left, length, held, left, slots, pos), n, status.data_ptr(),
+                    work.data_ptr(), need)
+    i = torch.arange(n, device="cuda")
+    served = i < n_free
+    assert torch.equal(slots, torch.where(served, (n_free - 1 - i) * page, torch.full_like(i, -1)))
+    assert torch.equal(pos, torch.where(served, 0, -1).int()) and torch.equal(held, served.int()) and torch.equal(length, served.int())
+    assert int(left[0]) == 0 and int(status[0]) == (0 if n_free == n else ref.POOL)
+    assert torch.equal(table[:n_free, 0], (n_free - 1 - i[:n_free]).int()) and (table[n_free:] == -5).all()
+    ctx.cache_trim(i32(n).data_ptr(), n, *p(length, held), page, n, table.data_ptr(), 1, 1, *p(free, left, length, held, left), status.data_ptr(),
+                   work.data_ptr(), need)
+    assert int(left[0]) == n_free and int(status[0]) == 0 and not held.any() and not length.any()
+    assert torch.equal(free[:n_free], (n_free - 1 - i[:n_free]).int())
 
 
 def test_cache_slots_beyond_32_bits(ctx, torch):
