@@ -539,7 +539,7 @@ def test_cache_slots_beyond_32_bits(ctx, torch):
         assert pos[:6].tolist() == [page - 1, page, 0, 1, 2, -7] and int(dev.n_free[0]) == 2 and int(dev.status[0]) == 0
 
 
-@pytest.mark.parametrize("n, most", [(3, 1300), (256, 4), (300, 13), (1024, 4), (1024, 5)])
+@pytest.mark.parametrize("n, most", [(3, 1300), (256, 4), (257, 4), (300, 13), (1024, 4), (1024, 128), (1024, 129), (1025, 5)])
 def test_cache_trims_of_many_pages(ctx, torch, n, most):
     """Everything given back at once, in one launch and in two; the next step takes the pages again, the last ones first."""
     pages = torch.randperm(n * most)

@@ -11,7 +11,7 @@
 // A step that one workgroup has through in the time of a launch does both in one (cache_slots_one_kernel, cache_trim_one_kernel).
 // All of it is bound by latency: chains of dependent loads, and launches.  Measured, us a call among others: 256 requests of one
 // token 5.2 (one launch; 4.6 on the GPU), 2,048 prompts with a million tokens 12.9 (3.8 + 9.5 on the GPU; 12.6 MB written, 2.5 us at a
-// copy's rate), a trim of 256 or 2,048 requests 8.0 (3.4 + 3.0).
+// copy's rate), a trim of 256 requests after drafts 5.1 (3.4 on the GPU), of 2,048 requests 8.1 (4.0 + 3.1).
 #include "l3_token_kernels.h"
 
 #include "l3_dev.h"
@@ -355,26 +355,29 @@ __global__ __launch_bounds__(kApplyThreads) void cache_trim_kernel(CacheArgs A, 
     for (int32_t j = lane_id(); j < r.delta; j += 64) to[j] = from[j];
 }
 
-// The whole call in one workgroup: a thread for each request, which hold kOnePages pages at the very most: 2.4 .. 2.9 us where few
-// pages go, as against 4.6 .. 5.5 in two launches, but 3 us more for every 4,096 pages, which two launches move in 0.3.
-constexpr uint64_t kOnePages = 4096;
+// The whole call in one workgroup: a thread for each request, which moves the first pages the request gives back itself -- after
+// drafts that were not accepted there are no more --, then sixteen lanes for each request that gives more, eight pages each in flight.
+// In one workgroup / in two launches, us on the GPU (and 4 us less for the caller, who makes one launch): 256 requests that give
+// nothing 2.8 / 4.8, of which a tenth gives 512 pages 5.4 / 5.8, of which all do 16.8 / 5.8; 1,024 requests 3.0 / 5.6, a tenth 8.9 / 6.5,
+// all 58 / 6.8.  A step after drafts is the first of these and a batch that ends at once is rare, so the limit is where that
+// costs 11 us.
+constexpr uint64_t kOnePages = 131072, kOnePagesSmall = 1024;   // pages that the requests hold at the very most
+constexpr int32_t kFirstPages = 2, kPageLanes = 16;
 
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void cache_trim_one_kernel(CacheArgs A) {
     __shared__ u64 tmp[THREADS / 64];
-    __shared__ uint32_t s_before[THREADS], s_status, s_given;
-    __shared__ int32_t s_first[THREADS];
+    __shared__ uint32_t s_before[THREADS], s_many[THREADS], s_status, s_given, s_n_many;
+    __shared__ int32_t s_first[THREADS], s_delta[THREADS];
     const uint64_t i = threadIdx.x;
     const int32_t n_free = *A.n_free;
     const bool bad = n_free < 0 || (uint32_t)n_free > A.n_pages;
     const u64 left = bad ? A.n_pages : (u64)n_free;
-    if (threadIdx.x == 0) { s_status = bad ? (uint32_t)kCacheBad : 0u; s_given = 0; }
+    if (threadIdx.x == 0) { s_status = bad ? (uint32_t)kCacheBad : 0u; s_given = 0; s_n_many = 0; }
     PlanRec r{};
     if (i < A.n) r = plan_trim(A.len[i], A.held[i], A.keep[i], A.page, A.max_pages);
     u64 all;
     const u64 before = block_escan64<THREADS>((u64)r.delta, tmp, &all);   // (at most kOnePages pages)
-    s_before[i] = (uint32_t)before;
-    s_first[i] = r.held - r.delta;
     bool gives = false;
     if (i < A.n) {
         const bool served = trim_served(r, before, left, A.n_pages);
@@ -384,20 +387,44 @@ __global__ __launch_bounds__(THREADS) void cache_trim_one_kernel(CacheArgs A) {
         if (!served) atomicOr(&s_status, r.flags ? r.flags : (uint32_t)kCachePool);
     }
     pages_of_wave(gives, before + (u64)r.delta, &s_given);
-    __syncthreads();
-    const uint32_t given = s_given;
-    for (uint32_t g = threadIdx.x; g < given; g += 4 * THREADS) {
-        int32_t page[4];
+    const int32_t stay = r.held - r.delta;
+    if (gives) {
+        const int32_t* from = A.table + i * A.table_stride + stay;
+        int32_t* to = A.free_pages + left + before;
+        int32_t page[kFirstPages];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const uint32_t x = g + j * THREADS < given ? g + j * THREADS : g, k = request_of_page(s_before, (uint32_t)A.n, x);
-            page[j] = A.table[k * A.table_stride + (uint32_t)s_first[k] + (x - s_before[k])];
+        for (int32_t j = 0; j < kFirstPages; j++) page[j] = from[j < r.delta ? j : 0];
+#pragma unroll
+        for (int32_t j = 0; j < kFirstPages; j++) if (j < r.delta) to[j] = page[j];
+    }
+    const bool many = gives && r.delta > kFirstPages;
+    const u64 m = __ballot(many);
+    if (m) {
+        uint32_t at = 0;
+        if (lane_id() == 0) at = atomicAdd(&s_n_many, (uint32_t)__popcll(m));
+        at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + (uint32_t)__popcll(m & ((1ull << lane_id()) - 1));
+        if (many) {
+            s_many[at] = (uint32_t)i;
+            s_before[at] = (uint32_t)before + kFirstPages;
+            s_first[at] = stay + kFirstPages;
+            s_delta[at] = r.delta - kFirstPages;
         }
+    }
+    __syncthreads();
+    for (uint32_t x = threadIdx.x / kPageLanes; x < s_n_many; x += THREADS / kPageLanes) {
+        const int32_t* from = A.table + (uint64_t)s_many[x] * A.table_stride + s_first[x];
+        int32_t* to = A.free_pages + left + s_before[x];
+        const int32_t n = s_delta[x];
+        for (int32_t j0 = threadIdx.x % kPageLanes; j0 < n; j0 += 8 * kPageLanes) {
+            int32_t page[8];
 #pragma unroll
-        for (int j = 0; j < 4; j++) if (g + j * THREADS < given) A.free_pages[left + g + j * THREADS] = page[j];
+            for (int k = 0; k < 8; k++) page[k] = from[j0 + kPageLanes * k < n ? j0 + kPageLanes * k : j0];
+#pragma unroll
+            for (int k = 0; k < 8; k++) if (j0 + kPageLanes * k < n) to[j0 + kPageLanes * k] = page[k];
+        }
     }
     if (threadIdx.x == 0) {
-        *A.n_free_out = bad ? n_free : n_free + (int32_t)given;
+        *A.n_free_out = bad ? n_free : n_free + (int32_t)s_given;
         *A.status = s_status;
     }
 }
@@ -423,7 +450,7 @@ hipError_t launch_cache_slots(const CacheArgs& A, hipStream_t stream) {
 }
 
 hipError_t launch_cache_trim(const CacheArgs& A, hipStream_t stream) {
-    if (A.n <= kOneSmall && A.n * A.max_pages <= kOnePages / 4) return launch(cache_trim_one_kernel<kOneSmall>, 1, kOneSmall, stream, A);
+    if (A.n <= kOneSmall && A.n * A.max_pages <= kOnePagesSmall) return launch(cache_trim_one_kernel<kOneSmall>, 1, kOneSmall, stream, A);
     if (A.n <= kPlanThreads && A.n * A.max_pages <= kOnePages) return launch(cache_trim_one_kernel<kPlanThreads>, 1, kPlanThreads, stream, A);
     const Parts P = parts_of(A);
     hipError_t e = launch(cache_plan_kernel<true>, P.plan_blocks, kPlanThreads, stream, A, P.recs, P.blocks, P.head);

@@ -18,10 +18,11 @@ namespace {
 // A launch whose error is its own: hipGetLastError would hand out (and clear) what another library's call left behind.
 template <class... P>
 hipError_t launch(void (*kernel)(P...), uint64_t blocks, uint32_t threads, hipStream_t stream, P... args) {
+    if (blocks * threads >= 1ull << 32) return hipErrorInvalidConfiguration;   // (the runtime cuts such a grid short without a word)
     void* a[] = {(void*)&args...};
     return hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3((uint32_t)blocks), dim3(threads), a, 0, stream);
 }
-// A grid has at most 2^32 - 1 work-items; every kernel here walks its work with the grid's stride, so a cap costs nothing.
+// For kernels that walk their work with the grid's stride.
 constexpr uint64_t kMaxBlocks = 1u << 21;
 inline uint64_t capped(uint64_t blocks) { return blocks < kMaxBlocks ? blocks : kMaxBlocks; }
 
