@@ -239,9 +239,28 @@ def test_grad_of_the_most_rows(ctx, torch, n):
         assert torch.equal(table, (want * (2 if accumulate else 1)).half())
 
 
-@pytest.mark.parametrize("n, dim", [(2048, 520), (600, 4096), (257, 8200)])
-def test_grad_few_ids_wide_rows(ctx, torch, n, dim):
-    """Few ids, one of them in half of the positions: with and without a sort (the number of workgroups decides)."""
+@pytest.mark.parametrize("n, dim, G", [(34000, 4001, BF16), (17000, 4097, F32), (33000, 4100, F16)])
+def test_grad_larger_than_the_last_cache(ctx, torch, n, dim, G):
+    """Gradients that are loaded past the caches; whole numbers, so that torch's own sums are exact."""
+    rows = 900
+    g = torch.randint(-8, 9, (n, dim), device="cuda").to(_t(torch, G))
+    assert g.numel() * g.element_size() > 256 << 20
+    ids = torch.randint(-1, rows + 1, (n,), device="cuda", dtype=torch.int32)
+    ids[torch.rand(n, device="cuda") < 0.2] = 5
+    there = ((ids >= 0) & (ids < rows)).float()[:, None]
+    want = torch.zeros(rows, dim, device="cuda").index_add_(0, ids.clamp(0, rows - 1).long(), g.float() * there)
+    table = torch.ones(rows, dim, device="cuda")
+    need = capi.embed_grad_workspace(n, dim)
+    work = torch.empty(need, dtype=torch.uint8, device="cuda")
+    ctx.embed_grad(ids.data_ptr(), n, g.data_ptr(), G, dim, rows, dim, table.data_ptr(), F32, dim, work.data_ptr(), need, 1.0, True)
+    assert torch.equal(table, want + 1)
+    ctx.embed_grad(ids.data_ptr(), n, g.data_ptr(), G, dim, rows, dim, table.data_ptr(), F32, dim, work.data_ptr(), need, 1.0, False)
+    assert torch.equal(table, want)
+
+
+@pytest.mark.parametrize("n, dim", [(2048, 520), (600, 4096), (257, 8200), (1000, 4090), (3000, 1100), (9000, 1030)])
+def test_grad_one_id_in_half_of_the_positions(ctx, torch, n, dim):
+    """With and without a sort, over several tiles of columns."""
     rng = np.random.default_rng(dim)
     ids = _ids(rng, n, 50)
     ids[rng.random(n) < 0.5] = 7
