@@ -208,7 +208,7 @@ def test_grad_numbers_of_digits(ctx, torch, rows, n):
     _grad_case(ctx, torch, rng, ids, 8, F32, F32, rows, True)
 
 
-@pytest.mark.parametrize("n", [2047, 2048, 2049, 8191, 8192, 8193, 65536, 65537, 262144, 262145, 300001])
+@pytest.mark.parametrize("n", [511, 512, 513, 1023, 1024, 1025, 2047, 2048, 2049, 4095, 4096, 4097, 8191, 8192, 8193, 65536, 65537, 262144, 262145, 300001])
 def test_grad_where_the_sort_changes(ctx, torch, n):
     """Every way of bringing equal ids together, next to the sizes at which another begins."""
     rng = np.random.default_rng(n)

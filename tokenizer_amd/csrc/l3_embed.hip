@@ -450,17 +450,18 @@ __global__ __launch_bounds__(kGradThreads) void grad_join_kernel(GradWalk P, con
 // ---- gradient: few ids --------------------------------------------------------------------------------------------
 // One launch, nothing sorted.  A workgroup per position and 512 columns: it compares all ids with its own, leaves if one before it
 // is the same, and else adds up the rows of those that are, every wave a quarter of them.  Its own row and the table's are on
-// their way while it compares.  Bound by the chain ids -> rows -> store: 7 us for 512 ids of 2,048 columns, 6.5 us a call among others
-// (sorted: 16 us).
-constexpr int kDirectWords = (int)(kDirectIds / 64), kDirectGroup = 8;
+// their way while it compares.  Bound by the chain ids -> rows -> store: 5.4 us for 512 ids of 2,048 columns, 5.0 a call among others
+// (sorted: 16 us).  WORDS * 64 ids are compared whatever n is, so there is a kernel each for 512, 1,024, 2,048 and 4,096 of them: 512
+// ids of 2,048 columns take 6.7 us in the one for 2,048.
+constexpr int kDirectGroup = 8;
 
-template <class G, class T, bool SMALL>
+template <class G, class T, bool SMALL, int WORDS>
 __global__ __launch_bounds__(kGradThreads) void grad_direct_kernel(const int32_t* __restrict__ ids, uint32_t n, const uint64_t* n_dev, uint32_t rows,
                                                                    const G* __restrict__ grad, uint64_t grad_stride, uint32_t dim,
                                                                    T* __restrict__ table, uint64_t table_stride, float scale, int accumulate,
                                                                    uint32_t tiles) {
-    __shared__ u64 words[kDirectWords];
-    __shared__ uint32_t list[kDirectIds];
+    __shared__ u64 words[WORDS];
+    __shared__ uint32_t list[WORDS * 64];
     __shared__ F8 acc[kGradWaves - 1][64];
     const uint32_t valid = (uint32_t)ids_that_count(n, n_dev);
     const int w = __builtin_amdgcn_readfirstlane((int)wave_id()), lane = lane_id();
@@ -478,9 +479,9 @@ __global__ __launch_bounds__(kGradThreads) void grad_direct_kernel(const int32_t
     }
     const uint32_t t = blockIdx.x / tiles;
     if (t >= valid) return;
-    int32_t other[kDirectWords / kGradWaves];
+    int32_t other[WORDS / kGradWaves];
 #pragma unroll
-    for (int y = 0; y < kDirectWords / kGradWaves; y++) {
+    for (int y = 0; y < WORDS / kGradWaves; y++) {
         const uint32_t j = (uint32_t)(y * kGradWaves + w) * 64 + lane;
         other[y] = ids[j < valid ? j : 0];
     }
@@ -498,7 +499,7 @@ __global__ __launch_bounds__(kGradThreads) void grad_direct_kernel(const int32_t
     }
     bool earlier = false;
 #pragma unroll
-    for (int y = 0; y < kDirectWords / kGradWaves; y++) {
+    for (int y = 0; y < WORDS / kGradWaves; y++) {
         const int x = y * kGradWaves + w;
         const uint32_t j = (uint32_t)x * 64 + lane;
         const u64 m = __ballot(j < valid && j != t && other[y] == id);
@@ -507,11 +508,11 @@ __global__ __launch_bounds__(kGradThreads) void grad_direct_kernel(const int32_t
     }
     if (__syncthreads_or(earlier)) return;
     // the others, in order: every wave knows how many there are in the words before its own
-    static_assert(kDirectWords <= 64, "a lane a word");
-    const u64 mine_word = lane < kDirectWords ? words[lane] : 0;
+    static_assert(WORDS <= 64, "a lane a word");
+    const u64 mine_word = lane < WORDS ? words[lane] : 0;
     const uint32_t upto = wave_iscan((uint32_t)__popcll(mine_word)), count = of_lane(upto, 63);
     if (count) {
-        for (int x = w; x < kDirectWords; x += kGradWaves) {
+        for (int x = w; x < WORDS; x += kGradWaves) {
             const u64 m = words[x];
             if ((m >> lane) & 1) list[of_lane(upto, x) - (uint32_t)__popcll(m) + (uint32_t)__popcll(m & ((1ull << lane) - 1))] = (uint32_t)x * 64 + lane;
         }
@@ -577,8 +578,12 @@ hipError_t launch_embed_grad(const EmbedGradArgs& A, hipStream_t stream) {
         return with_types([&](auto g, auto t, auto small) {
             typedef decltype(g) G;
             typedef decltype(t) T;
-            return launch(grad_direct_kernel<G, T, small.value>, A.n * col_tiles + zero_blocks, kGradThreads, stream, A.ids, (uint32_t)A.n, A.n_dev, rows, (const G*)A.grad,
-                          A.grad_stride, dim, (T*)A.table, A.table_stride, A.scale, A.accumulate, col_tiles);
+            auto* kernel = A.n <= 512    ? grad_direct_kernel<G, T, small.value, 8>
+                           : A.n <= 1024 ? grad_direct_kernel<G, T, small.value, 16>
+                           : A.n <= 2048 ? grad_direct_kernel<G, T, small.value, 32>
+                                         : grad_direct_kernel<G, T, small.value, (int)(kDirectIds / 64)>;
+            return launch(kernel, A.n * col_tiles + zero_blocks, kGradThreads, stream, A.ids, (uint32_t)A.n, A.n_dev, rows, (const G*)A.grad, A.grad_stride, dim,
+                          (T*)A.table, A.table_stride, A.scale, A.accumulate, col_tiles);
         });
     }
     const GradWork W = grad_work(A.n, A.dim);
