@@ -200,7 +200,8 @@ int l3_embed_grad(l3_ctx* ctx, const int32_t* d_ids, uint64_t n_ids, const uint6
  *   L3_CACHE_POOL  the pool ran short: no page is left for this request or, where pages are needed, any behind it (trim: the
  *                  pool would hold more than n_pages)
  *   L3_CACHE_ROW   more tokens than max_pages pages, or 2^31 - 1, hold
- *   L3_CACHE_BAD   new_off descends or ends behind cap; len, held or *n_free is negative, or more than there can be
+ *   L3_CACHE_BAD   new_off descends or ends behind cap; len, held or *n_free is negative, or more than there can be (where new_off
+ *                  descends, the table entries of requests that claim the same tokens are not to be relied on)
  *   L3_CACHE_PAGE  (slots) a page outside [0, n_pages): the slots of the tokens on it are -1, nothing else changes
  * d_work: l3_cache_workspace(n_seqs) bytes.  n_seqs <= 2^20. */
 #define L3_CACHE_POOL 1u

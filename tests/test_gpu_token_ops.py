@@ -512,6 +512,53 @@ def test_cache_counts_that_cannot_be(ctx, torch, n_free):
     assert int(dev.status[0]) == status and dev.state() == (model.length, model.held, model.table, model.free, model.n_free)
 
 
+@pytest.mark.parametrize("n, every, most", [(20000, 1, 500), (3, 1, 2000000), (2 ** 20, 1, 9), (2 ** 20, 1000, 8500), (16384, 1, 600), (16383, 1, 600)])
+def test_cache_of_millions_of_tokens(ctx, torch, n, every, most):
+    """Four million tokens and more, of few long requests and of many short ones, some under way, some without a new token."""
+    rng = np.random.default_rng(n + every)
+    page = 16
+    new = np.where(np.arange(n) % every == 0, rng.integers(most // 2, most + 1, n), 0)
+    old = np.where(np.arange(n) % 3 == 0, rng.integers(0, 3 * page, n), 0)
+    assert new.sum() >= 2 ** 22
+    held = -(-old // page)
+    need = -(-(old + new) // page) - held
+    wide = int((held + need).max())
+    n_pages = int(held.sum() + need.sum())
+    left = int(need.sum()) - int(need[-1]) if n == 20000 else int(need.sum())      # one page short for the last request
+    d = lambda a, t: torch.from_numpy(np.ascontiguousarray(a)).to("cuda", t)  # noqa: E731
+    off = np.append(0, np.cumsum(new))
+    total = int(off[-1])
+    table = torch.full((n, wide), -5, dtype=torch.int32, device="cuda")
+    first = d(np.cumsum(held) - held, torch.int64)[:, None]
+    j = torch.arange(min(wide, 3), device="cuda")
+    table[:, :len(j)] = torch.where(j < d(held, torch.int64)[:, None], (first + j).int(), table[:, :len(j)])
+    free = torch.arange(int(held.sum()), n_pages, dtype=torch.int32, device="cuda").flip(0).contiguous()[:max(left, 1)].contiguous()
+    L, H, N, S = d(old, torch.int32), d(held, torch.int32), d([left], torch.int32), d([77], torch.int32)
+    cap = total + 3
+    slots, pos = torch.full((cap,), -7, dtype=torch.int64, device="cuda"), torch.full((cap,), -7, dtype=torch.int32, device="cuda")
+    room = capi.cache_workspace(n)
+    work = torch.empty(room, dtype=torch.uint8, device="cuda")
+    d_off = d(off, torch.int64)
+    ctx.cache_slots(d_off.data_ptr(), n, L.data_ptr(), H.data_ptr(), page, n_pages, table.data_ptr(), wide, wide, free.data_ptr(), N.data_ptr(), L.data_ptr(),
+                    H.data_ptr(), N.data_ptr(), slots.data_ptr(), pos.data_ptr(), cap, S.data_ptr(), work.data_ptr(), room)
+    served = np.cumsum(need) <= left
+    served |= need == 0
+    assert int(S[0]) == (0 if served.all() else ref.POOL) and int(N[0]) == left - int(need[served].sum())
+    assert torch.equal(L, d(np.where(served, old + new, old), torch.int32)) and torch.equal(H, d(np.where(served, held + need, held), torch.int32))
+    seq = torch.repeat_interleave(torch.arange(n, device="cuda"), d(new, torch.int64))
+    t = torch.arange(total, device="cuda")
+    ok = d(served, torch.bool)[seq]
+    p = d(old, torch.int64)[seq] + t - d_off[seq]
+    fresh = p // page - d(held, torch.int64)[seq]
+    taken = left - 1 - (d(np.cumsum(need) - need, torch.int64)[seq] + fresh)
+    page_of = torch.where(fresh < 0, first[seq, 0] + p // page, free[taken.clamp(0, len(free) - 1)].long())
+    assert torch.equal(slots[:total], torch.where(ok, page_of * page + p % page, torch.full_like(p, -1)))
+    assert torch.equal(pos[:total], torch.where(ok, p, torch.full_like(p, -1)).int())
+    assert (slots[total:] == -7).all() and (pos[total:] == -7).all()
+    entry = ok & (p % page == 0) & (fresh >= 0)
+    assert torch.equal(table[seq[entry], (p // page)[entry]].long(), page_of[entry])
+
+
 @pytest.mark.parametrize("n_free", [2 ** 20, 700001, 1024 * 600, 5, 0])
 def test_cache_of_the_most_requests(ctx, torch, n_free):
     """2^20 requests of one new token each, on a pool that may run short; then every page back."""

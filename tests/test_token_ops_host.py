@@ -215,6 +215,18 @@ def test_cache_arithmetic(lib, seed):
     assert got[:5] == (model.length, model.held, model.table, model.free, model.n_free) and got[7] == status
 
 
+def test_division_by_the_page_size(lib):
+    """The product that stands for x / page, next to multiples of every page size up to 600 and of others up to 2^20."""
+    lib.l3t_page_div.restype, lib.l3t_page_div.argtypes = _U, [_U, _U]
+    rng = random.Random(1)
+    for page in [*range(1, 600), 1023, 1024, 1025, 65535, 65536, 65537, (1 << 20) - 1, 1 << 20] + [rng.randint(600, 1 << 20) for _ in range(200)]:
+        top = (2 ** 31 - 1) // page
+        for k in {0, 1, 2, top // 3, top - 1, top, rng.randint(0, top)}:
+            for x in (k * page - 1, k * page, k * page + 1, 2 ** 31 - 1):
+                if 0 <= x < 2 ** 31:
+                    assert lib.l3t_page_div(x, page) == x // page, (x, page)
+
+
 def test_positions_end_at_31_bits(lib):
     """A request that would pass 2^31 - 1 tokens is not served, whatever max_pages allows."""
     page, max_pages = 1 << 20, 4096

@@ -132,41 +132,79 @@ __device__ __forceinline__ uint64_t request_of(const uint64_t* off, uint64_t n, 
     }
 }
 
-// What a token needs of its request.
+constexpr int32_t kFirstPages = 2, kPageLanes = 16, kGroupPages = 512;
+
+// What a token needs of its request (tokens and pages are below 2^31; an offset that is not is the largest number instead).
 struct Owner {
-    uint64_t first, end;     // its new tokens
-    u64 next;                // free list: its first new page is at next - 1
+    uint32_t first, end;     // its new tokens
+    uint32_t next;           // free list: its first new page is at next - 1
     int32_t len, held;       // held < 0: not served
 };
-__device__ __forceinline__ Owner owner_of(const CacheArgs& A, const PlanRec& r, uint64_t first, uint64_t end, u64 before, u64 left) {
+__device__ __forceinline__ Owner owner_of(const PlanRec& r, uint64_t first, uint64_t end, u64 before, u64 left) {
+    const bool served = slots_served(r, before, left);
     Owner w;
-    w.first = first; w.end = end; w.next = left - before; w.len = r.len;
-    w.held = slots_served(r, before, left) ? r.held : -1;
+    w.first = first < ~0u ? (uint32_t)first : ~0u;
+    w.end = end < ~0u ? (uint32_t)end : ~0u;
+    w.next = served ? (uint32_t)(left - before) : 0;
+    w.len = r.len;
+    w.held = served ? r.held : -1;
     return w;
 }
-// Slot and position of token t of request i.
-__device__ __forceinline__ uint32_t place_token(const CacheArgs& A, const Owner& w, uint64_t i, uint64_t t, int64_t* slot, int32_t* pos) {
+// Slot and position of token t of request i.  ENTER: it enters its page, if that is beyond the first kGroupPages new ones.
+template <bool ENTER>
+__device__ __forceinline__ uint32_t place_token(const CacheArgs& A, PageDiv D, const Owner& w, uint64_t i, uint64_t t, int64_t* slot, int32_t* pos) {
     *slot = -1;
     *pos = -1;
     if (w.held < 0 || t < w.first || t >= w.end) return 0;
-    const uint32_t q = (uint32_t)w.len + (uint32_t)(t - w.first), p = q / A.page, in = q - p * A.page;
+    const uint32_t q = (uint32_t)w.len + (uint32_t)(t - w.first), p = D.of(q), in = q - p * A.page;
     // (pages that are new may not be in the table yet)
-    const int32_t id = p < (uint32_t)w.held ? A.table[i * A.table_stride + p] : A.free_pages[w.next - 1 - (p - (uint32_t)w.held)];
+    int32_t* entry = A.table + i * A.table_stride + p;
+    const int32_t id = p < (uint32_t)w.held ? *entry : A.free_pages[w.next - 1 - (p - (uint32_t)w.held)];
+    if (ENTER && in == 0 && p >= (uint32_t)w.held + kGroupPages) *entry = id;
     *pos = (int32_t)q;
     *slot = slot_of(id, in, A.page, A.n_pages);
     return *slot < 0 ? (uint32_t)kCachePage : 0u;
 }
 
-// Tokens in blocks of 512, two neighbours a thread; the requests of a block are found once and kept in LDS (more than kOwners of
-// them only where many requests have no new token: then every token looks for its own).
-constexpr int kTokensPer = 2, kTokenBlock = kApplyThreads * kTokensPer, kOwners = 512, kMaxPlans = (int)(kMaxSeqs / kPlanThreads);
-constexpr uint64_t kRequestBlock = 4 * kApplyWaves;   // requests of a workgroup, four a wave (it divides kPlanThreads)
+// Tokens in blocks of 256 PER, PER neighbours a thread; the requests of a block are found once and kept in LDS (more than there are
+// tokens in a block only where many requests have no new token: then every token looks for its own).  Two tokens a thread / four,
+// us: 65,536 requests of one token 11.6 / 13.5, a million tokens of 2,048 prompts 13.0 / 12.5, 4 million of 8,192 27.9 / 25.2, 14 million of
+// 65,536 74 / 63 (eight: 67): four from kManyTokens on.
+//
+// The state of a request is a thread's: 16 requests a workgroup, 256 where there are 16,384 and more.  It enters the first new pages
+// itself, sixteen lanes together the next up to kGroupPages, the tokens those behind: a new page's first slot is always a new token's.
+// (With a wave for all pages of a request one of a million tokens took 110 us, now 10.5; 2^20 requests of one token 205, now 40.)
+constexpr uint64_t kManyTokens = 1u << 20;
+constexpr int kMaxPlans = (int)(kMaxSeqs / kPlanThreads);
+constexpr uint64_t kManyRequests = 16384;
 
-__global__ __launch_bounds__(kApplyThreads) void cache_slots_kernel(CacheArgs A, const PlanRec* recs, const u64* blocks,
-                                                                    const CacheHead* head, uint64_t request_blocks) {
+// n entries of `from`, in steps of `step` (1 or -1), to `to`, by sixteen lanes with eight in flight.
+__device__ __forceinline__ void copy_pages(int32_t* to, const int32_t* from, int step, int32_t n) {
+    for (int32_t j0 = threadIdx.x % kPageLanes; j0 < n; j0 += 8 * kPageLanes) {
+        int32_t page[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) page[k] = from[step * (j0 + kPageLanes * k < n ? j0 + kPageLanes * k : j0)];
+#pragma unroll
+        for (int k = 0; k < 8; k++) if (j0 + kPageLanes * k < n) to[j0 + kPageLanes * k] = page[k];
+    }
+}
+// Places in a list for the lanes that want one; called by whole waves.
+__device__ __forceinline__ uint32_t list_place(bool want, uint32_t* count) {
+    const u64 m = __ballot(want);
+    uint32_t at = 0;
+    if (m && lane_id() == 0) at = atomicAdd(count, (uint32_t)__popcll(m));
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + (uint32_t)__popcll(m & ((1ull << lane_id()) - 1));
+}
+
+template <int PER>
+__global__ __launch_bounds__(kApplyThreads) void cache_slots_kernel(CacheArgs A, PageDiv D, const PlanRec* recs, const u64* blocks,
+                                                                    const CacheHead* head, uint64_t request_blocks, uint32_t per_request_block) {
+    constexpr int kTokenBlock = kApplyThreads * PER, kOwners = kTokenBlock;
     __shared__ u64 tmp[kApplyWaves];
     __shared__ Owner owners[kOwners];
     __shared__ uint64_t ends[2];
+    __shared__ uint32_t s_many, many_of[kApplyThreads];
+    static_assert(kOwners >= kApplyThreads, "the list of requests with many pages lies there too");
     const uint64_t left = head->left;
     uint32_t bits = 0;
     if (blockIdx.x == 0) {
@@ -175,24 +213,38 @@ __global__ __launch_bounds__(kApplyThreads) void cache_slots_kernel(CacheArgs A,
         return;
     }
     if (blockIdx.x <= request_blocks) {  // a wave per request: its new state, and its new pages into the table
-        const uint64_t i0 = (blockIdx.x - 1) * kRequestBlock;
-        const u64 base = pages_before(blocks, i0 / kPlanThreads, tmp);
+        const uint64_t i0 = (uint64_t)(blockIdx.x - 1) * per_request_block, i = i0 + threadIdx.x;   // (it divides kPlanThreads)
+        if (threadIdx.x == 0) s_many = 0;
+        const bool mine = threadIdx.x < per_request_block && i < A.n;
+        const PlanRec r = recs[mine ? i : i0];
+        const u64 before = pages_before(blocks, i0 / kPlanThreads, tmp) + r.before;   // (barriers inside)
+        const bool served = mine && slots_served(r, before, left);
+        if (mine) {
+            A.len_out[i] = served ? r.new_len : r.len;
+            A.held_out[i] = served ? r.held + r.delta : r.held;
+            bits = served ? 0u : r.flags ? r.flags : (uint32_t)kCachePool;
+        }
+        if (served && r.delta) {
+            int32_t* to = A.table + i * A.table_stride + r.held;
+            const int32_t* from = A.free_pages + (left - before) - 1;
+            int32_t page[kFirstPages];
 #pragma unroll
-        for (uint64_t i = i0 + wave_id(); i < i0 + kRequestBlock; i += kApplyWaves) {
-            if (i >= A.n) break;
-            const PlanRec r = recs[i];
-            const u64 before = base + r.before;
-            const bool served = slots_served(r, before, left);
-            if (lane_id() == 0) {
-                A.len_out[i] = served ? r.new_len : r.len;
-                A.held_out[i] = served ? r.held + r.delta : r.held;
-                bits |= served ? 0u : r.flags ? r.flags : (uint32_t)kCachePool;
-            }
-            if (served) {
-                int32_t* to = A.table + i * A.table_stride + r.held;
-                const int32_t* from = A.free_pages + (left - before) - 1;
-                for (int32_t j = lane_id(); j < r.delta; j += 64) to[j] = *(from - j);
-            }
+            for (int32_t j = 0; j < kFirstPages; j++) page[j] = *(from - (j < r.delta ? j : 0));
+#pragma unroll
+            for (int32_t j = 0; j < kFirstPages; j++) if (j < r.delta) to[j] = page[j];
+        }
+        const bool more = served && r.delta > kFirstPages;
+        const uint32_t at = list_place(more, &s_many);
+        if (more) {
+            owners[at].next = (uint32_t)(left - before);
+            owners[at].held = r.held;
+            owners[at].len = r.delta;
+            many_of[at] = threadIdx.x;
+        }
+        __syncthreads();
+        for (uint32_t x = threadIdx.x / kPageLanes; x < s_many; x += kApplyThreads / kPageLanes) {
+            const int32_t n = owners[x].len < kGroupPages ? owners[x].len : kGroupPages;
+            copy_pages(A.table + (i0 + many_of[x]) * A.table_stride + owners[x].held + kFirstPages, A.free_pages + owners[x].next - 1 - kFirstPages, -1, n - kFirstPages);
         }
     } else {
         const uint64_t t0 = (uint64_t)(blockIdx.x - 1 - request_blocks) * kTokenBlock;
@@ -221,33 +273,33 @@ __global__ __launch_bounds__(kApplyThreads) void cache_slots_kernel(CacheArgs A,
             u64 before = base;
             for (uint64_t b = b0; b < i / kPlanThreads; b++) before += blocks[b];
             const PlanRec r = recs[i];
-            return owner_of(A, r, A.off[i], A.off[i + 1], before + r.before, left);
+            return owner_of(r, A.off[i], A.off[i + 1], before + r.before, left);
         };
-        const uint64_t t = t0 + (uint64_t)threadIdx.x * kTokensPer;
-        int64_t slot[kTokensPer];
-        int32_t pos[kTokensPer];
+        const uint64_t t = t0 + (uint64_t)threadIdx.x * PER;
+        int64_t slot[PER];
+        int32_t pos[PER];
         if (many <= kOwners) {
             for (uint64_t k = threadIdx.x; k < many; k += kApplyThreads) owners[k] = load_owner(a0 + k);
             __syncthreads();
             uint32_t k = 0, e = (uint32_t)many;
             while (e - k > 1) { const uint32_t m = (k + e) / 2; if (owners[m].first <= t) k = m; else e = m; }
 #pragma unroll
-            for (int j = 0; j < kTokensPer; j++) {
+            for (int j = 0; j < PER; j++) {
                 while (k + 1 < (uint32_t)many && owners[k + 1].first <= t + j) k++;
-                if (t + j <= last) bits |= place_token(A, owners[k], a0 + k, t + j, &slot[j], &pos[j]);
+                if (t + j <= last) bits |= place_token<true>(A, D, owners[k], a0 + k, t + j, &slot[j], &pos[j]);
             }
         } else {
-            for (int j = 0; j < kTokensPer; j++) {
+            for (int j = 0; j < PER; j++) {
                 uint64_t a = 0, b = A.n;
                 while (b - a > 1) { const uint64_t m = (a + b) / 2; if (A.off[m] <= t + j) a = m; else b = m; }
-                if (t + j <= last) bits |= place_token(A, load_owner(a), a, t + j, &slot[j], &pos[j]);
+                if (t + j <= last) bits |= place_token<true>(A, D, load_owner(a), a, t + j, &slot[j], &pos[j]);
             }
         }
-        if (t + kTokensPer <= last + 1) {
+        if (t + PER <= last + 1) {
             __builtin_memcpy(A.slots + t, slot, sizeof slot);
             __builtin_memcpy(A.pos + t, pos, sizeof pos);
         } else {
-            for (int j = 0; j < kTokensPer; j++) if (t + j <= last) { A.slots[t + j] = slot[j]; A.pos[t + j] = pos[j]; }
+            for (int j = 0; j < PER; j++) if (t + j <= last) { A.slots[t + j] = slot[j]; A.pos[t + j] = pos[j]; }
         }
     }
     if (bits) atomicOr(A.status, bits);
@@ -275,7 +327,7 @@ constexpr uint64_t kOneTokens = 4096;   // (a workgroup of 1,024 has them in fou
 constexpr int kOneSmall = 256;
 
 template <int THREADS>
-__global__ __launch_bounds__(THREADS) void cache_slots_one_kernel(CacheArgs A) {
+__global__ __launch_bounds__(THREADS) void cache_slots_one_kernel(CacheArgs A, PageDiv D) {
     __shared__ u64 tmp[THREADS / 64];
     __shared__ Owner owners[THREADS];
     __shared__ uint32_t s_before[THREADS], s_status, s_taken;
@@ -298,7 +350,7 @@ __global__ __launch_bounds__(THREADS) void cache_slots_one_kernel(CacheArgs A) {
     if (i < A.n) {
         const bool served = slots_served(r, before, left);
         takes = served && r.delta;
-        owners[i] = owner_of(A, r, first, end, before, left);
+        owners[i] = owner_of(r, first, end, before, left);
         s_before[i] = (uint32_t)before;   // (a request asks for at most kOneTokens pages)
         A.len_out[i] = served ? r.new_len : r.len;
         A.held_out[i] = served ? r.held + r.delta : r.held;
@@ -317,7 +369,7 @@ __global__ __launch_bounds__(THREADS) void cache_slots_one_kernel(CacheArgs A) {
         while (e - k > 1) { const uint32_t m = (k + e) / 2; if (owners[m].first <= t) k = m; else e = m; }
         int64_t slot;
         int32_t pos;
-        const uint32_t bits = place_token(A, owners[k], k, t, &slot, &pos);
+        const uint32_t bits = place_token<false>(A, D, owners[k], k, t, &slot, &pos);
         A.slots[t] = slot;
         A.pos[t] = pos;
         if (bits) atomicOr(&s_status, bits);
@@ -362,7 +414,6 @@ __global__ __launch_bounds__(kApplyThreads) void cache_trim_kernel(CacheArgs A, 
 // all 58 / 6.8.  A step after drafts is the first of these and a batch that ends at once is rare, so the limit is where that
 // costs 11 us.
 constexpr uint64_t kOnePages = 131072, kOnePagesSmall = 1024;   // pages that the requests hold at the very most
-constexpr int32_t kFirstPages = 2, kPageLanes = 16;
 
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void cache_trim_one_kernel(CacheArgs A) {
@@ -398,31 +449,16 @@ __global__ __launch_bounds__(THREADS) void cache_trim_one_kernel(CacheArgs A) {
         for (int32_t j = 0; j < kFirstPages; j++) if (j < r.delta) to[j] = page[j];
     }
     const bool many = gives && r.delta > kFirstPages;
-    const u64 m = __ballot(many);
-    if (m) {
-        uint32_t at = 0;
-        if (lane_id() == 0) at = atomicAdd(&s_n_many, (uint32_t)__popcll(m));
-        at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + (uint32_t)__popcll(m & ((1ull << lane_id()) - 1));
-        if (many) {
-            s_many[at] = (uint32_t)i;
-            s_before[at] = (uint32_t)before + kFirstPages;
-            s_first[at] = stay + kFirstPages;
-            s_delta[at] = r.delta - kFirstPages;
-        }
+    const uint32_t at = list_place(many, &s_n_many);
+    if (many) {
+        s_many[at] = (uint32_t)i;
+        s_before[at] = (uint32_t)before + kFirstPages;
+        s_first[at] = stay + kFirstPages;
+        s_delta[at] = r.delta - kFirstPages;
     }
     __syncthreads();
-    for (uint32_t x = threadIdx.x / kPageLanes; x < s_n_many; x += THREADS / kPageLanes) {
-        const int32_t* from = A.table + (uint64_t)s_many[x] * A.table_stride + s_first[x];
-        int32_t* to = A.free_pages + left + s_before[x];
-        const int32_t n = s_delta[x];
-        for (int32_t j0 = threadIdx.x % kPageLanes; j0 < n; j0 += 8 * kPageLanes) {
-            int32_t page[8];
-#pragma unroll
-            for (int k = 0; k < 8; k++) page[k] = from[j0 + kPageLanes * k < n ? j0 + kPageLanes * k : j0];
-#pragma unroll
-            for (int k = 0; k < 8; k++) if (j0 + kPageLanes * k < n) to[j0 + kPageLanes * k] = page[k];
-        }
-    }
+    for (uint32_t x = threadIdx.x / kPageLanes; x < s_n_many; x += THREADS / kPageLanes)
+        copy_pages(A.free_pages + left + s_before[x], A.table + (uint64_t)s_many[x] * A.table_stride + s_first[x], 1, s_delta[x]);
     if (threadIdx.x == 0) {
         *A.n_free_out = bad ? n_free : n_free + (int32_t)s_given;
         *A.status = s_status;
@@ -439,14 +475,18 @@ Parts parts_of(const CacheArgs& A) {
 }  // namespace
 
 hipError_t launch_cache_slots(const CacheArgs& A, hipStream_t stream) {
-    if (A.n <= kOneSmall && A.cap <= kOneTokens / 4) return launch(cache_slots_one_kernel<kOneSmall>, 1, kOneSmall, stream, A);
-    if (A.n <= kPlanThreads && A.cap <= kOneTokens) return launch(cache_slots_one_kernel<kPlanThreads>, 1, kPlanThreads, stream, A);
+    const PageDiv D = page_div(A.page);
+    if (A.n <= kOneSmall && A.cap <= kOneTokens / 4) return launch(cache_slots_one_kernel<kOneSmall>, 1, kOneSmall, stream, A, D);
+    if (A.n <= kPlanThreads && A.cap <= kOneTokens) return launch(cache_slots_one_kernel<kPlanThreads>, 1, kPlanThreads, stream, A, D);
     const Parts P = parts_of(A);
     hipError_t e = launch(cache_plan_kernel<false>, P.plan_blocks, kPlanThreads, stream, A, P.recs, P.blocks, P.head);
     if (e != hipSuccess) return e;
-    const uint64_t request_blocks = (A.n + kRequestBlock - 1) / kRequestBlock, token_blocks = A.n ? (A.cap + kTokenBlock - 1) / kTokenBlock : 0;
-    return launch(cache_slots_kernel, 1 + request_blocks + token_blocks, kApplyThreads, stream, A, (const PlanRec*)P.recs, (const u64*)P.blocks, (const CacheHead*)P.head,
-                  request_blocks);
+    const uint32_t per_request_block = A.n < kManyRequests ? 16 : kApplyThreads;
+    const bool many = A.cap >= kManyTokens;
+    const uint64_t request_blocks = (A.n + per_request_block - 1) / per_request_block, token_block = (uint64_t)kApplyThreads * (many ? 4 : 2);
+    const uint64_t token_blocks = A.n ? (A.cap + token_block - 1) / token_block : 0;
+    return launch(many ? cache_slots_kernel<4> : cache_slots_kernel<2>, 1 + request_blocks + token_blocks, kApplyThreads, stream, A, D, (const PlanRec*)P.recs,
+                  (const u64*)P.blocks, (const CacheHead*)P.head, request_blocks, per_request_block);
 }
 
 hipError_t launch_cache_trim(const CacheArgs& A, hipStream_t stream) {

@@ -451,8 +451,8 @@ __global__ __launch_bounds__(kGradThreads) void grad_join_kernel(GradWalk P, con
 // One launch, nothing sorted.  A workgroup per position and 512 columns: it compares all ids with its own, leaves if one before it
 // is the same, and else adds up the rows of those that are, every wave a quarter of them.  Its own row and the table's are on
 // their way while it compares.  Bound by the chain ids -> rows -> store: 5.4 us for 512 ids of 2,048 columns, 5.0 a call among others
-// (sorted: 16 us).  WORDS * 64 ids are compared whatever n is, so there is a kernel each for 512, 1,024, 2,048 and 4,096 of them: 512
-// ids of 2,048 columns take 6.7 us in the one for 2,048.
+// (sorted: 16 us).  WORDS * 64 ids are compared whatever n is, so there is a kernel each for 512, 1,024 and 2,048 of them: 512 ids of
+// 2,048 columns take 6.7 us in the one for 2,048.
 constexpr int kDirectGroup = 8;
 
 template <class G, class T, bool SMALL, int WORDS>
@@ -580,7 +580,6 @@ hipError_t launch_embed_grad(const EmbedGradArgs& A, hipStream_t stream) {
             typedef decltype(t) T;
             auto* kernel = A.n <= 512    ? grad_direct_kernel<G, T, small.value, 8>
                            : A.n <= 1024 ? grad_direct_kernel<G, T, small.value, 16>
-                           : A.n <= 2048 ? grad_direct_kernel<G, T, small.value, 32>
                                          : grad_direct_kernel<G, T, small.value, (int)(kDirectIds / 64)>;
             return launch(kernel, A.n * col_tiles + zero_blocks, kGradThreads, stream, A.ids, (uint32_t)A.n, A.n_dev, rows, (const G*)A.grad, A.grad_stride, dim,
                           (T*)A.table, A.table_stride, A.scale, A.accumulate, col_tiles);

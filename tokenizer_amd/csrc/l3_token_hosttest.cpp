@@ -15,6 +15,8 @@ uint64_t l3t_grad_work(uint64_t n, uint64_t dim) { return grad_work(n, dim).tota
 uint64_t l3t_cache_work(uint64_t n) { return cache_work(n).total; }
 uint64_t l3t_verify_work(uint64_t n, uint64_t vocab) { return verify_work(n, vocab).total; }
 
+uint32_t l3t_page_div(uint32_t x, uint32_t page) { return page_div(page).of(x); }
+
 void l3t_cache_slots(const CacheArgs* P) {
     const CacheArgs& A = *P;
     const int32_t n_free = *A.n_free;

@@ -71,10 +71,11 @@ inline int sort_rounds(uint64_t n) { return n <= 65536 ? 1 : n <= 262144 ? 2 : 4
 inline uint64_t sort_tiles(uint64_t n) { const uint64_t t = (uint64_t)kSortThreads * sort_rounds(n); return (n + t - 1) / t; }
 // Few ids are not sorted: every position looks for the others of its id by itself, a workgroup for each and 512 columns.  On the GPU,
 // us, so / sorted (which is two launches more): 512 ids of 2,048 columns 5 / 16, 1,500 of 2,048 13.1 / 15.8, 768 of 4,096 13.7 / 15.0,
-// 1,024 of 4,096 16.9 / 15.6; above 2,048 ids, where every workgroup compares more: 3,000 of 512 12.4 / 15.5, of 1,024 19.3 / 16.6.  Up to
-// kRankIds ids are sorted in one launch by counting, more digit by digit (l3_embed.hip has the times of both).
-constexpr uint64_t kDirectIds = 4096, kRankIds = 8192;
-inline bool grad_direct(uint64_t n, uint64_t dim) { return n <= kDirectIds && n * ((dim + 511) / 512) <= (n <= 2048 ? 6144u : 4096u); }
+// 1,024 of 4,096 16.9 / 15.6.  The limit on the ids is for batches that are one id throughout, whose rows one workgroup adds up: 2,048
+// ids 57 / 16, 4,096 117 / 17.  Up to kRankIds ids are sorted in one launch by counting, more digit by digit (l3_embed.hip has the
+// times of both).
+constexpr uint64_t kDirectIds = 2048, kDirectBlocks = 6144, kRankIds = 8192;
+inline bool grad_direct(uint64_t n, uint64_t dim) { return n <= kDirectIds && n * ((dim + 511) / 512) <= kDirectBlocks; }
 // Sorted positions one wave adds up: few enough that there are about kGradWalkers waves, and 8 .. 64.  By kGradWalkers = 8,192 /
 // 4,096 / 2,048 / 1,024, us: 16,384 ids of 2,048 columns 72 / 60 / 56 / 60, 65,536 of 1,024 98 / 86 / 84 / 84 (more waves leave more parts).
 constexpr uint64_t kGradWalkers = 2048;
@@ -249,6 +250,17 @@ L3_HD bool slots_served(const PlanRec& r, uint64_t before, uint64_t left) {
 }
 L3_HD bool trim_served(const PlanRec& r, uint64_t before, uint64_t left, uint64_t n_pages) {
     return r.flags == 0 && (r.delta == 0 || left + before + (uint64_t)r.delta <= n_pages);
+}
+// x / page for x < 2^31 by a product: with 2^s the first power of two that is not below page, m = floor(2^(31 + s) / page) + 1 is
+// 2^(31 + s) / page + e, 0 < e <= 1, so x m / 2^(31 + s) is x / page + x e / 2^(31 + s), too large by less than 2^-s <= 1 / page.
+struct PageDiv {
+    uint32_t m, shift;
+    L3_HD uint32_t of(uint32_t x) const { return (uint32_t)(((uint64_t)x * m) >> shift); }
+};
+inline PageDiv page_div(uint32_t page) {
+    uint32_t s = 0;
+    while ((1u << s) < page) s++;
+    return {(uint32_t)((1ull << (31 + s)) / page + 1), 31 + s};
 }
 L3_HD int64_t slot_of(int32_t page_id, uint32_t in_page, uint32_t page, uint32_t n_pages) {
     if (page_id < 0 || (uint32_t)page_id >= n_pages) return -1;
