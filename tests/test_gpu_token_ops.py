@@ -686,6 +686,20 @@ def test_verify_vocabularies(ctx, torch, vocab, code, with_q):
             vocab + 3, vocab + 1, shift=1)
 
 
+@pytest.mark.parametrize("n, vocab", [(2047, 4097), (2048, 4097), (2048, 6144), (1536, 6145), (1536, 8193), (700, 20481)])
+@pytest.mark.parametrize("code", [F32, BF16])
+def test_verify_many_requests(ctx, torch, n, vocab, code):
+    """Enough requests that a workgroup has several pieces of a row; rows that end anywhere in them."""
+    rng = np.random.default_rng(n + vocab)
+    k = rng.integers(0, 2, n)
+    off = [0] + np.cumsum(k).tolist()
+    total = off[-1]
+    target, q = _probs(rng, total + n, vocab), _probs(rng, total, vocab)
+    target[rng.random(target.shape) < 0.999] = 0.0      # few entries with weight: wrong by one place is another token
+    draft = rng.integers(0, vocab, total).astype(np.int32)
+    _verify(ctx, torch, draft, off, total, 1, target, q, code, vocab, rng.random(total), rng.random(n), vocab, vocab)
+
+
 @pytest.mark.parametrize("k", [1, 2, 63, 64, 65, 130])
 def test_verify_many_drafts(ctx, torch, k):
     """Every place at which the first rejection can be, beyond a wave's width; draws at both ends of [0, 1)."""

@@ -104,32 +104,42 @@ __device__ __forceinline__ double of_lane_f64(double v, int lane) {
 }
 __device__ __forceinline__ double wave_sum_f64(double v) { return of_lane_f64(wave_iscan_f64(v), 63); }
 
-// Sums of kVerifyChunk entries: sums[i][chunk] = {rest, full}.  A workgroup per request and chunk; that of chunk 0 leaves the
+// Sums of kVerifyChunk entries: sums[i][chunk] = {rest, full}.  A workgroup per request and C chunks; that of chunk 0 leaves the
 // verdict, and all of the answer but the drawn token.  Bound by memory: 128 requests over 128,256 entries in 32 bits (131 MB) take
-// 23.5 us, 5.6 TB/s; one request 4 us, the chain offset -> token -> its probabilities -> row.  (Each workgroup works the verdict out for
-// itself: a launch of its own for it would cost as much as the chain.)
-template <class T>
+// 23 us, 5.7 TB/s; one request 4 us, the chain offset -> token -> its probabilities -> row.  (Each workgroup works the verdict out for
+// itself: a launch of its own for it would cost as much as the chain.)  Where there are more workgroups than the GPU holds at once,
+// three chunks share that chain; one / three, us of both launches: 128 requests in 32 bits 26.0 / 25.1, in 16 bits 23.1 / 21.1, 1,024 in
+// 16 bits 136 / 102, 2,000 over 32,000 entries 88 / 75, but 64 requests in 32 bits 17.6 / 19.1.
+constexpr uint64_t kVerifyMany = 6144;
+template <class T, int C>
 __global__ __launch_bounds__(kVerifyThreads) void verify_sum_kernel(VerifyArgs A, uint64_t chunks, double2* sums, Verdict* verdicts) {
-    __shared__ double2 tmp[kVerifyThreads / 64];
-    for (uint64_t g = blockIdx.x; g < A.n * chunks; g += gridDim.x) {
-        const uint64_t i = g / chunks, c = g - i * chunks;
+    __shared__ double2 tmp[C][kVerifyThreads / 64];
+    const uint64_t groups = (chunks + C - 1) / C;
+    for (uint64_t g = blockIdx.x; g < A.n * groups; g += gridDim.x) {
+        const uint64_t i = g / groups, c = (g - i * groups) * C;
         const Verdict R = verdict_of<T>(A, i);
-        double sr = 0, sf = 0;
-        const uint64_t col = c * kVerifyChunk + (uint64_t)threadIdx.x * 8;
-        if (R.state != kBadRequest && col < A.vocab) {
-            double rest[8], full[8];
-            weights8<T>(A, R, col, rest, full);
+        double sr[C], sf[C];
 #pragma unroll
-            for (int j = 0; j < 8; j++) { sr += rest[j]; sf += full[j]; }
+        for (int x = 0; x < C; x++) {
+            sr[x] = sf[x] = 0;
+            const uint64_t col = (c + x) * kVerifyChunk + (uint64_t)threadIdx.x * 8;
+            if (R.state != kBadRequest && col < A.vocab) {
+                double rest[8], full[8];
+                weights8<T>(A, R, col, rest, full);
+#pragma unroll
+                for (int j = 0; j < 8; j++) { sr[x] += rest[j]; sf[x] += full[j]; }
+            }
         }
-        sr = wave_sum_f64(sr);
-        sf = wave_sum_f64(sf);
-        if (lane_id() == 0) tmp[wave_id()] = make_double2(sr, sf);
+#pragma unroll
+        for (int x = 0; x < C; x++) {
+            const double wr = wave_sum_f64(sr[x]), wf = wave_sum_f64(sf[x]);
+            if (lane_id() == 0) tmp[x][wave_id()] = make_double2(wr, wf);
+        }
         __syncthreads();
-        if (threadIdx.x == 0) {
-            double2 s = tmp[0];
-            for (int w = 1; w < kVerifyThreads / 64; w++) { s.x += tmp[w].x; s.y += tmp[w].y; }
-            sums[g] = s;
+        if (threadIdx.x < C && c + threadIdx.x < chunks) {
+            double2 s = tmp[threadIdx.x][0];
+            for (int w = 1; w < kVerifyThreads / 64; w++) { s.x += tmp[threadIdx.x][w].x; s.y += tmp[threadIdx.x][w].y; }
+            sums[i * chunks + c + threadIdx.x] = s;
         }
         if (c == 0) {
             int32_t* out = A.out + i * (A.max_draft + 1ull);
@@ -223,7 +233,9 @@ hipError_t launch_verify(const VerifyArgs& A, hipStream_t stream) {
     Verdict* verdicts = (Verdict*)((uint8_t*)A.work + W.verdicts);
     return with_dtype(A.dtype, [&](auto t) {
         typedef decltype(t) T;
-        hipError_t e = launch(verify_sum_kernel<T>, capped(A.n * W.chunks), kVerifyThreads, stream, A, W.chunks, sums, verdicts);
+        const bool many = W.chunks >= 3 && A.n * W.chunks >= kVerifyMany;
+        hipError_t e = launch(many ? verify_sum_kernel<T, 3> : verify_sum_kernel<T, 1>, capped(A.n * (many ? (W.chunks + 2) / 3 : W.chunks)), kVerifyThreads, stream, A,
+                              W.chunks, sums, verdicts);
         if (e != hipSuccess) return e;
         return launch(verify_draw_kernel<T>, capped(A.n), kVerifyThreads, stream, A, W.chunks, (const double2*)sums, (const Verdict*)verdicts);
     });
