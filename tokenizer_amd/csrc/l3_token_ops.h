@@ -76,9 +76,10 @@ inline uint64_t sort_tiles(uint64_t n) { const uint64_t t = (uint64_t)kSortThrea
 // times of both).
 constexpr uint64_t kDirectIds = 2048, kDirectBlocks = 6144, kRankIds = 8192;
 inline bool grad_direct(uint64_t n, uint64_t dim) { return n <= kDirectIds && n * ((dim + 511) / 512) <= kDirectBlocks; }
-// Sorted positions one wave adds up: few enough that there are about kGradWalkers waves, and 8 .. 64.  By kGradWalkers = 8,192 /
-// 4,096 / 2,048 / 1,024, us: 16,384 ids of 2,048 columns 72 / 60 / 56 / 60, 65,536 of 1,024 98 / 86 / 84 / 84 (more waves leave more parts).
-constexpr uint64_t kGradWalkers = 2048;
+// Sorted positions one wave adds up: few enough that there are about kGradWalkers waves, and 8 .. 64.  By kGradWalkers = 1,024 / 2,048 /
+// 4,096 / 8,192, us: 65,536 ids of 64 columns 52 / 40 / 39 / 40, of 2,048 168 / 169 / 167 / 160, 16,384 of 2,048 57 / 50 / 51 / 53 (fewer waves
+// leave the GPU idle, more leave more parts).
+constexpr uint64_t kGradWalkers = 4096;
 constexpr int kGradWaves = 4;        // waves of a workgroup
 inline uint32_t grad_chunk(uint64_t n, uint64_t dim) {
     const uint64_t want = n * ((dim + 511) / 512) / kGradWalkers;
