@@ -512,6 +512,18 @@ def test_cache_counts_that_cannot_be(ctx, torch, n_free):
     assert int(dev.status[0]) == status and dev.state() == (model.length, model.held, model.table, model.free, model.n_free)
 
 
+@pytest.mark.parametrize("n", [5, 3000])
+def test_cache_trim_leaves_alone_whatever_stands_there(ctx, torch, n):
+    """keep < 0: also where length and pages make no sense; nothing is reported, the requests beside it are served."""
+    length, held = [(5, -5, 9)[i % 3] for i in range(n)], [(1, -5, 2 ** 31 - 1)[i % 3] for i in range(n)]
+    state = (length, held, [[i, -5, -5] for i in range(n)], [-5] * n, 0, 8, n, 3)
+    dev, model = DeviceCache(torch, state), ref.Cache(*state)
+    keep = [0 if i % 3 == 0 else -1 - i for i in range(n)]
+    assert model.trim(keep) == 0
+    dev.trim(ctx, torch.tensor(keep, dtype=torch.int32, device="cuda"))
+    assert dev.state() == (model.length, model.held, model.table, model.free, model.n_free) and int(dev.status[0]) == 0
+
+
 @pytest.mark.parametrize("n, every, most", [(20000, 1, 500), (3, 1, 2000000), (2 ** 20, 1, 9), (2 ** 20, 1000, 8500), (16384, 1, 600), (16383, 1, 600)])
 def test_cache_of_millions_of_tokens(ctx, torch, n, every, most):
     """Four million tokens and more, of few long requests and of many short ones, some under way, some without a new token."""

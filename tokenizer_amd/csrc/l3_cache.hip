@@ -10,8 +10,8 @@
 //   apply  adds up the workgroups' sums, decides who is served, writes table, slots, positions and the new state.
 // A step that one workgroup has through in the time of a launch does both in one (cache_slots_one_kernel, cache_trim_one_kernel).
 // All of it is bound by latency: chains of dependent loads, and launches.  Measured, us a call among others: 256 requests of one
-// token 5.2 (one launch; 4.6 on the GPU), 2,048 prompts with a million tokens 12.9 (3.8 + 9.5 on the GPU; 12.6 MB written, 2.5 us at a
-// copy's rate), a trim of 256 requests after drafts 5.1 (3.4 on the GPU), of 2,048 requests 8.1 (4.0 + 3.1).
+// token 5.4 (one launch; 4.4 on the GPU), 2,048 prompts with a million tokens 12.4 (4.0 + 9.0 on the GPU; 12.6 MB written, 2.5 us at a
+// copy's rate), a trim of 256 requests after drafts 5.1 (3.3 on the GPU), of 2,048 requests 8.3 (4.0 + 3.1).
 #include "l3_token_kernels.h"
 
 #include "l3_dev.h"
@@ -134,14 +134,28 @@ __device__ __forceinline__ uint64_t request_of(const uint64_t* off, uint64_t n, 
 
 constexpr int32_t kFirstPages = 2, kPageLanes = 16, kGroupPages = 512;
 
+// A record of the plan that would lead outside the table or the pool is not served.  The plan makes none; a workspace shared by
+// mistake may hold one.
+__device__ __forceinline__ bool kept_within(const CacheArgs& A, const PlanRec& r, bool trim, u64 before, u64 left) {
+    if (r.held < 0 || r.delta < 0 || left > A.n_pages || (uint64_t)r.held + (trim ? 0u : (uint32_t)r.delta) > A.max_pages) return false;
+    const u64 most = trim ? A.n_pages - left : left;
+    return r.delta == 0 || ((!trim || r.delta <= r.held) && before <= most && (u64)r.delta <= most - before);
+}
+__device__ __forceinline__ bool slots_served_within(const CacheArgs& A, const PlanRec& r, u64 before, u64 left) {
+    return slots_served(r, before, left) && kept_within(A, r, false, before, left);
+}
+
 // What a token needs of its request (tokens and pages are below 2^31; an offset that is not is the largest number instead).
 struct Owner {
     uint32_t first, end;     // its new tokens
     uint32_t next;           // free list: its first new page is at next - 1
     int32_t len, held;       // held < 0: not served
 };
-__device__ __forceinline__ Owner owner_of(const PlanRec& r, uint64_t first, uint64_t end, u64 before, u64 left) {
-    const bool served = slots_served(r, before, left);
+__device__ __forceinline__ Owner owner_of(const CacheArgs& A, const PlanRec& r, uint64_t first, uint64_t end, u64 before, u64 left) {
+    // (its tokens end within its pages, so that place_token need not look at each)
+    const u64 upto = (u64)r.len + (end - first);
+    const bool served = slots_served_within(A, r, before, left) && r.len >= 0 && end >= first && upto <= kMaxCount &&
+                        upto <= ((u64)r.held + (u64)r.delta) * A.page;
     Owner w;
     w.first = first < ~0u ? (uint32_t)first : ~0u;
     w.end = end < ~0u ? (uint32_t)end : ~0u;
@@ -212,13 +226,13 @@ __global__ __launch_bounds__(kApplyThreads) void cache_slots_kernel(CacheArgs A,
         if (threadIdx.x == 0) { const int32_t n = *A.n_free; *A.n_free_out = head->bad ? n : n - (int32_t)taken; }
         return;
     }
-    if (blockIdx.x <= request_blocks) {  // a wave per request: its new state, and its new pages into the table
+    if (blockIdx.x <= request_blocks) {  // a thread per request: its new state, and its new pages into the table
         const uint64_t i0 = (uint64_t)(blockIdx.x - 1) * per_request_block, i = i0 + threadIdx.x;   // (it divides kPlanThreads)
         if (threadIdx.x == 0) s_many = 0;
         const bool mine = threadIdx.x < per_request_block && i < A.n;
         const PlanRec r = recs[mine ? i : i0];
         const u64 before = pages_before(blocks, i0 / kPlanThreads, tmp) + r.before;   // (barriers inside)
-        const bool served = mine && slots_served(r, before, left);
+        const bool served = mine && slots_served_within(A, r, before, left);
         if (mine) {
             A.len_out[i] = served ? r.new_len : r.len;
             A.held_out[i] = served ? r.held + r.delta : r.held;
@@ -273,7 +287,7 @@ __global__ __launch_bounds__(kApplyThreads) void cache_slots_kernel(CacheArgs A,
             u64 before = base;
             for (uint64_t b = b0; b < i / kPlanThreads; b++) before += blocks[b];
             const PlanRec r = recs[i];
-            return owner_of(r, A.off[i], A.off[i + 1], before + r.before, left);
+            return owner_of(A, r, A.off[i], A.off[i + 1], before + r.before, left);
         };
         const uint64_t t = t0 + (uint64_t)threadIdx.x * PER;
         int64_t slot[PER];
@@ -350,7 +364,7 @@ __global__ __launch_bounds__(THREADS) void cache_slots_one_kernel(CacheArgs A, P
     if (i < A.n) {
         const bool served = slots_served(r, before, left);
         takes = served && r.delta;
-        owners[i] = owner_of(r, first, end, before, left);
+        owners[i] = owner_of(A, r, first, end, before, left);
         s_before[i] = (uint32_t)before;   // (a request asks for at most kOneTokens pages)
         A.len_out[i] = served ? r.new_len : r.len;
         A.held_out[i] = served ? r.held + r.delta : r.held;
@@ -395,7 +409,7 @@ __global__ __launch_bounds__(kApplyThreads) void cache_trim_kernel(CacheArgs A, 
     if (i >= A.n) return;
     const PlanRec r = recs[i];
     const u64 before = base + r.before;
-    const bool served = trim_served(r, before, left, A.n_pages);
+    const bool served = trim_served(r, before, left, A.n_pages) && (r.delta == 0 || kept_within(A, r, true, before, left));   // (one left alone may hold anything)
     if (lane_id() == 0) {
         A.len_out[i] = served ? r.new_len : r.len;
         A.held_out[i] = served ? r.held - r.delta : r.held;

@@ -193,8 +193,8 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const int32_t*
 #pragma unroll
     for (int k = 0; k < ROUNDS; k++) {
         const uint64_t i = lo + (uint64_t)k * 64 + lane;
-        if (i < n) {
-            const uint32_t at = cnt[w][(key[k] >> shift) & mask] + rank[k];
+        const uint32_t at = cnt[w][(key[k] >> shift) & mask] + rank[k];
+        if (i < n && at < n) {   // (always, unless the ids or the workspace change under the call)
             keys_out[at] = key[k];
             pos_out[at] = FIRST ? (uint32_t)i : poss[i];
         }
@@ -255,7 +255,8 @@ __global__ __launch_bounds__(kSortThreads) void sort_rank_kernel(const int32_t* 
 // from one wave of a workgroup to the next meet in LDS; a run that crosses the workgroup's border leaves its part in the
 // workspace: part[2 b] of the run that came in from the workgroup before, part[2 b + 1] of the run that starts here and goes
 // on; grad_join_kernel adds these up at the workgroup where the run starts.  Nothing is added by atomics: the same ids give the
-// same bits.
+// same bits.  What comes from the workspace is held to the arrays' bounds, so that a workspace shared by mistake gives wrong sums and
+// no access outside them.
 //
 // Bound by memory: 65,536 ids onto 32-bit gradients of 128,256 x 4,096 read 0.81 GB and write 0.32 GB (counters: the distinct rows,
 // each once, and 4 % for the parts) in 250 us, 4.5 TB/s; a copy of 4 GiB reaches 4.7.  Rows in flight, us of the whole call: two 308,
@@ -319,7 +320,7 @@ __global__ __launch_bounds__(kGradThreads) void grad_walk_kernel(GradWalk P, con
         if (threadIdx.x < kZeroRows) named[threadIdx.x] = 0;
         if (wave_id() < 2) ends[wave_id()] = first_key(keys, P.n, r0 + wave_id() * kZeroRows);
         __syncthreads();
-        for (uint64_t i = ends[0] + threadIdx.x; i < ends[1]; i += kGradThreads) named[keys[i] - r0] = 1;
+        for (uint64_t i = ends[0] + threadIdx.x; i < ends[1]; i += kGradThreads) if (keys[i] - r0 < kZeroRows) named[keys[i] - r0] = 1;
         __syncthreads();
         zero_rows<SMALL>(table, P.table_stride, rows, dim, r0, named);
         return;
@@ -330,11 +331,12 @@ __global__ __launch_bounds__(kGradThreads) void grad_walk_kernel(GradWalk P, con
     const uint32_t w = (uint32_t)__builtin_amdgcn_readfirstlane((int)wave_id());
     const uint64_t c = block * kGradWaves + w, lo = c * P.chunk < P.n ? c * P.chunk : P.n;
     const uint32_t vec = (uint32_t)(blockIdx.x - block * P.tiles) * 64 + lane_id(), len = lo + P.chunk < P.n ? P.chunk : (uint32_t)(P.n - lo);
-    const uint32_t key = (uint32_t)lane_id() < len ? keys[lo + lane_id()] : ~0u, pos = (uint32_t)lane_id() < len ? poss[lo + lane_id()] : 0;
+    const uint32_t key = (uint32_t)lane_id() < len ? keys[lo + lane_id()] : ~0u, pos = (uint32_t)lane_id() < len ? min(poss[lo + lane_id()], (uint32_t)P.n - 1) : 0;
     // the key behind the chunk, and the run that came in, if one did
     const uint32_t behind = lo + len < P.n ? keys[lo + len] : ~0u, first = of_lane(key, 0), in_front = lo && len ? keys[lo - 1] : ~0u;
     const uint32_t came_in = first == in_front && first < rows ? first : ~0u;
-    const uint32_t used = (uint32_t)__popcll(__ballot(key < rows));   // ids that are no rows come last
+    const u64 none = __ballot(key >= rows);                           // ids that are no rows come last
+    const uint32_t used = none ? (uint32_t)__builtin_ctzll(none) : 64;
     const bool mine = vec * 8 < dim;
     const Cols at = cols_of(mine ? vec : 0, dim);
     F8 sum = 0.f, head = 0.f;

@@ -5,7 +5,8 @@ set -e
 cd "$(dirname "$0")/../tokenizer_amd/csrc"
 U=${3:-l3_tile}
 mkdir -p ../lib/variants
-/opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -Wno-unused-function -I../../include $2 -c -o ../lib/variants/k_$1.o $U.hip
+case $U in l3_embed|l3_cache|l3_verify) FLOAT="-Xclang -target-feature -Xclang -packed-fp32-ops";; *) FLOAT=;; esac   # as in the Makefile
+/opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -Wno-unused-function -I../../include $FLOAT $2 -c -o ../lib/variants/k_$1.o $U.hip
 OBJS=$(ls ../lib/obj/*.o | grep -v "/$U.o")
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o ../lib/variants/libl3hip_$1.so $OBJS ../lib/variants/k_$1.o
 rm -f ../lib/variants/k_$1.o
