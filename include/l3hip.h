@@ -191,7 +191,8 @@ int l3_embed_grad(l3_ctx* ctx, const int32_t* d_ids, uint64_t n_ids, const uint6
  * 0, 1, 2, .. for a step of one token each).  Pages that are missing are taken off the end of the pool, in order of the
  * requests, and entered in the table.  The j-th new token of request i, at t = new_off[i] + j, gets pos[t] = len[i] + j and
  * slots[t] = table[i][pos / page_size] * page_size + pos % page_size.  len_out, held_out and n_free_out are the state behind
- * the step.  Slots and positions at or behind new_off[n_seqs] (there are cap of them) are left as they were.
+ * the step.  Slots and positions in front of new_off[0], and at or behind new_off[n_seqs] (there are cap of them), are left as
+ * they were: a batch may be served in several calls, each with a slice of its offsets.
  * l3_cache_trim: request i keeps its first min(keep[i], len[i]) tokens and the pages these need; the others go to the end of
  * the pool, in order of the requests.  keep[i] < 0: the request is left as it is.
  *
@@ -201,7 +202,8 @@ int l3_embed_grad(l3_ctx* ctx, const int32_t* d_ids, uint64_t n_ids, const uint6
  *                  pool would hold more than n_pages)
  *   L3_CACHE_ROW   more tokens than max_pages pages, or 2^31 - 1, hold
  *   L3_CACHE_BAD   new_off descends or ends behind cap; len, held or *n_free is negative, or more than there can be (where new_off
- *                  descends, the table entries of requests that claim the same tokens are not to be relied on)
+ *                  descends, the table entries of requests that claim the same tokens are not to be relied on, nor the slots of
+ *                  requests that lie in front of new_off[0])
  *   L3_CACHE_PAGE  (slots) a page outside [0, n_pages): the slots of the tokens on it are -1, nothing else changes
  * d_work: l3_cache_workspace(n_seqs) bytes.  n_seqs <= 2^20. */
 #define L3_CACHE_POOL 1u

@@ -495,6 +495,77 @@ def test_cache_offsets_that_cannot_be(ctx, torch):
         assert (d_slots[cap:] == -7).all() and (d_pos[cap:] == -7).all()
 
 
+# (by one workgroup, by two launches with two tokens a thread, with four)
+FIRST_OFFSETS = [(1, 1, 5, 3), (4, 7, 3, 0), (200, 300, 4, 5), (300, 513, 5, 1), (1000, 2049, 2, 0), (5, 5000, 40, 3), (1, 4097, 1, 0), (3, 511, 3000, 0),
+                 (2000, 1, 3, 2), (3000, 777, 3, 0), (20000, 1023, 2, 1), (50, (1 << 20) + 13, 30, 7), (2, (1 << 20) - 1023, 2500, 0)]
+
+
+def _prefilled(torch, cap):
+    """Slots and positions that no call writes: (lists, the same on the GPU)"""
+    slots, pos = [-1000 - t for t in range(cap)], [-30000000 - t for t in range(cap)]
+    return slots, pos, torch.tensor(slots, dtype=torch.int64, device="cuda"), torch.tensor(pos, dtype=torch.int32, device="cuda")
+
+
+def _holds(torch, buf, values):
+    return torch.equal(buf, torch.tensor(values, dtype=buf.dtype, device="cuda"))
+
+
+@pytest.mark.parametrize("n, first, most, more_cap", FIRST_OFFSETS)
+def test_cache_slots_in_front_of_the_first_offset(ctx, torch, n, first, most, more_cap):
+    """Offsets that do not begin at 0, as a slice of a larger batch's: what is in front of them is not the call's."""
+    import random
+    rng = np.random.default_rng(n + first)
+    page, max_pages, n_pages = 16, max(4, -(-most // 16) + 2), 3 * n + 400 + n * -(-most // 16)
+    state = (*random_cache(random.Random(n), n, page, 2, n_pages, full=0.2), page, n_pages, max_pages)
+    state = (state[0], state[1], [r + [-5] * (max_pages - 2) for r in state[2]], *state[3:])
+    off = (first + np.append(0, np.cumsum(rng.integers(0, most + 1, n)))).tolist()
+    cap = off[-1] + more_cap
+    dev, model = DeviceCache(torch, state), ref.Cache(*state)
+    slots, pos, d_slots, d_pos = _prefilled(torch, cap)
+    status = model.slots(off, cap, slots, pos)
+    dev.slots(ctx, torch.tensor(off, dtype=torch.int64, device="cuda"), d_slots, d_pos, cap)
+    assert _holds(torch, d_slots, slots) and _holds(torch, d_pos, pos) and int(dev.status[0]) == status
+    assert dev.state() == (model.length, model.held, model.table, model.free, model.n_free)
+
+
+@pytest.mark.parametrize("n, k, most", [(20, 7, 30), (3000, 1200, 5), (40, 11, 60000)])
+def test_cache_slots_of_one_batch_in_two_calls(ctx, torch, n, k, most):
+    """Two groups of requests, each with a pool of its own, and one array of slots: slices of one batch's offsets, in either order."""
+    rng = np.random.default_rng(n)
+    page = 16
+    off = np.append(0, np.cumsum(rng.integers(0, most + 1, n)))
+    cap = int(off[-1])
+    d_off = torch.from_numpy(off).cuda()
+    for order in ((0, 1), (1, 0)):
+        slots, pos, d_slots, d_pos = _prefilled(torch, cap)
+        for g in order:
+            part = slice(0, k + 1) if g == 0 else slice(k, n + 1)
+            m = part.stop - part.start - 1
+            most_pages = -(-most // page)
+            state = ([0] * m, [0] * m, [[-5] * most_pages] * m, list(range(m * most_pages)), m * most_pages, page, m * most_pages, most_pages)
+            dev, model = DeviceCache(torch, state), ref.Cache(*state)
+            end = int(off[part.stop - 1])
+            assert model.slots(off[part].tolist(), end, slots, pos) == 0
+            dev.slots(ctx, d_off[part], d_slots, d_pos, end)
+            assert int(dev.status[0]) == 0 and dev.state() == (model.length, model.held, model.table, model.free, model.n_free)
+        assert _holds(torch, d_slots, slots) and _holds(torch, d_pos, pos) and min(pos) >= 0
+
+
+@pytest.mark.parametrize("front", [0, 5000])
+def test_cache_slots_where_the_first_offset_is_not_the_smallest(ctx, torch, front):
+    """Offsets that descend below the first one: its request is not served, the tokens of those behind it have their slots."""
+    state = ([5, 0, 3, 0], [1, 0, 1, 0], [[4, -5], [-5, -5], [6, -5], [-5, -5]], list(range(10, 30)) + [-5] * 12, 20, 8, 32, 2)
+    for off in ([5, 2, 4, 4, 6], [9, 1, 1, 3, 4]):
+        off = [front + x for x in off]
+        cap = off[-1] + 3 if off[0] < off[-1] else off[0]
+        dev, model = DeviceCache(torch, state), ref.Cache(*state)
+        slots, pos, d_slots, d_pos = _prefilled(torch, cap)
+        status = model.slots(off, cap, slots, pos)
+        dev.slots(ctx, torch.tensor(off, dtype=torch.int64, device="cuda"), d_slots, d_pos, cap)
+        assert status == ref.BAD == int(dev.status[0]) and _holds(torch, d_slots, slots) and _holds(torch, d_pos, pos)
+        assert dev.state() == (model.length, model.held, model.table, model.free, model.n_free)
+
+
 @pytest.mark.parametrize("n_free", [-1, -2 ** 31, 33, 2 ** 31 - 1])
 def test_cache_counts_that_cannot_be(ctx, torch, n_free):
     state = ([5, 16], [1, 2], [[4, -5, -5], [6, 7, -5]], list(range(32)), n_free, 8, 32, 3)

@@ -118,6 +118,10 @@ __device__ __forceinline__ uint64_t request_probe(const uint64_t* off, uint64_t 
     const uint64_t at = (uint64_t)lane_id() * ((n + 63) / 64);
     return at < n ? off[at] : ~0ull;
 }
+__device__ __forceinline__ uint64_t first_lane64(uint64_t v) {
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)), lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+    return (uint64_t)hi << 32 | lo;
+}
 __device__ __forceinline__ uint64_t request_of(const uint64_t* off, uint64_t n, uint64_t t, uint64_t probe) {
     uint64_t lo = 0, len = n, step = (n + 63) / 64;
     u64 m = __ballot(probe <= t && (uint64_t)lane_id() * step < n);
@@ -164,12 +168,13 @@ __device__ __forceinline__ Owner owner_of(const CacheArgs& A, const PlanRec& r, 
     w.held = served ? r.held : -1;
     return w;
 }
+__device__ __forceinline__ bool owns(const Owner& w, uint64_t t) { return t >= w.first && t < w.end; }
 // Slot and position of token t of request i.  ENTER: it enters its page, if that is beyond the first kGroupPages new ones.
 template <bool ENTER>
 __device__ __forceinline__ uint32_t place_token(const CacheArgs& A, PageDiv D, const Owner& w, uint64_t i, uint64_t t, int64_t* slot, int32_t* pos) {
     *slot = -1;
     *pos = -1;
-    if (w.held < 0 || t < w.first || t >= w.end) return 0;
+    if (w.held < 0 || !owns(w, t)) return 0;
     const uint32_t q = (uint32_t)w.len + (uint32_t)(t - w.first), p = D.of(q), in = q - p * A.page;
     // (pages that are new may not be in the table yet)
     int32_t* entry = A.table + i * A.table_stride + p;
@@ -179,6 +184,10 @@ __device__ __forceinline__ uint32_t place_token(const CacheArgs& A, PageDiv D, c
     *slot = slot_of(id, in, A.page, A.n_pages);
     return *slot < 0 ? (uint32_t)kCachePage : 0u;
 }
+
+// A token in front of the first offset is no request's, and what stands there is not the call's (a step that has a slice of a larger
+// batch's offsets).  Unless it is one's after all: offsets that descend may have a request below the first one.
+__device__ __forceinline__ bool not_the_calls(uint64_t first, const Owner& w, uint64_t t) { return t < first && !owns(w, t); }
 
 // Tokens in blocks of 256 PER, PER neighbours a thread; the requests of a block are found once and kept in LDS (more than there are
 // tokens in a block only where many requests have no new token: then every token looks for its own).  Two tokens a thread / four,
@@ -263,7 +272,7 @@ __global__ __launch_bounds__(kApplyThreads) void cache_slots_kernel(CacheArgs A,
     } else {
         const uint64_t t0 = (uint64_t)(blockIdx.x - 1 - request_blocks) * kTokenBlock;
         uint64_t total = A.off[A.n];
-        const uint64_t probe = request_probe(A.off, A.n);
+        const uint64_t probe = request_probe(A.off, A.n), first = first_lane64(probe);   // (lane 0 has loaded off[0])
         if (total > A.cap) total = A.cap;
         if (t0 >= total) return;
         const uint64_t last = (t0 + kTokenBlock < total ? t0 + kTokenBlock : total) - 1;
@@ -292,6 +301,7 @@ __global__ __launch_bounds__(kApplyThreads) void cache_slots_kernel(CacheArgs A,
         const uint64_t t = t0 + (uint64_t)threadIdx.x * PER;
         int64_t slot[PER];
         int32_t pos[PER];
+        bool stays[PER];
         if (many <= kOwners) {
             for (uint64_t k = threadIdx.x; k < many; k += kApplyThreads) owners[k] = load_owner(a0 + k);
             __syncthreads();
@@ -300,20 +310,23 @@ __global__ __launch_bounds__(kApplyThreads) void cache_slots_kernel(CacheArgs A,
 #pragma unroll
             for (int j = 0; j < PER; j++) {
                 while (k + 1 < (uint32_t)many && owners[k + 1].first <= t + j) k++;
+                stays[j] = not_the_calls(first, owners[k], t + j);
                 if (t + j <= last) bits |= place_token<true>(A, D, owners[k], a0 + k, t + j, &slot[j], &pos[j]);
             }
         } else {
             for (int j = 0; j < PER; j++) {
                 uint64_t a = 0, b = A.n;
                 while (b - a > 1) { const uint64_t m = (a + b) / 2; if (A.off[m] <= t + j) a = m; else b = m; }
-                if (t + j <= last) bits |= place_token<true>(A, D, load_owner(a), a, t + j, &slot[j], &pos[j]);
+                const Owner w = load_owner(a);
+                stays[j] = not_the_calls(first, w, t + j);
+                if (t + j <= last) bits |= place_token<true>(A, D, w, a, t + j, &slot[j], &pos[j]);
             }
         }
-        if (t + PER <= last + 1) {
+        if (t >= first && t + PER <= last + 1) {
             __builtin_memcpy(A.slots + t, slot, sizeof slot);
             __builtin_memcpy(A.pos + t, pos, sizeof pos);
         } else {
-            for (int j = 0; j < PER; j++) if (t + j <= last) { A.slots[t + j] = slot[j]; A.pos[t + j] = pos[j]; }
+            for (int j = 0; j < PER; j++) if (t + j <= last && !stays[j]) { A.slots[t + j] = slot[j]; A.pos[t + j] = pos[j]; }
         }
     }
     if (bits) atomicOr(A.status, bits);
@@ -384,6 +397,7 @@ __global__ __launch_bounds__(THREADS) void cache_slots_one_kernel(CacheArgs A, P
         int64_t slot;
         int32_t pos;
         const uint32_t bits = place_token<false>(A, D, owners[k], k, t, &slot, &pos);
+        if (not_the_calls(owners[0].first, owners[k], t)) continue;
         A.slots[t] = slot;
         A.pos[t] = pos;
         if (bits) atomicOr(&s_status, bits);
