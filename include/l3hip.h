@@ -158,7 +158,8 @@ int l3_last_counters(l3_ctx* ctx, uint64_t* out, int cap);
  * calls, a stream of the context).  They allocate nothing, keep nothing in the context, call nothing a stream capture forbids,
  * leave the current device as it was, and may run at the same time on several streams and threads, each with a workspace of
  * its own.  Workspaces need not be cleared, are aligned to 16 bytes and may be used again by the next call on the same
- * stream; two captured graphs that may run at the same time need two.  Outputs must not overlap inputs unless said so.
+ * stream; two captured graphs that may run at the same time need two; one for the largest sizes is enough for all smaller ones.
+ * Outputs must not overlap inputs unless said so.
  * What the host can see is refused with L3_E_INVALID_ARG before anything is queued; what only the device can see is answered as
  * each call says.  Strides are in elements, at least the row's length, and need no alignment beyond the element's own. */
 #define L3_F32 0

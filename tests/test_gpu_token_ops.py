@@ -356,6 +356,22 @@ def test_grad_same_bits(ctx, torch):
     assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
 
 
+def test_grad_batches_of_every_size_on_the_largest_ones_workspace(ctx, torch):
+    """One workspace, sized once: the last batches of an epoch are smaller."""
+    rng = np.random.default_rng(12)
+    rows, dim, most = 700, 2048, 19000
+    need = capi.embed_grad_workspace(most, dim)
+    work = torch.empty(need, dtype=torch.uint8, device="cuda")
+    dy = torch.from_numpy(rng.integers(-8, 9, (most, dim))).cuda().bfloat16()
+    ids = torch.from_numpy(_ids(rng, most, rows)).cuda()
+    for n in (most, 18432, 18400, 9217, 9215, 8192, 4600, 2100, 1):
+        got = torch.full((rows, dim), -7.0, device="cuda")
+        ctx.embed_grad(ids.data_ptr(), n, dy.data_ptr(), BF16, dim, rows, dim, got.data_ptr(), F32, dim, work.data_ptr(), need)
+        there = ((ids[:n] >= 0) & (ids[:n] < rows))[:, None]
+        want = torch.zeros(rows, dim, device="cuda").index_add_(0, ids[:n].clamp(0, rows - 1).long(), dy[:n].float() * there)
+        assert torch.equal(got, want), n                   # (whole numbers below 2^24 add up without rounding)
+
+
 # ---- paged cache --------------------------------------------------------------------------------------------------
 class DeviceCache:
     """A cache's state on the GPU, its calls in place or to other arrays."""

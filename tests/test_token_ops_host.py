@@ -149,6 +149,38 @@ def test_workspace_sizes(lib):
         capi.cache_workspace(2 ** 20 + 1)
 
 
+def test_a_workspace_for_the_largest_batch_is_enough_for_all(lib):
+    """Sizes never shrink as n or dim grow (a smaller batch on the largest one's workspace must not be refused), and hold what the
+    kernels lay out in them."""
+    lib.l3t_grad_pieces.restype, lib.l3t_grad_pieces.argtypes = None, [_Q, _Q, _P]
+    rng = random.Random(2)
+    edges = {m + d for m in (512, 1024, 2048, 4096, 4600, 8192, 18400, 18432, 36864, 65536, 69632, 135168, 262144, 1 << 20, 1 << 24) for d in (-1, 0, 1)}
+    # (where the chunk changes: n * ceil(dim / 512) at 9, 17 and 33 times 4,096)
+    edges |= {-(-k * 4096 // t) + d for k in (9, 17, 33) for t in range(1, 34) for d in (-1, 0, 1)}
+    ns = sorted({n for n in edges | set(range(0, 3000, 37)) | {int(10 ** rng.uniform(0, 7.22)) for _ in range(300)} if 0 <= n <= 1 << 24})
+    dims = sorted({1, 7, 8, 9, 64, 511, 512, 513, 1001, 1024, 1025, 2048, 4095, 4096, 4097, 8192, 16000, 65536, 1 << 20, 1 << 24})
+    pieces = np.zeros(4, np.uint64)
+    below = [0] * len(ns)
+    for dim in dims:
+        size = [lib.l3t_grad_work(n, dim) for n in ns]
+        assert all(a <= b for a, b in zip(size, size[1:])), dim
+        assert all(a <= b for a, b in zip(below, size)), dim
+        below = size
+        for n in ns:
+            lib.l3t_grad_pieces(n, dim, pieces.ctypes.data)
+            assert pieces[0] <= pieces[1] and pieces[2] <= pieces[3] == lib.l3t_grad_work(n, dim), (n, dim)
+    for n, dim in ((4600, 4096), (18400, 1024), (65536, 64), (262144, 64), (512, 2048)):
+        assert _check(lib, "grad", n=n, dim=dim, grad_stride=dim, table_stride=dim, work_bytes=lib.l3t_grad_work(2 * n, dim)) is None
+    ns = sorted({int(2 ** rng.uniform(0, 20)) for _ in range(500)} | {0, 1, 1023, 1024, 1025, 1 << 20})
+    size = [lib.l3t_cache_work(n) for n in ns]
+    assert all(a <= b for a, b in zip(size, size[1:]))
+    below = [0] * len(ns)
+    for vocab in (1, 2047, 2048, 2049, 128256, 2 ** 31 - 1):
+        size = [lib.l3t_verify_work(n, vocab) for n in ns]
+        assert all(a <= b for a, b in zip(size, size[1:])) and all(a <= b for a, b in zip(below, size))
+        below = size
+
+
 # ---- the paged cache ----------------------------------------------------------------------------------------------
 def random_cache(rng, n, page, max_pages, n_pages, full=0.5):
     """A sane state: (length, held, table, free, n_free); entries that mean nothing hold -5."""

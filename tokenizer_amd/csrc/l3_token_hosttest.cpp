@@ -12,6 +12,14 @@ const char* l3t_check_embed_grad(const EmbedGradArgs* A) { return check_embed_gr
 const char* l3t_check_cache(const CacheArgs* A, int trim) { return check_cache(*A, trim != 0); }
 const char* l3t_check_verify(const VerifyArgs* A) { return check_verify(*A); }
 uint64_t l3t_grad_work(uint64_t n, uint64_t dim) { return grad_work(n, dim).total; }
+// where the counts and the parts of a gradient's workspace end, and where the next piece begins
+void l3t_grad_pieces(uint64_t n, uint64_t dim, uint64_t* out) {
+    const GradWork w = grad_work(n, dim);
+    out[0] = w.hist + sort_tiles(n) * kSortBins * 4;
+    out[1] = w.part;
+    out[2] = w.part + 2 * w.blocks * w.dim8 * 4;
+    out[3] = w.total;
+}
 uint64_t l3t_cache_work(uint64_t n) { return cache_work(n).total; }
 uint64_t l3t_verify_work(uint64_t n, uint64_t vocab) { return verify_work(n, vocab).total; }
 

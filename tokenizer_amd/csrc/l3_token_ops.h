@@ -87,6 +87,23 @@ inline uint32_t grad_chunk(uint64_t n, uint64_t dim) {
     while (c < 64 && c < want) c *= 2;
     return c;
 }
+// The tiles and the parts take up what the largest of all calls of at most n ids and dim columns needs, so that a workspace for the largest
+// batch is enough for every smaller one: tiles and chunks double in size where n passes a limit, and what they leave halves.
+//   tiles   those of n, or of the limits that n has passed.
+//   parts   2 blocks dim8, blocks = ceil(n / (4 chunk)): with the smallest chunk at most 2 ceil(n / 32) dim8.  The largest chunk's grow with
+//           n and dim.  A chunk c below it means want <= c, that is n ceil(dim / 512) < (c + 1) kGradWalkers, so n dim8 <= 512 (c + 1)
+//           kGradWalkers and blocks dim8 <= n dim8 / (4 c) + dim8 <= 128 (1 + 1 / 8) kGradWalkers + dim8.
+inline uint64_t sort_tiles_most(uint64_t n) {
+    const uint64_t limits[] = {65536, 262144};
+    uint64_t most = sort_tiles(n);
+    for (const uint64_t limit : limits) if (n > limit && sort_tiles(limit) > most) most = sort_tiles(limit);
+    return most;
+}
+inline uint64_t grad_parts_most(uint64_t n, uint64_t dim8) {
+    const uint64_t few = (n + 8 * kGradWaves - 1) / (8 * kGradWaves) * dim8, many = (n + 64 * kGradWaves - 1) / (64 * kGradWaves) * dim8;
+    const uint64_t between = 144 * kGradWalkers + dim8, most = many > between ? many : between;
+    return 2 * (few < most ? few : most);
+}
 struct GradWork { uint64_t keys0, pos0, keys1, pos1, hist, part, total; uint32_t chunk; uint64_t blocks, dim8; };
 inline GradWork grad_work(uint64_t n, uint64_t dim) {
     GradWork w;
@@ -96,8 +113,8 @@ inline GradWork grad_work(uint64_t n, uint64_t dim) {
     uint64_t at = 0;
     auto take = [&](uint64_t b) { const uint64_t p = at; at += align256(b); return p; };
     w.keys0 = take(4 * n); w.pos0 = take(4 * n); w.keys1 = take(4 * n); w.pos1 = take(4 * n);
-    w.hist = take(sort_tiles(n) * kSortBins * 4);
-    w.part = take(2 * w.blocks * w.dim8 * 4);
+    w.hist = take(sort_tiles_most(n) * kSortBins * 4);
+    w.part = take(grad_parts_most(n, w.dim8) * 4);
     w.total = at ? at : 256;
     return w;
 }
