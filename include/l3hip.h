@@ -53,7 +53,9 @@ int l3_create(const void* vocab_b64, size_t vocab_len, const void* merges_b64, s
 int l3_create_ex(const void* vocab_b64, size_t vocab_len, const void* merges_b64, size_t merges_len,
                  const char* const* special_tokens, size_t n_special, int device, l3_ctx** out);
 void l3_destroy(l3_ctx* ctx);
-/* text of the last error on this context (ctx == NULL: of the last failed l3_create on this thread) */
+/* text of the last error on this context (ctx == NULL: of the last failed l3_create on this thread).  The operators on token ids
+ * may fail on several threads at once: their text is there for the thread that made the call, until a later call of that thread
+ * fails.  May be called at any time; a context's texts stay readable until it is destroyed. */
 const char* l3_last_error(const l3_ctx* ctx);
 
 /* Tokenizer.Encode / EncodeBytes / AppendTokens (tokenizer.go:217-330) for a BATCH of documents.
@@ -160,8 +162,8 @@ int l3_last_counters(l3_ctx* ctx, uint64_t* out, int cap);
  * its own.  Workspaces need not be cleared, are aligned to 16 bytes and may be used again by the next call on the same
  * stream; two captured graphs that may run at the same time need two; one for the largest sizes is enough for all smaller ones.
  * Outputs must not overlap inputs unless said so.
- * What the host can see is refused with L3_E_INVALID_ARG before anything is queued; what only the device can see is answered as
- * each call says.  Strides are in elements, at least the row's length, and need no alignment beyond the element's own. */
+ * What the host can see is refused with L3_E_INVALID_ARG before anything is queued (l3_last_error, on the same thread, says why);
+ * what only the device can see is answered as each call says.  Strides are in elements, at least the row's length, and need no alignment beyond the element's own. */
 #define L3_F32 0
 #define L3_F16 1
 #define L3_BF16 2

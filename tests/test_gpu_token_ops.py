@@ -1064,6 +1064,50 @@ def test_refusals_leave_the_context_usable(ctx, torch):
     assert torch.equal(out, table[ids.long()])
 
 
+def test_refusals_on_two_threads_have_their_own_texts(ctx, torch):
+    import threading
+    at = torch.zeros(64, device="cuda").data_ptr()
+    wrong = []
+
+    def go(dim, rows, word):
+        for _ in range(3000):
+            try:
+                ctx.embed(at, 1, at, F32, rows, dim, dim, at, F32, dim)
+                wrong.append("taken")
+            except capi.L3Error as e:
+                if e.code != capi.L3_E_INVALID_ARG or word not in str(e):
+                    wrong.append(str(e))
+
+    threads = [threading.Thread(target=go, args=a) for a in ((0, 1, "dim"), (1, 0, "n_rows"), (1, 2 ** 40, "n_rows"))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[:3]
+
+
+def test_refusals_do_not_wait_for_a_batch(ctx, torch):
+    """An encode call of another thread holds the context while its batch runs; a refused operator returns meanwhile.  With a
+    batch of tens of milliseconds and refusals of some ten microseconds there is room for thousands; where each waits there are two
+    for a batch at most."""
+    import threading
+    text = np.frombuffer(b"some words, 123 of them\n" * (1 << 21), dtype=np.uint8)      # 48 MiB
+    off = np.arange(0, len(text) + 1, 1 << 16, dtype=np.uint64)
+    off[-1] = len(text)
+    ctx.encode_batch(text, off)
+    at = torch.zeros(64, device="cuda").data_ptr()
+    batches = 6
+    side = threading.Thread(target=lambda: [ctx.encode_batch(text, off) for _ in range(batches)])
+    side.start()
+    refused = 0
+    while side.is_alive():
+        with pytest.raises(capi.L3Error):
+            ctx.embed(at, 1, at, 9, 1, 1, 1, at, F32, 1)
+        refused += 1
+    side.join()
+    assert refused > 10 * batches, refused
+
+
 # ---- together -----------------------------------------------------------------------------------------------------
 def test_from_text_to_text(ctx, torch, oracle):
     """Prompts are encoded, take pages, are looked up; drafts are verified, what was not accepted is trimmed, the answers decoded; and

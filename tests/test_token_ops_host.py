@@ -181,6 +181,87 @@ def test_a_workspace_for_the_largest_batch_is_enough_for_all(lib):
         below = size
 
 
+# ---- error texts --------------------------------------------------------------------------------------------------
+@pytest.fixture
+def texts(lib):
+    """make() -> (assign(text), leave(what, more), text()) of a context's error texts"""
+    lib.l3t_err_new.restype, lib.l3t_err_delete.argtypes = _P, [_P]
+    lib.l3t_err_assign.argtypes, lib.l3t_err_leave.argtypes = [_P, C.c_char_p], [_P, C.c_char_p, C.c_char_p]
+    lib.l3t_err_text.restype, lib.l3t_err_text.argtypes = _P, [_P]
+    made = []
+
+    def make():
+        e = lib.l3t_err_new()
+        made.append(e)
+        return lambda t: lib.l3t_err_assign(e, t), lambda w, m=b"": lib.l3t_err_leave(e, w, m), lambda: C.string_at(lib.l3t_err_text(e)), e
+    yield make
+    for e in made:
+        lib.l3t_err_delete(e)
+
+
+def test_error_texts_of_one_thread(lib, texts):
+    """The last error of the thread's own calls, whatever kind of call it was; nothing that was handed out changes."""
+    assign, leave, text, e = texts()
+    assign2, leave2, text2, _ = texts()
+    assert text() == text2() == b""
+    assign(b"encode")
+    assert text() == b"encode"
+    first = lib.l3t_err_text(e)
+    leave(b"launch: ", b"reason")
+    leave2(b"other")
+    assert text() == b"launch: reason" and text2() == b"other"
+    leave(b"again")
+    assert text() == b"again"
+    for i in range(3000):
+        assign(b"encode %d" % (i % 50))
+    assert text() == b"encode 49" and text2() == b"other" and C.string_at(first) == b"encode"
+    assign2(b"")
+    assert text2() == b""
+
+
+def test_error_texts_of_a_context_are_not_the_next_ones(lib, texts):
+    """A context that comes to lie where one was destroyed has none of its texts."""
+    for _ in range(200):
+        e = lib.l3t_err_new()
+        assert C.string_at(lib.l3t_err_text(_P(e))) == b""
+        lib.l3t_err_leave(_P(e), b"gone", b"")
+        lib.l3t_err_delete(_P(e))
+
+
+def test_error_texts_of_threads_that_fail_at_the_same_time(lib, texts):
+    """Operators that are refused on several threads of one context while encode calls fail on another: everyone reads their own."""
+    import threading
+    assign, leave, text, e = texts()
+    wrong, stop = [], threading.Event()
+
+    def refused(k):
+        for i in range(4000):
+            mine = b"thread %d, call %d " % (k, i % 7) + b"x" * (20 * k)
+            leave(b"", mine)
+            if text() != mine:
+                wrong.append((k, i))
+
+    def encodes():
+        i = 0
+        while not stop.is_set():
+            i += 1
+            assign(b"batch %d: too large" % (i % 5))
+            if not text().startswith(b"batch"):
+                wrong.append(("encode", i))
+
+    threads = [threading.Thread(target=refused, args=(k,)) for k in range(4)]
+    side = threading.Thread(target=encodes)
+    side.start()
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    stop.set()
+    side.join()
+    assert not wrong, wrong[:5]
+    assert text().startswith(b"batch")        # this thread had no refused call
+
+
 # ---- the paged cache ----------------------------------------------------------------------------------------------
 def random_cache(rng, n, page, max_pages, n_pages, full=0.5):
     """A sane state: (length, held, table, free, n_free); entries that mean nothing hold -5."""

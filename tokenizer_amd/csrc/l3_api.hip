@@ -14,6 +14,7 @@
 #include <vector>
 
 #include "../../include/l3hip.h"
+#include "l3_errtext.h"
 #include "l3_kernels.h"
 #include "l3_tables.h"
 #include "l3_token_kernels.h"
@@ -132,7 +133,7 @@ struct l3_ctx {
     int n_pending = 0;
     std::unordered_map<std::string, int> special_by_name;
     std::mutex mu;
-    std::string err;
+    ErrText err;
 };
 
 namespace {
@@ -531,7 +532,7 @@ int l3_create_ex(const void* vocab_b64, size_t vocab_len, const void* merges_b64
     }
     c->device = device;
     auto fail = [&](int rc) {
-        g_create_err = c->err;
+        g_create_err = c->err.shared();
         l3_destroy(c);
         return rc;
     };
@@ -1211,7 +1212,7 @@ int l3_last_counters(l3_ctx* c, uint64_t* out, int cap) {
 struct l3_multi {
     std::vector<l3_ctx*> ctx;
     std::mutex mu;   // one batch at a time per handle
-    std::string err;
+    ErrText err;
 };
 
 int l3_partition_by_bytes(const uint64_t* doc_off, uint64_t n_docs, int world, uint64_t* cuts) {
@@ -1266,9 +1267,9 @@ int l3_multi_encode_batch(l3_multi* m, const uint8_t* text, const uint64_t* doc_
     l3_ctx* c0 = m->ctx[0];
     {
         std::lock_guard<std::mutex> l0(c0->mu);
-        if (bad_flags(c0, flags)) { m->err = c0->err; return L3_E_INVALID_ARG; }
+        if (bad_flags(c0, flags)) { m->err = c0->err.shared(); return L3_E_INVALID_ARG; }
         int rc = check_offsets_host(c0, doc_off, n_docs);
-        if (rc) { m->err = c0->err; return rc; }
+        if (rc) { m->err = c0->err.shared(); return rc; }
     }
     if (!text && doc_off[n_docs]) { m->err = "null text"; return L3_E_INVALID_ARG; }
     const int world = (int)m->ctx.size();
@@ -1320,7 +1321,12 @@ int l3_multi_encode_batch(l3_multi* m, const uint8_t* text, const uint64_t* doc_
     uint64_t sum = 0;
     for (int r = 0; r < world; r++) {
         const int rc = rcs[(size_t)r] != L3_OK ? rcs[(size_t)r] : rcs_dl[(size_t)r];
-        if (rc != L3_OK) { m->err = "device " + std::to_string(m->ctx[(size_t)r]->device) + ": " + m->ctx[(size_t)r]->err; return rc; }
+        if (rc != L3_OK) {
+            l3_ctx* c = m->ctx[(size_t)r];
+            m->err = "device " + std::to_string(c->device) + ": " + c->err.shared();
+            c->err.forget_this_threads();   // (the shard's thread has left a newer one)
+            return rc;
+        }
         sum += totals[(size_t)r];
     }
     out_off[n_docs] = sum;
@@ -1333,7 +1339,7 @@ int l3_multi_encode_batch(l3_multi* m, const uint8_t* text, const uint64_t* doc_
 
 // ---- operators on token ids ------------------------------------------------------------------------------------
 // They keep nothing in the context: its device and its error text are all they use of it.  So they do not wait for its lock
-// either (an encode call of another thread holds it while its batch runs), except to leave an error text.
+// either (an encode call of another thread holds it while its batch runs), and their error text is the calling thread's.
 namespace {
 
 static_assert(L3_F32 == kF32 && L3_F16 == kF16 && L3_BF16 == kBF16, "public element types are the kernels'");
@@ -1352,22 +1358,18 @@ struct OnDevice {
     ~OnDevice() { if (before >= 0 && before != device) (void)hipSetDevice(before); }
 };
 
-int leave_error(l3_ctx* c, int rc, const char* what, const char* more) noexcept {
-    try {
-        std::lock_guard<std::mutex> lk(c->mu);
-        c->err = std::string(what) + more;
-    } catch (...) {
-    }
-    return rc;
-}
-
 template <class Args>
 int run_op(l3_ctx* c, const Args& A, const char* wrong, hipError_t (*go)(const Args&, hipStream_t), void* stream) noexcept {
-    if (wrong) return leave_error(c, L3_E_INVALID_ARG, wrong, "");
+    if (wrong) {
+        c->err.leave_for_this_thread(wrong, "");
+        return L3_E_INVALID_ARG;
+    }
     OnDevice here(c->device);
     hipError_t e = here.e;
     if (e == hipSuccess) e = go(A, (hipStream_t)stream);
-    return e == hipSuccess ? L3_OK : leave_error(c, L3_E_HIP, "launch: ", hipGetErrorString(e));
+    if (e == hipSuccess) return L3_OK;
+    c->err.leave_for_this_thread("launch: ", hipGetErrorString(e));
+    return L3_E_HIP;
 }
 
 }  // namespace

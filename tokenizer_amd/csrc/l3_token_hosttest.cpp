@@ -1,6 +1,7 @@
-// l3_token_hosttest.cpp -- host build of l3_token_ops.h for the CPU test-suite (tests/test_token_ops_host.py): the checks the C
-// ABI makes of its arguments, the workspace sizes, and the paged cache one request after the other with the arithmetic the
-// kernels use.  A unit-test shim: nothing in the product calls it.
+// l3_token_hosttest.cpp -- host build of l3_token_ops.h and l3_errtext.h for the CPU test-suite (tests/test_token_ops_host.py): the
+// checks the C ABI makes of its arguments, the workspace sizes, the error texts, and the paged cache one request after the other
+// with the arithmetic the kernels use.  A unit-test shim: nothing in the product calls it.
+#include "l3_errtext.h"
 #include "l3_token_ops.h"
 
 using namespace l3;
@@ -22,6 +23,12 @@ void l3t_grad_pieces(uint64_t n, uint64_t dim, uint64_t* out) {
 }
 uint64_t l3t_cache_work(uint64_t n) { return cache_work(n).total; }
 uint64_t l3t_verify_work(uint64_t n, uint64_t vocab) { return verify_work(n, vocab).total; }
+
+ErrText* l3t_err_new() { return new ErrText(); }
+void l3t_err_delete(ErrText* e) { delete e; }
+void l3t_err_assign(ErrText* e, const char* text) { *e = text; }
+void l3t_err_leave(ErrText* e, const char* what, const char* more) { e->leave_for_this_thread(what, more); }
+const char* l3t_err_text(const ErrText* e) { return e->c_str(); }
 
 uint32_t l3t_page_div(uint32_t x, uint32_t page) { return page_div(page).of(x); }
 
