@@ -726,6 +726,44 @@ def test_cache_trims_of_many_pages(ctx, torch, n, most):
     assert d.tolist() == slots and p.tolist() == pos
 
 
+@pytest.mark.parametrize("n, most", [(1, 131072), (1, 131073), (1, 1000000), (3, 40001), (3, 333333), (16, 8192), (17, 8191), (256, 512), (300, 436),
+                                     (1000, 131), (1023, 128), (7, 130), (5, 131), (2, 2)])
+@pytest.mark.parametrize("room", [1.0, 0.6])
+def test_cache_trims_of_long_requests(ctx, torch, n, most, room):
+    """Few requests with very many pages and the sizes next to the rule's limits: some give all, some a few, some nothing; at 0.6 the
+    pool has no room for the later ones."""
+    rng = np.random.default_rng(n + most)
+    held = rng.integers(most // 2, most + 1, n)
+    held[n // 2] = most
+    page, n_pages = 2, int(held.sum())
+    kind = rng.integers(0, 4, n) if n > 4 else np.arange(n) % 2 * 2
+    stay = np.where(kind == 0, 0, np.where(kind == 1, held - 1, np.where(kind == 2, held // 3, held)))
+    keep = np.where(kind == 3, -1, stay * page - (stay > 0))
+    pages = rng.permutation(n_pages).astype(np.int32)
+    table = np.full((n, most), -5, np.int32)
+    at = np.append(0, np.cumsum(held))
+    for i in range(n):
+        table[i, :held[i]] = pages[at[i]:at[i + 1]]
+    give = held - stay
+    end = np.cumsum(give)
+    n_free = n_pages - int(end[-1] * room)
+    served = (give == 0) | (n_free + end <= n_pages)
+    free = np.arange(-n_pages, 0, dtype=np.int32)
+    want = free.copy()
+    for i in range(n):
+        if served[i] and give[i]:
+            want[n_free + end[i] - give[i]:n_free + end[i]] = table[i, stay[i]:held[i]]
+    d = lambda a: torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).cuda()  # noqa: E731
+    L, H, T, F, N, S, K = d(held * page), d(held), d(table), d(free), d([n_free]), d([77]), d(keep)
+    need = capi.cache_workspace(n)
+    work = torch.full((need,), 0xAB, dtype=torch.uint8, device="cuda")
+    ctx.cache_trim(K.data_ptr(), n, L.data_ptr(), H.data_ptr(), page, n_pages, T.data_ptr(), most, most, F.data_ptr(), N.data_ptr(), L.data_ptr(),
+                   H.data_ptr(), N.data_ptr(), S.data_ptr(), work.data_ptr(), need)
+    assert int(S[0]) == (0 if served.all() else ref.POOL) and int(N[0]) == n_free + int(give[served].sum())
+    assert torch.equal(F, d(want)) and torch.equal(T, d(table)) and torch.equal(H, d(np.where(served, stay, held)))
+    assert torch.equal(L, d(np.where(served & (kind != 3), np.maximum(keep, 0), held * page)))
+
+
 def test_cache_without_requests(ctx, torch):
     dev = DeviceCache(torch, ([], [], [], [1, 2, 3, 4], 3, 8, 4, 2))
     z = torch.full((4,), -7, dtype=torch.int64, device="cuda")

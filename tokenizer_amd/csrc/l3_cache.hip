@@ -201,14 +201,15 @@ constexpr uint64_t kManyTokens = 1u << 20;
 constexpr int kMaxPlans = (int)(kMaxSeqs / kPlanThreads);
 constexpr uint64_t kManyRequests = 16384;
 
-// n entries of `from`, in steps of `step` (1 or -1), to `to`, by sixteen lanes with eight in flight.
+// n entries of `from`, in steps of `step` (1 or -1), to `to`, by LANES neighbouring threads with eight in flight.
+template <int32_t LANES = kPageLanes>
 __device__ __forceinline__ void copy_pages(int32_t* to, const int32_t* from, int step, int32_t n) {
-    for (int32_t j0 = threadIdx.x % kPageLanes; j0 < n; j0 += 8 * kPageLanes) {
+    for (int32_t j0 = threadIdx.x % LANES; j0 < n; j0 += 8 * LANES) {
         int32_t page[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) page[k] = from[step * (j0 + kPageLanes * k < n ? j0 + kPageLanes * k : j0)];
+        for (int k = 0; k < 8; k++) page[k] = from[step * (j0 + LANES * k < n ? j0 + LANES * k : j0)];
 #pragma unroll
-        for (int k = 0; k < 8; k++) if (j0 + kPageLanes * k < n) to[j0 + kPageLanes * k] = page[k];
+        for (int k = 0; k < 8; k++) if (j0 + LANES * k < n) to[j0 + LANES * k] = page[k];
     }
 }
 // Places in a list for the lanes that want one; called by whole waves.
@@ -436,23 +437,27 @@ __global__ __launch_bounds__(kApplyThreads) void cache_trim_kernel(CacheArgs A, 
 }
 
 // The whole call in one workgroup: a thread for each request, which moves the first pages the request gives back itself -- after
-// drafts that were not accepted there are no more --, then sixteen lanes for each request that gives more, eight pages each in flight.
+// drafts that were not accepted there are no more --, then sixteen lanes for each request that gives more, eight pages each in flight,
+// and all threads for one that gives more than kLongPages.  By sixteen lanes / by all threads, us: one request of 131,072 pages 410 /
+// 14.5, 16 of 8,192 33 / 16, but 64 of 2,048 17 / 37 (most of the threads have nothing to do).
+//
 // In one workgroup / in two launches, us on the GPU (and 4 us less for the caller, who makes one launch): 256 requests that give
-// nothing 2.8 / 4.8, of which a tenth gives 512 pages 5.4 / 5.8, of which all do 16.8 / 5.8; 1,024 requests 3.0 / 5.6, a tenth 8.9 / 6.5,
-// all 58 / 6.8.  A step after drafts is the first of these and a batch that ends at once is rare, so the limit is where that
-// costs 11 us.
+// nothing 3.4 / 5.2, of which a tenth gives 512 pages 5.9 / 6.2, of which all do 17.4 / 6.3; 1,024 requests 3.8 / 5.9, a tenth of which
+// give 128 pages 5.7 / 6.3, all 20.7 / 6.5; 1,000 that all give 131 pages 23.4 / 6.5; 64 that all give 2,048 16.9 / 8.8; one that gives
+// 131,072 14.5 / 218.  A step after drafts is the first of these, and a batch that ends at once is rare and costs 17 us at most.
 constexpr uint64_t kOnePages = 131072, kOnePagesSmall = 1024;   // pages that the requests hold at the very most
+constexpr int32_t kLongPages = 4096;                             // (at most 32 requests of a call give more)
 
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void cache_trim_one_kernel(CacheArgs A) {
     __shared__ u64 tmp[THREADS / 64];
-    __shared__ uint32_t s_before[THREADS], s_many[THREADS], s_status, s_given, s_n_many;
+    __shared__ uint32_t s_before[THREADS], s_many[THREADS], s_status, s_given, s_n_many, s_n_long;
     __shared__ int32_t s_first[THREADS], s_delta[THREADS];
     const uint64_t i = threadIdx.x;
     const int32_t n_free = *A.n_free;
     const bool bad = n_free < 0 || (uint32_t)n_free > A.n_pages;
     const u64 left = bad ? A.n_pages : (u64)n_free;
-    if (threadIdx.x == 0) { s_status = bad ? (uint32_t)kCacheBad : 0u; s_given = 0; s_n_many = 0; }
+    if (threadIdx.x == 0) { s_status = bad ? (uint32_t)kCacheBad : 0u; s_given = 0; s_n_many = 0; s_n_long = 0; }
     PlanRec r{};
     if (i < A.n) r = plan_trim(A.len[i], A.held[i], A.keep[i], A.page, A.max_pages);
     u64 all;
@@ -476,9 +481,10 @@ __global__ __launch_bounds__(THREADS) void cache_trim_one_kernel(CacheArgs A) {
 #pragma unroll
         for (int32_t j = 0; j < kFirstPages; j++) if (j < r.delta) to[j] = page[j];
     }
-    const bool many = gives && r.delta > kFirstPages;
-    const uint32_t at = list_place(many, &s_n_many);
+    const bool many = gives && r.delta > kFirstPages, longer = gives && r.delta > kLongPages;   // (the longer ones from the list's end)
+    const uint32_t place = list_place(many && !longer, &s_n_many), from_end = list_place(longer, &s_n_long);
     if (many) {
+        const uint32_t at = longer ? THREADS - 1 - from_end : place;
         s_many[at] = (uint32_t)i;
         s_before[at] = (uint32_t)before + kFirstPages;
         s_first[at] = stay + kFirstPages;
@@ -487,6 +493,8 @@ __global__ __launch_bounds__(THREADS) void cache_trim_one_kernel(CacheArgs A) {
     __syncthreads();
     for (uint32_t x = threadIdx.x / kPageLanes; x < s_n_many; x += THREADS / kPageLanes)
         copy_pages(A.free_pages + left + s_before[x], A.table + (uint64_t)s_many[x] * A.table_stride + s_first[x], 1, s_delta[x]);
+    for (uint32_t x = THREADS - s_n_long; x < THREADS; x++)
+        copy_pages<THREADS>(A.free_pages + left + s_before[x], A.table + (uint64_t)s_many[x] * A.table_stride + s_first[x], 1, s_delta[x]);
     if (threadIdx.x == 0) {
         *A.n_free_out = bad ? n_free : n_free + (int32_t)s_given;
         *A.status = s_status;
