@@ -328,6 +328,69 @@ def test_cache_arithmetic(lib, seed):
     assert got[:5] == (model.length, model.held, model.table, model.free, model.n_free) and got[7] == status
 
 
+class PlanRec(C.Structure):
+    _fields_ = [("before", _Q), ("len", C.c_int32), ("held", C.c_int32), ("delta", C.c_int32), ("new_len", C.c_int32), ("flags", _U), ("pad", _U)]
+
+
+class Owner(C.Structure):
+    _fields_ = [("first", _U), ("end", _U), ("next", _U), ("len", C.c_int32), ("held", C.c_int32)]
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_records_of_another_call_lead_nowhere(lib, seed):
+    """Whatever a workspace holds that another call has written over, and whatever offsets stand beside it: what is served lies inside the
+    table and the pool.  Numbers near the borders of the sizes and of the types, all of them mixed."""
+    for f in ("slots", "trim"):
+        getattr(lib, "l3t_%s_served_within" % f).argtypes = [_P, _P, _Q, _Q]
+    lib.l3t_owner_of.restype, lib.l3t_owner_of.argtypes = None, [_P, _P, _Q, _Q, _Q, _Q, _P]
+    rng = random.Random(seed)
+    served = [0, 0, 0]
+    for _ in range(30000):
+        page, max_pages, n_pages = rng.choice([1, 3, 16, 1 << 20]), rng.choice([1, 5, 4096, 2 ** 31 - 1]), rng.choice([1, 40, 2 ** 20, 2 ** 31 - 1])
+        near = lambda *of: max(0, rng.choice(of) + rng.choice([-1, 0, 0, 1, 2])) % 2 ** 64  # noqa: E731
+        i32 = lambda *of: max(-2 ** 31, min(2 ** 31 - 1, rng.choice(of) + rng.choice([-1, 0, 0, 1])))  # noqa: E731
+        A = CacheArgs(n=3, page=page, n_pages=n_pages, max_pages=max_pages, table_stride=max_pages, cap=100)
+        held = i32(0, 0, 1, max_pages, 2 ** 31 - 1, -2 ** 31)
+        r = PlanRec(len=i32(0, 5, min(2 ** 31 - 1, max(held, 0) * page), 2 ** 31 - 1, -7), held=held, delta=i32(0, 0, 1, 3, held, max_pages - max(held, 0), n_pages, -4),
+                    flags=rng.choice([0, 0, 0, 0, 4, 2 ** 31]))
+        left = near(0, n_pages, n_pages // 2, n_pages, 2 ** 63)
+        before = near(0, 0, left, left - max(r.delta, 0), n_pages - left - max(r.delta, 0), 2 ** 64 - max(r.delta, 0) - 1, 2 ** 64 - 1)
+        if lib.l3t_trim_served_within(C.byref(A), C.byref(r), before, left) and r.delta:
+            served[0] += 1
+            assert 0 < r.delta <= r.held <= max_pages and left + before + r.delta <= n_pages
+        if lib.l3t_slots_served_within(C.byref(A), C.byref(r), before, left):
+            served[1] += 1
+            assert 0 <= r.held <= r.held + r.delta <= max_pages and r.delta >= 0
+            assert r.delta == 0 or before + r.delta <= left <= n_pages
+        first = near(0, 7, 99, 2 ** 32, 2 ** 63)
+        end = near(first, first + 1, first + page * max(r.delta, 0), first + page * (max(r.held, 0) + max(r.delta, 0)) - max(r.len, 0), 0, 2 ** 64 - 1,
+                   first + 2 ** 64 - max(r.len, 0))
+        w = Owner()
+        lib.l3t_owner_of(C.byref(A), C.byref(r), first, end, before, left, C.byref(w))
+        if w.held >= 0 and w.first < w.end:
+            served[2] += 1
+            for t in (w.first, w.end - 1):
+                q = w.len + t - w.first
+                assert 0 <= q < 2 ** 31 and q // page < r.held + r.delta <= max_pages, (r.len, r.held, r.delta, first, end)
+                fresh = q // page - r.held
+                assert fresh < 0 or 0 <= w.next - 1 - fresh < n_pages
+    assert min(served) > 100, served
+
+
+class Verdict(C.Structure):
+    _fields_ = [("state", C.c_int32), ("a", _U), ("p_row", _Q), ("q_row", _Q), ("token", C.c_int32), ("pad", C.c_int32)]
+
+
+def test_verdicts_of_another_call_lead_nowhere(lib):
+    A = VerifyArgs(n=3, n_draft=10, max_draft=4)
+    for state in (1, 2, 3, -1):
+        for a in (0, 4, 5, 2 ** 32 - 1):
+            for p in (0, 12, 13, 2 ** 64 - 1):
+                for q in (0, 9, 10, 2 ** 64 - 1):
+                    got = lib.l3t_verdict_within(C.byref(A), C.byref(Verdict(state=state, a=a, p_row=p, q_row=q, token=7)))
+                    assert bool(got) == (a <= 4 and p < 13 and (state != 2 or q < 10))
+
+
 def test_division_by_the_page_size(lib):
     """The product that stands for x / page, next to multiples of every page size up to 600 and of others up to 2^20."""
     lib.l3t_page_div.restype, lib.l3t_page_div.argtypes = _U, [_U, _U]

@@ -138,37 +138,6 @@ __device__ __forceinline__ uint64_t request_of(const uint64_t* off, uint64_t n, 
 
 constexpr int32_t kFirstPages = 2, kPageLanes = 16, kGroupPages = 512;
 
-// A record of the plan that would lead outside the table or the pool is not served.  The plan makes none; a workspace shared by
-// mistake may hold one.
-__device__ __forceinline__ bool kept_within(const CacheArgs& A, const PlanRec& r, bool trim, u64 before, u64 left) {
-    if (r.held < 0 || r.delta < 0 || left > A.n_pages || (uint64_t)r.held + (trim ? 0u : (uint32_t)r.delta) > A.max_pages) return false;
-    const u64 most = trim ? A.n_pages - left : left;
-    return r.delta == 0 || ((!trim || r.delta <= r.held) && before <= most && (u64)r.delta <= most - before);
-}
-__device__ __forceinline__ bool slots_served_within(const CacheArgs& A, const PlanRec& r, u64 before, u64 left) {
-    return slots_served(r, before, left) && kept_within(A, r, false, before, left);
-}
-
-// What a token needs of its request (tokens and pages are below 2^31; an offset that is not is the largest number instead).
-struct Owner {
-    uint32_t first, end;     // its new tokens
-    uint32_t next;           // free list: its first new page is at next - 1
-    int32_t len, held;       // held < 0: not served
-};
-__device__ __forceinline__ Owner owner_of(const CacheArgs& A, const PlanRec& r, uint64_t first, uint64_t end, u64 before, u64 left) {
-    // (its tokens end within its pages, so that place_token need not look at each)
-    const u64 upto = (u64)r.len + (end - first);
-    const bool served = slots_served_within(A, r, before, left) && r.len >= 0 && end >= first && upto <= kMaxCount &&
-                        upto <= ((u64)r.held + (u64)r.delta) * A.page;
-    Owner w;
-    w.first = first < ~0u ? (uint32_t)first : ~0u;
-    w.end = end < ~0u ? (uint32_t)end : ~0u;
-    w.next = served ? (uint32_t)(left - before) : 0;
-    w.len = r.len;
-    w.held = served ? r.held : -1;
-    return w;
-}
-__device__ __forceinline__ bool owns(const Owner& w, uint64_t t) { return t >= w.first && t < w.end; }
 // Slot and position of token t of request i.  ENTER: it enters its page, if that is beyond the first kGroupPages new ones.
 template <bool ENTER>
 __device__ __forceinline__ uint32_t place_token(const CacheArgs& A, PageDiv D, const Owner& w, uint64_t i, uint64_t t, int64_t* slot, int32_t* pos) {
@@ -424,7 +393,7 @@ __global__ __launch_bounds__(kApplyThreads) void cache_trim_kernel(CacheArgs A, 
     if (i >= A.n) return;
     const PlanRec r = recs[i];
     const u64 before = base + r.before;
-    const bool served = trim_served(r, before, left, A.n_pages) && (r.delta == 0 || kept_within(A, r, true, before, left));   // (one left alone may hold anything)
+    const bool served = trim_served_within(A, r, before, left);
     if (lane_id() == 0) {
         A.len_out[i] = served ? r.new_len : r.len;
         A.held_out[i] = served ? r.held - r.delta : r.held;
@@ -446,7 +415,7 @@ __global__ __launch_bounds__(kApplyThreads) void cache_trim_kernel(CacheArgs A, 
 // give 128 pages 5.7 / 6.3, all 20.7 / 6.5; 1,000 that all give 131 pages 23.4 / 6.5; 64 that all give 2,048 16.9 / 8.8; one that gives
 // 131,072 14.5 / 218.  A step after drafts is the first of these, and a batch that ends at once is rare and costs 17 us at most.
 constexpr uint64_t kOnePages = 131072, kOnePagesSmall = 1024;   // pages that the requests hold at the very most
-constexpr int32_t kLongPages = 4096;                             // (at most 32 requests of a call give more)
+constexpr int32_t kLongPages = 4096;                             // (at most 31 requests of a call give more)
 
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void cache_trim_one_kernel(CacheArgs A) {

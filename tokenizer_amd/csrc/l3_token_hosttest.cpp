@@ -32,6 +32,14 @@ const char* l3t_err_text(const ErrText* e) { return e->c_str(); }
 
 uint32_t l3t_page_div(uint32_t x, uint32_t page) { return page_div(page).of(x); }
 
+// the checks of what a kernel finds in a workspace
+int l3t_slots_served_within(const CacheArgs* A, const PlanRec* r, uint64_t before, uint64_t left) { return slots_served_within(*A, *r, before, left); }
+int l3t_trim_served_within(const CacheArgs* A, const PlanRec* r, uint64_t before, uint64_t left) { return trim_served_within(*A, *r, before, left); }
+void l3t_owner_of(const CacheArgs* A, const PlanRec* r, uint64_t first, uint64_t end, uint64_t before, uint64_t left, Owner* out) {
+    *out = owner_of(*A, *r, first, end, before, left);
+}
+int l3t_verdict_within(const VerifyArgs* A, const VerifyVerdict* R) { return verdict_within(*A, *R); }
+
 void l3t_cache_slots(const CacheArgs* P) {
     const CacheArgs& A = *P;
     const int32_t n_free = *A.n_free;

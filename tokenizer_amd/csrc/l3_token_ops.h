@@ -140,7 +140,9 @@ inline CacheWork cache_work(uint64_t n) {
 }
 
 constexpr int kVerifyChunk = 2048;   // entries of a row one workgroup adds up
-struct VerifyVerdict { int32_t state; uint32_t a; uint64_t p_row, q_row; int32_t token; int32_t pad; };   // (l3_verify.hip)
+// What became of a request's drafted tokens: all accepted, or token `a` rejected.
+enum : int { kBadRequest = 0, kDrawTarget = 1, kDrawRest = 2 };
+struct VerifyVerdict { int32_t state; uint32_t a; uint64_t p_row, q_row; int32_t token; int32_t pad; };
 struct VerifyWork { uint64_t sums, verdicts, total, chunks; };
 inline VerifyWork verify_work(uint64_t n, uint64_t vocab) {
     VerifyWork w;
@@ -268,6 +270,43 @@ L3_HD bool slots_served(const PlanRec& r, uint64_t before, uint64_t left) {
 }
 L3_HD bool trim_served(const PlanRec& r, uint64_t before, uint64_t left, uint64_t n_pages) {
     return r.flags == 0 && (r.delta == 0 || left + before + (uint64_t)r.delta <= n_pages);
+}
+// A record of the plan that would lead outside the table or the pool is not served.  The plan makes none; a workspace that two
+// calls share by mistake may hold anything.
+L3_HD bool kept_within(const CacheArgs& A, const PlanRec& r, bool trim, uint64_t before, uint64_t left) {
+    if (r.held < 0 || r.delta < 0 || left > A.n_pages || (uint64_t)r.held + (trim ? 0u : (uint32_t)r.delta) > A.max_pages) return false;
+    const uint64_t most = trim ? A.n_pages - left : left;
+    return r.delta == 0 || ((!trim || r.delta <= r.held) && before <= most && (uint64_t)r.delta <= most - before);
+}
+L3_HD bool slots_served_within(const CacheArgs& A, const PlanRec& r, uint64_t before, uint64_t left) {
+    return slots_served(r, before, left) && kept_within(A, r, false, before, left);
+}
+L3_HD bool trim_served_within(const CacheArgs& A, const PlanRec& r, uint64_t before, uint64_t left) {
+    return trim_served(r, before, left, A.n_pages) && (r.delta == 0 || kept_within(A, r, true, before, left));   // (one left alone may hold anything)
+}
+// What a token needs of its request (tokens and pages are below 2^31; an offset that is not is the largest number instead).
+struct Owner {
+    uint32_t first, end;     // its new tokens
+    uint32_t next;           // free list: its first new page is at next - 1
+    int32_t len, held;       // held < 0: not served
+};
+L3_HD Owner owner_of(const CacheArgs& A, const PlanRec& r, uint64_t first, uint64_t end, uint64_t before, uint64_t left) {
+    // (its tokens end within its pages, so that none of them need be looked at by itself)
+    const uint64_t count = end - first, upto = (uint64_t)r.len + count;
+    const bool served = slots_served_within(A, r, before, left) && r.len >= 0 && end >= first && count <= kMaxCount && upto <= kMaxCount &&
+                        upto <= ((uint64_t)r.held + (uint64_t)r.delta) * A.page;
+    Owner w;
+    w.first = first < ~0u ? (uint32_t)first : ~0u;
+    w.end = end < ~0u ? (uint32_t)end : ~0u;
+    w.next = served ? (uint32_t)(left - before) : 0;
+    w.len = r.len;
+    w.held = served ? r.held : -1;
+    return w;
+}
+L3_HD bool owns(const Owner& w, uint64_t t) { return t >= w.first && t < w.end; }
+// The same for the verification: a verdict is held to the rows there are.
+L3_HD bool verdict_within(const VerifyArgs& A, const VerifyVerdict& R) {
+    return R.a <= A.max_draft && R.p_row < A.n_draft + A.n && (R.state != kDrawRest || R.q_row < A.n_draft);
 }
 // x / page for x < 2^31 by a product: with 2^s the first power of two that is not below page, m = floor(2^(31 + s) / page) + 1 is
 // 2^(31 + s) / page + e, 0 < e <= 1, so x m / 2^(31 + s) is x / page + x e / 2^(31 + s), too large by less than 2^-s <= 1 / page.

@@ -19,8 +19,6 @@ namespace {
 
 constexpr int kVerifyThreads = 256;
 
-// What became of a request's drafted tokens.  state: kBadRequest / kDrawTarget (all accepted) / kDrawRest (token `a` rejected).
-enum : int { kBadRequest = 0, kDrawTarget = 1, kDrawRest = 2 };
 using Verdict = VerifyVerdict;
 
 // Called by a whole wave.
@@ -165,8 +163,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
     for (uint64_t i = blockIdx.x; i < A.n; i += gridDim.x) {
         const double2* S = sums + i * chunks;
         Verdict R = verdicts[i];
-        // (what comes from the workspace is held to the arrays' bounds)
-        if (R.a > A.max_draft || R.p_row >= A.n_draft + A.n || (R.state == kDrawRest && R.q_row >= A.n_draft)) R.state = kBadRequest;
+        if (!verdict_within(A, R)) R.state = kBadRequest;
         const double u = (double)A.u_draw[i];
         const double2 first = (uint64_t)lane < chunks ? S[lane] : make_double2(0, 0);   // (most vocabularies have no more chunks)
         if (threadIdx.x == 0) { s_token = 0x7FFFFFFF; s_last = -1; }
