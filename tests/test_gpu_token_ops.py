@@ -1038,6 +1038,87 @@ def test_captured_and_replayed(ctx, torch):
             assert a["cache"].state() == b["cache"].state() and int(a["cache"].status[0]) == int(b["cache"].status[0])
 
 
+# ids that are ranked / sorted by digits, requests of two launches
+@pytest.mark.parametrize("n, dim, seqs", [(3000, 1100, 1100), (9000, 136, 1500)])
+def test_captured_and_replayed_on_their_workspaces(ctx, torch, n, dim, seqs):
+    """The calls of several launches that hand their work on through a workspace, in two captured graphs with a workspace each, replayed
+    with new inputs, at the same time on two streams, with eager work between, against eager calls.  Within a graph the two gradients
+    share one workspace, and so do slots and trim."""
+    import random
+    rng = np.random.default_rng(n)
+    rows, vocab, most, page, max_pages = 500, 5001, 2, 8, 12
+    n_pages = seqs * max_pages
+    k = np.arange(seqs) % (most + 1)
+    total = int(k.sum())
+    start = random_cache(random.Random(1), seqs, page, max_pages, n_pages, full=0.03)
+
+    def buffers(seed):
+        torch.manual_seed(seed)
+        b = dict(ids=torch.zeros(n, dtype=torch.int32, device="cuda"), dy=torch.randn(n, dim, device="cuda").bfloat16(),
+                 grad=torch.zeros(rows, dim, device="cuda"), whole=torch.zeros(rows, dim, device="cuda"),
+                 work=torch.randint(0, 256, (capi.embed_grad_workspace(n, dim),), dtype=torch.uint8, device="cuda"),
+                 off=torch.zeros(seqs + 1, dtype=torch.int64, device="cuda"), slots=torch.zeros(n, dtype=torch.int64, device="cuda"),
+                 pos=torch.zeros(n, dtype=torch.int32, device="cuda"), keep=torch.zeros(seqs, dtype=torch.int32, device="cuda"),
+                 voff=torch.from_numpy(np.append(0, np.cumsum(k))).cuda(), draft=torch.zeros(total, dtype=torch.int32, device="cuda"),
+                 target=torch.softmax(torch.randn(total + seqs, vocab, device="cuda"), -1), q=torch.softmax(torch.randn(total, vocab, device="cuda"), -1),
+                 ua=torch.zeros(total, device="cuda"), ud=torch.zeros(seqs, device="cuda"),
+                 vout=torch.zeros(seqs, most + 1, dtype=torch.int32, device="cuda"), acc=torch.zeros(seqs, dtype=torch.int32, device="cuda"),
+                 vwork=torch.randint(0, 256, (capi.verify_workspace(seqs, vocab),), dtype=torch.uint8, device="cuda"))
+        b["cache"] = DeviceCache(torch, (*start, page, n_pages, max_pages))
+        return b
+
+    def run(b):
+        s = torch.cuda.current_stream().cuda_stream
+        for t, acc in ((b["grad"], True), (b["whole"], False)):
+            ctx.embed_grad(b["ids"].data_ptr(), n, b["dy"].data_ptr(), BF16, dim, rows, dim, t.data_ptr(), F32, dim, b["work"].data_ptr(),
+                           b["work"].numel(), 1.0, acc, b["off"].data_ptr() + 8 * seqs, s)
+        b["cache"].slots(ctx, b["off"], b["slots"], b["pos"], n, s)
+        b["cache"].trim(ctx, b["keep"], s)
+        ctx.verify_draft(b["draft"].data_ptr(), b["voff"].data_ptr(), seqs, total, most, b["target"].data_ptr(), F32, vocab, b["q"].data_ptr(), vocab,
+                         vocab, b["ua"].data_ptr(), b["ud"].data_ptr(), b["vout"].data_ptr(), b["acc"].data_ptr(), b["vwork"].data_ptr(),
+                         b["vwork"].numel(), s)
+
+    def inputs(bs):
+        off = np.minimum(np.append(0, np.cumsum(rng.integers(0, 2 * n // seqs + 1, seqs))), n)
+        keep = rng.choice([-1, 0, 30, 1000], seqs).astype(np.int32)
+        draft, ua, ud = rng.integers(0, vocab, total).astype(np.int32), rng.random(total).astype(np.float32), rng.random(seqs).astype(np.float32)
+        for b in bs:
+            for name, v in (("off", off), ("ids", _ids(np.random.default_rng(int(off[-1])), n, rows)), ("keep", keep), ("draft", draft), ("ua", ua), ("ud", ud)):
+                b[name].copy_(torch.from_numpy(v))
+
+    pairs = []
+    for seed in range(2):
+        a, b = buffers(seed), buffers(seed)
+        inputs((a, b))
+        g, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=s):
+            run(a)
+        pairs.append((g, s, a, b))
+    for turn in range(4):
+        for _, _, a, b in pairs:
+            inputs((a, b))
+        torch.cuda.synchronize()
+        for g, s, _, _ in pairs:
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for _, _, a, b in pairs:
+            run(b)
+            torch.cuda.synchronize()
+            for name in ("grad", "whole", "slots", "pos", "vout", "acc"):
+                assert torch.equal(a[name], b[name]), (turn, name)
+            assert a["cache"].state() == b["cache"].state() and int(a["cache"].status[0]) == int(b["cache"].status[0])
+            # (and the eager calls are right: the sums of whole gradients, the positions)
+            count = int(b["off"][seqs])
+            ids = b["ids"][:count].long()
+            there = (ids >= 0) & (ids < rows)
+            want = torch.zeros(rows, dim, device="cuda", dtype=torch.float64).index_add_(0, ids[there], b["dy"][:count][there].double())
+            size = torch.zeros(rows, dim, device="cuda", dtype=torch.float64).index_add_(0, ids[there], b["dy"][:count][there].double().abs())
+            m = torch.bincount(ids[there], minlength=rows).double()[:, None]
+            assert ((b["whole"].double() - want).abs() <= (m + 2) * U * size * (1 + (m + 2) * U) + U * want.abs() + 2.0 ** -149).all()
+
+
 def test_two_threads(ctx, torch):
     """Calls on one context from two threads, each on a stream and workspace of its own."""
     import threading
