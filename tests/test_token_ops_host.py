@@ -219,6 +219,20 @@ def test_error_texts_of_one_thread(lib, texts):
     assert text2() == b""
 
 
+def test_error_texts_of_many_contexts(lib, texts):
+    """A thread has the texts of as many contexts at once as one handle over several GPUs has."""
+    all_of = [texts() for _ in range(64)]
+    for turn in range(3):
+        for i, (_, leave, _, _) in enumerate(all_of):
+            leave(b"%d of " % i, b"%d" % turn)
+        assert [t() for _, _, t, _ in all_of] == [b"%d of %d" % (i, turn) for i in range(64)]
+    assign, leave, text, _ = texts()
+    leave(b"one more")
+    assert text() == b"one more" and sum(t() == b"" for _, _, t, _ in all_of) == 1
+    all_of[5][0](b"encode")
+    assert all_of[5][2]() == b"encode" and text() == b"one more"
+
+
 def test_error_texts_of_a_context_are_not_the_next_ones(lib, texts):
     """A context that comes to lie where one was destroyed has none of its texts."""
     for _ in range(200):

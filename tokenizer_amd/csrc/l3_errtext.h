@@ -6,8 +6,6 @@
 #include <mutex>
 #include <set>
 #include <string>
-#include <utility>
-#include <vector>
 
 namespace l3 {
 
@@ -24,10 +22,18 @@ class ErrText {
         static std::atomic<uint64_t> n{0};
         return ++n;
     }
-    typedef std::pair<uint64_t, const char*> Mine;
-    static std::vector<Mine>& mine() {    // this thread's texts, one for each context
-        thread_local std::vector<Mine> texts;
-        return texts;
+    // This thread's texts, one for each of the last kMine contexts that it has one of.  Without a destructor: a thread's (and the
+    // program's) last calls may come from the destructors of others.
+    static constexpr uint32_t kMine = 64;
+    struct Mine { uint64_t id; const char* text; };
+    struct AllMine { Mine of[kMine]; uint32_t next; };
+    static AllMine& mine() {
+        thread_local AllMine all;         // (zeros: no context has the id 0)
+        return all;
+    }
+    Mine* find_mine() const {
+        for (Mine& m : mine().of) if (m.id == id_) return &m;
+        return nullptr;
     }
     const char* keep(const std::string& text) {
         std::lock_guard<std::mutex> lk(mu_);
@@ -47,23 +53,19 @@ class ErrText {
             text = keep(std::string(what) + more);
         } catch (...) {
         }
-        try {
-            forget_this_threads();
-            mine().emplace_back(id_, text);
-        } catch (...) {
-        }
+        Mine* m = find_mine();
+        if (!m) m = &mine().of[mine().next++ % kMine];
+        *m = {id_, text};
     }
     void forget_this_threads() noexcept {
-        std::vector<Mine>& m = mine();
-        for (size_t i = 0; i < m.size(); i++)
-            if (m[i].first == id_) { m[i] = m.back(); m.pop_back(); return; }
+        if (Mine* m = find_mine()) m->id = 0;
     }
     // of the calls that hold the context's lock
     const char* shared() const { return now_.load(std::memory_order_acquire); }
     // the calling thread's own text, if it has one that is newer
     const char* c_str() const {
-        for (const Mine& m : mine()) if (m.first == id_) return m.second;
-        return shared();
+        const Mine* m = find_mine();
+        return m ? m->text : shared();
     }
 };
 
