@@ -10,7 +10,7 @@
 //   apply  adds up the workgroups' sums, decides who is served, writes table, slots, positions and the new state.
 // A step that one workgroup has through in the time of a launch does both in one (cache_slots_one_kernel, cache_trim_one_kernel).
 // All of it is bound by latency: chains of dependent loads, and launches.  Measured, us a call among others: 256 requests of one
-// token 5.4 (one launch; 4.4 on the GPU), 2,048 prompts with a million tokens 12.4 (4.0 + 9.0 on the GPU; 12.6 MB written, 2.5 us at a
+// token 5.4 (one launch; 4.4 on the GPU), 2,048 prompts with a million tokens 12.5 (4.0 + 9.1 on the GPU; 12.6 MB written, 2.5 us at a
 // copy's rate), a trim of 256 requests after drafts 5.1 (3.3 on the GPU), of 2,048 requests 8.3 (4.0 + 3.1).
 #include "l3_token_kernels.h"
 

@@ -56,10 +56,11 @@ __device__ __forceinline__ void store_cols(T* row, Cols c, uint32_t dim, typenam
 // ---- lookup -------------------------------------------------------------------------------------------------------
 // A thread has PER times as many neighbouring columns as make 16 bytes of the output, all loads in flight before the first store.
 // What is divided is a workgroup's first vector (once) and 32-bit offsets from it.  Bound by memory: 16,384 rows of 4,096 in 16 bits
-// take 31 us (186 MB of distinct rows read and rows written: 6.0 TB/s; a copy of 1 GiB reaches 5.1), 64 rows a launch (2.5 us).
+// take 35.7 us with inputs in turn (56 MB of distinct rows read and 134 MB written: 5.3 TB/s, and 29 us at the rates of reading alone, 5.7,
+// and of filling alone, 6.85), and 31 on the same inputs again, whose rows the last cache still has; 64 rows a launch (2.5 us).
 //
 // Outputs of 16 MiB and more (kEmbedOnce) pass the caches: stored the usual way, the output drives the table's rows out of them
-// (44 us instead of 32 at the size above; 16,384 rows of 2,048 in 32 bits 46 and 32).  A smaller output stays in them for the
+// (the same inputs again: 44 us instead of 32 at the size above; 16,384 rows of 2,048 in 32 bits 46 and 32).  A smaller output stays in them for the
 // kernel that reads it next.  One vector a thread is best up to 2^24 vectors (16,384 x 4,096: 32 us, with four 35), four above
 // (65,536 x 4,096: 169 and 144).
 constexpr int kEmbedThreads = 256;

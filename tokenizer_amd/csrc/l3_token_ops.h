@@ -1,6 +1,6 @@
 // l3_token_ops.h -- the operators on token ids that stand on either side of a model (l3_embed.hip, l3_cache.hip,
 // l3_verify.hip): their arguments, the checks the C ABI makes of them, the sizes of their workspaces and the arithmetic of
-// one request.  Plain C++ (the CPU test-suite compiles it too, l3_hosttest.cpp).
+// one request.  Plain C++ (the CPU test-suite compiles it too, l3_token_hosttest.cpp).
 #pragma once
 #include <stddef.h>
 #include <stdint.h>
@@ -14,7 +14,9 @@ L3_HD int dtype_size(int t) { return t == kF32 ? 4 : 2; }
 
 constexpr uint64_t kMaxCount = 0x7FFFFFFFull;    // ids, rows, tokens, pages: 31 bits
 constexpr uint64_t kMaxDim = 1ull << 24;
-constexpr uint64_t kMaxGradIds = 1ull << 24;     // ids sorted in one call: every tile adds up the counts of all tiles before it
+// Ids sorted in one call.  Every tile adds up the counts of all tiles before it, which is cheap up to about 2^20 ids and grows with
+// their square: 64 columns in 16 bits, us: 2^18 ids 85, 2^20 178, 2^22 709, 2^24 4,926.
+constexpr uint64_t kMaxGradIds = 1ull << 24;
 constexpr uint64_t kMaxGradRows = 1ull << 28;    // rows of a gradient: one workgroup for 32 of them
 constexpr uint64_t kMaxSeqs = 1ull << 20;
 constexpr uint64_t kMaxStride = kMaxCount;       // elements: (2^31 - 1) rows of (2^31 - 1) elements of 4 bytes stay inside 64 bits

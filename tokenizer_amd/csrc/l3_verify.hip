@@ -103,8 +103,10 @@ __device__ __forceinline__ double of_lane_f64(double v, int lane) {
 __device__ __forceinline__ double wave_sum_f64(double v) { return of_lane_f64(wave_iscan_f64(v), 63); }
 
 // Sums of kVerifyChunk entries: sums[i][chunk] = {rest, full}.  A workgroup per request and C chunks; that of chunk 0 leaves the
-// verdict, and all of the answer but the drawn token.  Bound by memory: 128 requests over 128,256 entries in 32 bits (131 MB) take
-// 23 us, 5.7 TB/s; one request 4 us, the chain offset -> token -> its probabilities -> row.  (Each workgroup works the verdict out for
+// verdict, and all of the answer but the drawn token.  128 requests over 128,256 entries in 32 bits take 22 us: 105 MB
+// (a row of p for each, one of q for the 60 % that had a token rejected; the others' q is not read), 4.8 TB/s, where a reading alone reaches
+// 5.7 -- memory, and the chain offset -> token -> its probabilities in front of the first wide load.  One request takes 4 us, that chain
+// and its row.  (Each workgroup works the verdict out for
 // itself: a launch of its own for it would cost as much as the chain.)  Where there are more workgroups than the GPU holds at once,
 // three chunks share that chain; one / three, us of both launches: 128 requests in 32 bits 26.0 / 25.1, in 16 bits 23.1 / 21.1, 1,024 in
 // 16 bits 136 / 102, 2,000 over 32,000 entries 88 / 75, but 64 requests in 32 bits 17.6 / 19.1.
